@@ -1270,7 +1270,7 @@ static_assert(FP8_ROWS <= ROUTE_ONE_ROWS, "the FP8 shared expert rides on the on
 hipError_t launch_route_group_rot(gfr_fast_experts* fx, hipStream_t s, const gfr_exl3_experts* w,
                                   const uint16_t* input, int input_stride, const float* logits, int rows, int routed,
                                   int topk, int* picks, float* weights, int* ids, int* count, int* members, int maxm,
-                                  const float* bias, float scale, const Fp8Shared* fp8) {
+                                  const float* bias, float scale, const Fp8Shared* fp8, const GateJob* gate) {
     const PrefillDims& d = fx->d;
     const int slots = topk + 1;
     const size_t lds = route_group_lds(rows, slots, routed + 1);
@@ -1287,8 +1287,10 @@ hipError_t launch_route_group_rot(gfr_fast_experts* fx, hipStream_t s, const gfr
     // 214.6, 20 rows 232.2 / 232.1, 32 rows 285.9 / 283.4, 48 rows 404 / 402; hidden 4096, top-8 of 288, FP8 shared
     // expert: 14 rows 84.1 / 84.4, 16 rows 96.3 / 96.3, 20 rows 122.9 / 119.1, 32 rows 155 / 148, 48 rows 193 / 179;
     // 220 rows (eager) 187 / 171, 680 / 638 and 416 / 336.
-    if (rows > ROUTE_ONE_ROWS && rows * topk > ROUTE_ONE_PICKS) {
-        hipError_t e = launch_route(s, logits, rows, routed, topk, routed, picks, weights, bias, scale);
+    // (the general gate is a launch of its own at any size)
+    if (gate || (rows > ROUTE_ONE_ROWS && rows * topk > ROUTE_ONE_PICKS)) {
+        hipError_t e = gate ? launch_gate(s, *gate)
+                            : launch_route(s, logits, rows, routed, topk, routed, picks, weights, bias, scale);
         if (e != hipSuccess) return e;
         group_small_rot_kernel<2><<<grid, WG, group_small_lds(rows, slots, routed + 1), s>>>(
             picks, rows, slots, routed + 1, ids, count, members, maxm, prefill_item_rows(fx, rows, w->bits), fx->ucnt,

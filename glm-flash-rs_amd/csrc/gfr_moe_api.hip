@@ -114,6 +114,10 @@ struct gfr_moe {
     int launches;              // measurement: rows == 1 issues only the first `launches` launches (0: all)
     gfr_shared_fp8* sfp8;      // shared_exl3 = 0: the FP8 shared expert's engine and output [max_rows][hidden]
     float* shared_out;
+    bool has_gate;             // the general gate (gfr_moe_set_gate) instead of route_bias / route_scale
+    gfr_gate gate;
+    uint16_t* bf16_act;        // shared_exl3 = 0: the bf16 shared expert's activations [max_rows][inter] and output
+    float* bf16_out;           // (gfr_moe_run_bf16)
 };
 
 struct gfr_shared_fp8 {
@@ -123,6 +127,37 @@ struct gfr_shared_fp8 {
     rocblas_handle blas;   // the prefill form's GEMMs, with a workspace of its own (no allocation at run)
     void* blas_ws;
 };
+
+namespace {
+// The general gate's checks, and its launch's arguments
+bool known_type(int t) { return t == GFR_BF16 || t == GFR_F16 || t == GFR_F32; }
+size_t type_bytes(int t) { return t == GFR_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+int check_gate(const gfr_gate* g, int routed, int topk) {
+    if (!g) return fail(GFR_EINVAL, "null gate");
+    if (routed <= 0 || routed > 1024) return fail(GFR_EINVAL, "gate routed %d outside 1..1024", routed);
+    if (g->score != GFR_SCORE_SOFTMAX && g->score != GFR_SCORE_SIGMOID) return fail(GFR_EINVAL, "gate score %d", g->score);
+    if (g->groups <= 0 || g->groups > 64 || routed % g->groups)
+        return fail(GFR_EINVAL, "gate groups %d: 1..64, a divisor of routed %d", g->groups, routed);
+    if (g->kept_groups <= 0 || g->kept_groups > g->groups)
+        return fail(GFR_EINVAL, "gate kept groups %d outside 1..%d", g->kept_groups, g->groups);
+    if (g->group_score != GFR_GROUP_MAX && g->group_score != GFR_GROUP_TOP2)
+        return fail(GFR_EINVAL, "gate group score %d", g->group_score);
+    if (topk <= 0 || topk > 31 || topk > g->kept_groups * (routed / g->groups))
+        return fail(GFR_EINVAL, "gate topk %d: 1..31, at most the %d experts of the kept groups", topk,
+                    g->kept_groups * (routed / g->groups));
+    if (!(g->scale > 0.f) || g->scale > 3.4e38f)
+        return fail(GFR_EINVAL, "gate scale %g must be positive and finite", (double)g->scale);
+    if (!aligned(g->bias, 4)) return fail(GFR_EINVAL, "gate bias must be 4-byte aligned");
+    return 0;
+}
+gfr::GateJob gate_job(const gfr_gate& g, const void* logits, int type, int64_t stride, int rows, int routed, int topk,
+                      int shared, int32_t* picks, float* weights) {
+    return {logits,      type,     stride, rows,    routed, topk,  topk + (shared ? 1 : 0), g.score == GFR_SCORE_SOFTMAX,
+            g.group_score == GFR_GROUP_TOP2, g.renormalise != 0, g.groups, g.kept_groups, g.scale, g.bias, picks, weights,
+            0, 0, 0};
+}
+}  // namespace
 
 extern "C" {
 
@@ -350,6 +385,73 @@ int gfr_route_topk_biased(hipStream_t stream, const float* logits, const float* 
     return 0;
 }
 
+// ---- the general gate -------------------------------------------------------------------------------------------
+int gfr_route_gate(hipStream_t stream, const void* logits, int logits_type, int64_t logits_stride, int rows, int routed,
+                   int topk, const gfr_gate* gate, int shared, int32_t* picks, float* weights) {
+    if (!logits || !picks || !weights) return fail(GFR_EINVAL, "null argument");
+    int rc = check_gate(gate, routed, topk);
+    if (rc) return rc;
+    if (rows <= 0) return fail(GFR_EINVAL, "gate rows %d", rows);
+    if (!known_type(logits_type)) return fail(GFR_EINVAL, "gate logits type %d", logits_type);
+    if (logits_stride < routed) return fail(GFR_EINVAL, "gate logits stride %lld < routed %d", (long long)logits_stride, routed);
+    if (shared != 0 && shared != 1) return fail(GFR_EINVAL, "gate shared %d: 0 or 1", shared);
+    if (!aligned(logits, type_bytes(logits_type)) || !aligned(picks, 4) || !aligned(weights, 4))
+        return fail(GFR_EINVAL, "gate tensors must be aligned to their elements");
+    hipError_t e = gfr::launch_gate(stream, gate_job(*gate, logits, logits_type, logits_stride, rows, routed, topk, shared,
+                                                     picks, weights));
+    if (e != hipSuccess) return hip_fail(e, "gate");
+    return 0;
+}
+
+int gfr_moe_set_gate(gfr_moe* m, const gfr_gate* gate) {
+    if (!m) return fail(GFR_EINVAL, "null moe");
+    if (gate) {
+        int rc = check_gate(gate, m->routed, m->topk);
+        if (rc) return rc;
+        m->gate = *gate;
+    }
+    m->has_gate = gate != nullptr;
+    return 0;
+}
+
+// ---- 16-bit products ----------------------------------------------------------------------------------------------
+int gfr_dense_run(hipStream_t stream, const gfr_dense* d) {
+    if (!d || !d->x || !d->w || !d->out) return fail(GFR_EINVAL, "dense: null argument");
+    const int limit = 1 << 24;
+    if (d->rows <= 0 || d->n <= 0 || d->k <= 0 || d->rows > limit || d->n > limit || d->k > limit)
+        return fail(GFR_EINVAL, "dense: rows %d, n %d, k %d outside 1..%d", d->rows, d->n, d->k, limit);
+    if (d->type != GFR_BF16 && d->type != GFR_F16) return fail(GFR_EINVAL, "dense: type %d is not bf16 or fp16", d->type);
+    const auto suits = [&](int t) { return t == d->type || t == GFR_F32; };
+    if (!suits(d->out_type) || (d->bias && !suits(d->bias_type)) || (d->residual && !suits(d->residual_type)))
+        return fail(GFR_EINVAL, "dense: out %d, bias %d and residual %d must have x's type or fp32", d->out_type,
+                    d->bias_type, d->residual_type);
+    if (d->gated != 0 && d->gated != 1) return fail(GFR_EINVAL, "dense: gated %d: 0 or 1", d->gated);
+    if (d->act < GFR_ACT_NONE || d->act > GFR_ACT_SILU) return fail(GFR_EINVAL, "dense: activation %d", d->act);
+    if (!(d->limit >= 0.f)) return fail(GFR_EINVAL, "dense: limit %g must not be negative", (double)d->limit);
+    if (d->limit > 0.f && !d->gated) return fail(GFR_EINVAL, "dense: a limit is the gated form's");
+    if (d->x_stride < d->k || d->w_stride < d->k)
+        return fail(GFR_EINVAL, "dense: strides of x %lld and w %lld below k %d", (long long)d->x_stride,
+                    (long long)d->w_stride, d->k);
+    if (d->out_stride < d->n || (d->residual && d->residual_stride < d->n))
+        return fail(GFR_EINVAL, "dense: strides of out %lld and residual %lld below n %d", (long long)d->out_stride,
+                    (long long)d->residual_stride, d->n);
+    const int64_t far = (int64_t)1 << 31;
+    if (d->x_stride > far || d->w_stride > far || d->out_stride > far || (d->residual && d->residual_stride > far))
+        return fail(GFR_EINVAL, "dense: a stride above 2^31");
+    if (!aligned(d->x, 2) || !aligned(d->w, 2) || !aligned(d->out, type_bytes(d->out_type)) ||
+        (d->bias && !aligned(d->bias, type_bytes(d->bias_type))) ||
+        (d->residual && !aligned(d->residual, type_bytes(d->residual_type))))
+        return fail(GFR_EINVAL, "dense: tensors must be aligned to their elements");
+    if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 31))
+        return fail(GFR_EINVAL, "dense: %d rows of %d columns are too many tiles for a launch", d->rows, d->n);
+    const gfr::DenseJob job{d->x, d->w, d->bias, d->residual, d->out, d->x_stride, d->w_stride, d->residual_stride,
+                            d->out_stride, d->rows, d->n, d->k, d->type, d->bias_type, d->residual_type, d->out_type,
+                            d->act, d->limit > 0.f ? d->limit : __builtin_inff(), d->gated != 0, 0, false};
+    hipError_t e = gfr::launch_dense(stream, job);
+    if (e != hipSuccess) return hip_fail(e, "dense");
+    return 0;
+}
+
 // ---- debug rotation ---------------------------------------------------------------------------------------------
 int gfr_exl3_rotate(hipStream_t stream, const uint16_t* x, int x_stride, int x_f16, const int32_t* expert,
                     const uint16_t* suh, int k, int rows, uint16_t* out) {
@@ -444,7 +546,7 @@ int gfr_moe_create_shared(gfr_moe** out, int hidden, int inter, int routed, int 
     gfr_moe* m = new gfr_moe{hidden, inter, routed, topk, topk + 1, max_rows,
                              MOE_DECODE_ROWS < max_rows ? MOE_DECODE_ROWS : max_rows,
                              nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1.f,
-                             shared_exl3 ? 1 : 0, nullptr, 0, nullptr, nullptr};
+                             shared_exl3 ? 1 : 0, nullptr, 0, nullptr, nullptr, false, {}, nullptr, nullptr};
     const int exl3_slots = shared_exl3 ? topk + 1 : topk, experts = shared_exl3 ? routed + 1 : routed;
     m->route_bias = nullptr;   // the softmax gate until gfr_moe_set_router
     m->route_scale = 1.f;
@@ -461,6 +563,16 @@ int gfr_moe_create_shared(gfr_moe** out, int hidden, int inter, int routed, int 
     if (!shared_exl3 && hidden % 512 == 0 &&
         ((rc = gfr_shared_fp8_create(&m->sfp8, hidden, inter, max_rows)) ||
          (rc = alloc_zero(&m->shared_out, (size_t)max_rows * hidden, "moe shared output")))) {
+        gfr_moe_destroy(m);
+        return rc;
+    }
+    // the bf16 shared expert's activations and output: the FP8 one's buffers where the layer has them (one shared expert
+    // a run)
+    if (!shared_exl3 && m->sfp8) {
+        m->bf16_act = m->sfp8->act;
+        m->bf16_out = m->shared_out;
+    } else if (!shared_exl3 && ((rc = alloc_zero(&m->bf16_act, (size_t)max_rows * inter, "moe shared activations")) ||
+                                (rc = alloc_zero(&m->bf16_out, (size_t)max_rows * hidden, "moe shared output")))) {
         gfr_moe_destroy(m);
         return rc;
     }
@@ -506,8 +618,18 @@ int moe_run(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uin
                     shared_stride);
     if (shared_ready && !shared) return fail(GFR_EINVAL, "a shared-ready event without a shared output");
     hipError_t e;
+    const gfr::GateJob gate = m->has_gate ? gate_job(m->gate, logits, GFR_F32, m->routed, rows, m->routed, m->topk, 1,
+                                                     m->picks, m->weights)
+                                          : gfr::GateJob{};
     if (rows <= m->decode_rows) {
         gfr_grouping* g = m->group_dec;
+        if (m->has_gate) {
+            // five launches: gate, group, gate/up (+ rotation), down (+ gate/up epilogue), down epilogue (+ combine)
+            if ((e = gfr::launch_gate(stream, gate)) != hipSuccess) return hip_fail(e, "gate");
+            if ((rc = gfr_grouping_run(g, stream, m->picks, rows))) return rc;
+            return experts_run(m->dec, stream, w, input, m->hidden, m->picks, g->ids, g->count, g->members, rows,
+                               g->max_rows, m->weights, m->out, nullptr, shared, shared_stride, 0, shared_ready);
+        }
         if (rows == 1) {
             // three launches: gate/up (+ route, rotation), down (+ gate/up epilogue), down epilogue (+ combine)
             const gfr::RouteOne r{logits, m->route_bias, m->route_scale, m->routed, m->picks, m->weights, g->ids,
@@ -528,12 +650,13 @@ int moe_run(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uin
     bool planned = false, rotated = false;
     if ((e = gfr::launch_route_group_rot(m->pre, stream, w, input, m->hidden, logits, rows, m->routed, m->topk,
                                          m->picks, m->weights, g->ids, g->count, g->members, g->max_rows,
-                                         m->route_bias, m->route_scale, fp8)) == hipSuccess) {
+                                         m->route_bias, m->route_scale, fp8, m->has_gate ? &gate : nullptr)) ==
+        hipSuccess) {
         // route + group + item plan and the input rotation in one launch
         planned = rotated = true;
     } else if (e != hipErrorNotSupported) {
         return hip_fail(e, "route + group + rotation");
-    } else if (rows <= gfr::GROUP_SMALL_ROWS && g->experts <= 1024 &&
+    } else if (!m->has_gate && rows <= gfr::GROUP_SMALL_ROWS && g->experts <= 1024 &&
         gfr::route_group_lds(rows, m->slots, g->experts) <= gfr::GROUP_LDS_MAX) {
         // route + group + the prefill engine's item plan in one launch (the same router, grouping and plan as the
         // separate launches below)
@@ -546,8 +669,9 @@ int moe_run(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uin
             return hip_fail(e, "route + group");
         planned = true;
     } else {
-        if ((e = gfr::launch_route(stream, logits, rows, m->routed, m->topk, m->routed, m->picks, m->weights,
-                                   m->route_bias, m->route_scale)) != hipSuccess)
+        if ((e = m->has_gate ? gfr::launch_gate(stream, gate)
+                             : gfr::launch_route(stream, logits, rows, m->routed, m->topk, m->routed, m->picks,
+                                                 m->weights, m->route_bias, m->route_scale)) != hipSuccess)
             return hip_fail(e, "route");
         if (rows <= gfr::GROUP_SMALL_ROWS) {
             if ((rc = gfr_grouping_run(g, stream, m->picks, rows))) return rc;
@@ -821,7 +945,7 @@ int gfr_shared_fp8_destroy(gfr_shared_fp8* sh) {
 
 namespace {
 // The layer with its FP8 shared expert. A one-token window whose launches have the shared slot's workgroups (the
-// grid's last unit exists: the weights hold at least `slots` experts) runs the shared expert inside the gate/up and
+// grid's last unit exists: the weights hold at least `slots` experts; not under gfr_moe_set_gate) runs the shared expert inside the gate/up and
 // down launches (three launches in all), a prefill-engine window of at most 16 rows inside its route + group + rotation
 // and gate/up epilogue launches; other windows run its two launches first.
 int moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
@@ -830,7 +954,8 @@ int moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const
     if (!w || !input) return fail(GFR_EINVAL, "null weights or input");
     if (!al16(input)) return fail(GFR_EINVAL, "input rows must be 16-byte aligned");
     // (the weights' other checks follow in moe_run, before any launch)
-    const bool fused = rows <= m->decode_rows
+    const bool fused = m->has_gate ? false
+                       : rows <= m->decode_rows
                            ? rows == 1 && w->experts >= m->slots && gfr::gemv_gateup_splits(m->hidden) <= 16
                            : w->hidden == m->hidden && w->inter == m->inter && gfr::prefill_fits(m->pre, w, rows) &&
                                  gfr::prefill_takes_fp8(m->pre, w, rows, m->routed, m->topk);
@@ -861,6 +986,59 @@ int gfr_moe_run_router_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_expert
     if ((rc = gfr_router_logits(stream, input, m->hidden, router_weight, m->hidden, m->routed, rows, m->logits)))
         return rc;
     return moe_run_fp8(m, stream, w, input, m->logits, sw, rows);
+}
+
+// ---- the bf16 shared expert -------------------------------------------------------------------------------------
+namespace {
+int moe_bf16_ready(gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input, const gfr_bf16_shared_weights* sw,
+                   int rows) {
+    if (!m) return fail(GFR_EINVAL, "null moe");
+    if (m->shared_exl3) return fail(GFR_EINVAL, "the layer's shared expert is EXL3: no bf16 shared expert");
+    if (!sw || !sw->gu || !sw->down) return fail(GFR_EINVAL, "null bf16 shared weights");
+    if (sw->hidden != m->hidden || sw->inter <= 0 || sw->inter > m->inter)
+        return fail(GFR_EINVAL, "bf16 shared weights %dx%d: the layer's hidden %d, inter up to %d", sw->hidden, sw->inter,
+                    m->hidden, m->inter);
+    if (!(sw->limit >= 0.f)) return fail(GFR_EINVAL, "bf16 shared limit %g must not be negative", (double)sw->limit);
+    if (!input) return fail(GFR_EINVAL, "null input");
+    if (rows <= 0 || rows > m->max_rows) return fail(GFR_EINVAL, "rows %d outside 1..%d", rows, m->max_rows);
+    return check_weights(w, m->hidden, m->inter);
+}
+int moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
+                 const float* logits, const gfr_bf16_shared_weights* sw, int rows) {
+    const int H = m->hidden, I = sw->inter;
+    gfr_dense up{};
+    up.rows = rows, up.n = I, up.k = H;
+    up.x = input, up.x_stride = H;
+    up.w = sw->gu, up.w_stride = H;
+    up.gated = 1, up.act = GFR_ACT_SILU, up.limit = sw->limit;
+    up.out = m->bf16_act, up.out_stride = I, up.out_type = GFR_BF16;
+    gfr_dense down{};
+    down.rows = rows, down.n = H, down.k = I;
+    down.x = m->bf16_act, down.x_stride = I;
+    down.w = sw->down, down.w_stride = I;
+    down.out = m->bf16_out, down.out_stride = H, down.out_type = GFR_F32;
+    int rc;
+    if ((rc = gfr_dense_run(stream, &up)) || (rc = gfr_dense_run(stream, &down))) return rc;
+    return moe_run(m, stream, w, input, logits, m->bf16_out, H, rows);
+}
+}  // namespace
+
+int gfr_moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
+                     const float* logits, const gfr_bf16_shared_weights* sw, int rows) {
+    int rc = moe_bf16_ready(m, w, input, sw, rows);
+    if (rc) return rc;
+    if (!logits) return fail(GFR_EINVAL, "null logits");
+    return moe_run_bf16(m, stream, w, input, logits, sw, rows);
+}
+
+int gfr_moe_run_router_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
+                            const uint16_t* router_weight, const gfr_bf16_shared_weights* sw, int rows) {
+    int rc = moe_bf16_ready(m, w, input, sw, rows);
+    if (rc) return rc;
+    if (!router_weight) return fail(GFR_EINVAL, "null router weight");
+    if ((rc = gfr_router_logits(stream, input, m->hidden, router_weight, m->hidden, m->routed, rows, m->logits)))
+        return rc;
+    return moe_run_bf16(m, stream, w, input, m->logits, sw, rows);
 }
 
 float* gfr_moe_shared_output(const gfr_moe* m) { return m ? m->shared_out : nullptr; }
@@ -910,6 +1088,8 @@ int gfr_moe_destroy(gfr_moe* m) {
     gfr_grouping_destroy(m->group_pre);
     gfr_experts_destroy(m->dec);
     gfr_fast_experts_destroy(m->pre);
+    const bool own_bf16 = !m->sfp8 || m->bf16_act != m->sfp8->act;
+    if (own_bf16) free_all({m->bf16_act, m->bf16_out});
     gfr_shared_fp8_destroy(m->sfp8);
     free_all({m->weights, m->picks, m->out, m->logits, m->shared_out});
     delete m;

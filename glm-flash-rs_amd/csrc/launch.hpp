@@ -118,6 +118,49 @@ int router_logits_max_hidden();
 hipError_t launch_router_logits(hipStream_t s, const uint16_t* x, int x_stride, const uint16_t* W, int D, int E,
                                 int rows, float* logits);
 
+// Element types of the general gate and the 16-bit products (the values of GFR_BF16, GFR_F16, GFR_F32)
+constexpr int TYPE_BF16 = 0, TYPE_F16 = 1, TYPE_F32 = 2;
+// Activations of the 16-bit products (GFR_ACT_*)
+constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_SILU = 4;
+
+// gate.hip
+// The general router gate over rows of logits [rows][stride]: picks / weights [rows][slots], slots = topk or topk + 1
+// (the shared expert last). routed <= 1024, a multiple of groups; groups <= 64; slots <= 32; topk <= kept * routed / groups.
+struct GateJob {
+    const void* logits;
+    int type;
+    int64_t stride;
+    int rows, routed, topk, slots;
+    bool softmax, top2, renorm;
+    int groups, kept;
+    float scale;
+    const float* bias;
+    int* picks;
+    float* weights;
+    int lpg, per_group, per_lane;   // set by launch_gate: lanes a group, experts a group, experts a lane
+};
+hipError_t launch_gate(hipStream_t s, GateJob g);
+
+// dense.hip
+// out[r][c] = act(x[r] . w[c] + bias[c]) + residual[r][c]; gated: act(min(g, limit)) * clamp(u, -limit, limit) +
+// residual with g = x . w[c] + bias[c], u = x . w[n + c] + bias[n + c]. x, w bf16 or fp16; sums and epilogue in fp32.
+struct DenseJob {
+    const uint16_t* x;
+    const uint16_t* w;
+    const void* bias;
+    const void* residual;
+    void* out;
+    int64_t x_stride, w_stride, residual_stride, out_stride;
+    int rows, n, k;
+    int type, bias_type, residual_type, out_type;
+    int act;
+    float limit;                    // infinity: none
+    bool gated;
+    int n_tiles;                    // set by launch_dense: tiles along the columns
+    bool vector;                    // set by launch_dense: residual and out are read and written four columns at a time (residual, out)
+};
+hipError_t launch_dense(hipStream_t s, DenseJob d);
+
 // shared_fp8.hip
 // The reference's FP8 shared expert (moe.rs:132-167) for rows [rows][x_stride] bf16: gate/up (8 K slices, bf16 gu
 // [rows][2 inter], limited SwiGLU -> act [rows][inter] bf16), then down -> out [rows][out_stride] fp32. hidden a

@@ -39,7 +39,8 @@ hipError_t launch_group_large_rot(gfr_fast_experts* fx, hipStream_t s, const gfr
 hipError_t launch_route_group_rot(gfr_fast_experts* fx, hipStream_t s, const gfr_exl3_experts* w,
                                   const uint16_t* input, int input_stride, const float* logits, int rows, int routed,
                                   int topk, int* picks, float* weights, int* ids, int* count, int* members, int maxm,
-                                  const float* bias, float scale, const Fp8Shared* fp8 = nullptr);
+                                  const float* bias, float scale, const Fp8Shared* fp8 = nullptr,
+                                  const GateJob* gate = nullptr);   // the rows' gate instead (not with fp8)
 // The layer's FP8 shared expert can ride on the window's launches (launch_route_group_rot's fp8 and prefill_run's: at
 // most 16 rows, the split-K form).
 bool prefill_takes_fp8(const gfr_fast_experts* fx, const gfr_exl3_experts* w, int rows, int routed, int topk);

@@ -104,6 +104,11 @@ def _load() -> ctypes.CDLL:
         "gfr_prefetch_capturing": ([P, ctypes.POINTER(I)], I),
         "gfr_prefetch_segments": ([P, I, I, P], I),
         "gfr_prefetch_experts": ([P, P, I, P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, I, P], I),
+        "gfr_route_gate": ([P, P, I, ctypes.c_int64, I, I, I, ctypes.POINTER(_GateStruct), I, P, P], I),
+        "gfr_moe_set_gate": ([VP, ctypes.POINTER(_GateStruct)], I),
+        "gfr_dense_run": ([P, ctypes.POINTER(_DenseStruct)], I),
+        "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
+        "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_tensor_extent": ([ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64), I, I,
                                ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)], I),
     }
@@ -307,6 +312,75 @@ class _Fp8Struct(ctypes.Structure):
         (n, ctypes.c_void_p) for n in ("gu", "gu_scale", "down", "down_scale", "gu_bf16", "down_bf16")]
 
 
+@dataclass
+class Bf16SharedWeights:
+    """An unquantised shared expert: gu [2 inter, hidden] (gate rows, then up rows) and down [hidden, inter] bf16,
+    contiguous on the GPU; limit: the SwiGLU's bound (None: none)."""
+
+    gu: torch.Tensor
+    down: torch.Tensor
+    limit: float = 10.0
+
+    def struct(self) -> "_Bf16Struct":
+        gu, down = self.gu, self.down
+        H, I = gu.shape[1], gu.shape[0] // 2
+        if gu.shape != (2 * I, H) or down.shape != (H, I) or gu.dtype != torch.bfloat16 or down.dtype != torch.bfloat16:
+            raise ValueError(f"gu {tuple(gu.shape)} {gu.dtype}, down {tuple(down.shape)} {down.dtype}: want bf16 "
+                             "[2 inter, hidden] and [hidden, inter]")
+        if not (gu.is_contiguous() and down.is_contiguous() and gu.is_cuda and down.is_cuda):
+            raise ValueError("gu, down: want contiguous tensors on the GPU")
+        return _Bf16Struct(H, I, gu.data_ptr(), down.data_ptr(), self.limit or 0.0)
+
+
+class _Bf16Struct(ctypes.Structure):
+    _fields_ = [("hidden", ctypes.c_int), ("inter", ctypes.c_int), ("gu", ctypes.c_void_p), ("down", ctypes.c_void_p),
+                ("limit", ctypes.c_float)]
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORES = {"max": 0, "top2": 1}
+
+
+@dataclass
+class Gate:
+    """The general router gate (gfr_gate): score "softmax" (over all experts) or "sigmoid"; bias [routed] fp32 added to
+    the scores for the choice only; groups of neighbouring experts of which kept_groups (None: all) stay, by their
+    "max" or the sum of their "top2"; weights renormalised over the picks or kept, times scale."""
+
+    score: str = "sigmoid"
+    bias: torch.Tensor = None
+    groups: int = 1
+    kept_groups: int = None
+    group_score: str = "top2"
+    renormalise: bool = True
+    scale: float = 1.0
+
+    def struct(self, routed: int) -> "_GateStruct":
+        bias = self.bias
+        if bias is not None and not (bias.dtype is torch.float32 and bias.shape == (routed,) and bias.is_contiguous()
+                                     and bias.is_cuda):
+            raise ValueError(f"gate bias: {tuple(bias.shape)} {bias.dtype}, want ({routed},) float32 contiguous on GPU")
+        if self.score not in _SCORES or self.group_score not in _GROUP_SCORES:
+            raise ValueError(f"gate: score {self.score!r} of {list(_SCORES)}, group score {self.group_score!r} of "
+                             f"{list(_GROUP_SCORES)}")
+        return _GateStruct(_SCORES[self.score], self.groups, self.groups if self.kept_groups is None else self.kept_groups,
+                           _GROUP_SCORES[self.group_score], bool(self.renormalise), self.scale, _ptr(bias))
+
+
+class _GateStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("score", "groups", "kept_groups", "group_score", "renormalise")] + [
+        ("scale", ctypes.c_float), ("bias", ctypes.c_void_p)]
+
+
+class _DenseStruct(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("type", ctypes.c_int),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("w", ctypes.c_void_p),
+                ("w_stride", ctypes.c_int64), ("gated", ctypes.c_int), ("act", ctypes.c_int),
+                ("limit", ctypes.c_float), ("bias_type", ctypes.c_int), ("bias", ctypes.c_void_p),
+                ("residual_type", ctypes.c_int), ("out_type", ctypes.c_int), ("residual", ctypes.c_void_p),
+                ("residual_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64)]
+
+
 class _Engine:
     _destroy = None
 
@@ -462,6 +536,26 @@ class Moe(_Engine):
         ws, ss = w.struct(), sw.struct()
         _check(lib().gfr_moe_run_router_fp8(self._h, _stream(stream), ctypes.byref(ws), _ptr(input),
                                             _ptr(router_weight), ctypes.byref(ss), rows))
+
+    def set_gate(self, gate: "Gate" = None):
+        """The general gate (gfr_moe_set_gate) instead of set_router's, in a launch of its own; None: back to that one.
+        The gate's bias must outlive the runs (this object holds it)."""
+        self._gate = gate
+        _check(lib().gfr_moe_set_gate(self._h, None if gate is None else ctypes.byref(gate.struct(self.routed))))
+
+    def run_bf16(self, w: Exl3Experts, input: torch.Tensor, logits: torch.Tensor, sw: Bf16SharedWeights, rows: int,
+                 stream=None):
+        """The layer with an unquantised shared expert (a layer made with shared_exl3=False): gfr_moe_run_bf16."""
+        ws, ss = w.struct(), sw.struct()
+        _check(lib().gfr_moe_run_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input), _ptr(logits),
+                                      ctypes.byref(ss), rows))
+
+    def run_router_bf16(self, w: Exl3Experts, input: torch.Tensor, router_weight: torch.Tensor, sw: Bf16SharedWeights,
+                        rows: int, stream=None):
+        """run_bf16 with the router logits computed from the hidden rows first (router_weight [routed, hidden])."""
+        ws, ss = w.struct(), sw.struct()
+        _check(lib().gfr_moe_run_router_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input),
+                                             _ptr(router_weight), ctypes.byref(ss), rows))
 
     @property
     def shared_output(self) -> torch.Tensor:
@@ -753,6 +847,91 @@ def route_biased(logits: torch.Tensor, bias: torch.Tensor, topk: int, scale: flo
     _check(lib().gfr_route_topk_biased(_stream(stream), _ptr(logits), _ptr(bias), float(scale), rows, routed, topk,
                                        _ptr(picks), _ptr(weights)))
     return picks, weights
+
+
+_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _here(*tensors):
+    """The tensors' device has to be the current one: a launch goes to the current device's stream."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"tensor on {t.device}, the current device is cuda:{here}")
+
+
+def _empty(shape, dtype, device, stream):
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):       # memory of the stream it is written on
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _row_stride(t) -> int:
+    """Elements between rows of a [rows, columns] tensor whose columns are neighbours."""
+    rows, cols = t.shape
+    stride, step = t.stride()
+    if step != 1 and cols > 1:
+        raise ValueError(f"tensor {tuple(t.shape)} strides {tuple(t.stride())}: columns must be neighbours")
+    return stride if rows > 1 else max(stride, cols)
+
+
+def route_gate(logits: torch.Tensor, gate: Gate, topk: int, shared: bool = True, stream=None):
+    """gfr_route_gate: (picks [rows, topk + 1] int32, weights [rows, topk + 1] fp32) of logits [rows, routed] (fp32, bf16
+    or fp16), the shared expert's id = routed last; shared=False: [rows, topk] without it."""
+    rows, routed = logits.shape
+    if logits.dtype not in _TYPE:
+        raise ValueError(f"gate logits {logits.dtype}: fp32, bf16 or fp16")
+    _here(logits, gate.bias)
+    slots = topk + 1 if shared else topk
+    st = gate.struct(routed)
+    picks = _empty((rows, slots), torch.int32, logits.device, stream)
+    weights = _empty((rows, slots), torch.float32, logits.device, stream)
+    _check(lib().gfr_route_gate(_stream(stream), logits.data_ptr(), _TYPE[logits.dtype], _row_stride(logits), rows, routed,
+                                topk, ctypes.byref(st), int(shared), picks.data_ptr(), weights.data_ptr()))
+    return picks, weights
+
+
+def _dense(x, w, n, gated, bias, activation, limit, residual, out, out_dtype, stream):
+    if w.dtype is not x.dtype or x.shape[1] != w.shape[1] or activation not in _ACTIVATIONS:
+        raise ValueError(f"x {tuple(x.shape)} {x.dtype}, w {tuple(w.shape)} {w.dtype}, activation {activation!r}: want the "
+                         f"same 16-bit type and columns, an activation of {[a for a in _ACTIVATIONS if a]}")
+    rows, k = x.shape
+    _here(x, w, bias, residual, out)
+    if bias is not None and (bias.shape != (w.shape[0],) or not bias.is_contiguous()):
+        raise ValueError(f"bias {tuple(bias.shape)}: want ({w.shape[0]},) contiguous")
+    if out is None:
+        out = _empty((rows, n), x.dtype if out_dtype is None else out_dtype, x.device, stream)
+    elif out.shape != (rows, n) or (out_dtype is not None and out.dtype is not out_dtype):
+        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: want ({rows}, {n})")
+    if residual is not None and residual.shape != (rows, n):
+        raise ValueError(f"residual {tuple(residual.shape)}: want ({rows}, {n})")
+    types = _TYPE
+    st = _DenseStruct(rows, n, k, types.get(x.dtype, -1), x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w),
+                      gated, _ACTIVATIONS[activation], limit or 0.0,
+                      0 if bias is None else types.get(bias.dtype, -1), _ptr(bias),
+                      0 if residual is None else types.get(residual.dtype, -1), types.get(out.dtype, -1), _ptr(residual),
+                      0 if residual is None else _row_stride(residual), out.data_ptr(), _row_stride(out))
+    _check(lib().gfr_dense_run(_stream(stream), ctypes.byref(st)))
+    return out
+
+
+def dense(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, activation: str = None,
+          residual: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
+    """gfr_dense_run: act(x w^T + bias) + residual for x [rows, k] and w [n, k] of one 16-bit type; bias [n], residual and
+    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself."""
+    return _dense(x, w, w.shape[0], 0, bias, activation, 0.0, residual, out, out_dtype, stream)
+
+
+def dense_gated(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, activation: str = "silu",
+                limit: float = None, residual: torch.Tensor = None, out: torch.Tensor = None,
+                out_dtype: torch.dtype = None, stream=None):
+    """gfr_dense_run, gated: act(min(g, limit)) * clamp(u, -limit, limit) + residual, g and u the halves of x w^T + bias
+    for w [2 n, k] (gate rows, then up rows); limit None or 0: none. Otherwise as dense."""
+    if w.shape[0] % 2:
+        raise ValueError(f"w {tuple(w.shape)}: want an even number of rows, the gate's and the up matrix's")
+    return _dense(x, w, w.shape[0] // 2, 1, bias, activation, limit, residual, out, out_dtype, stream)
 
 
 def rotate(x: torch.Tensor, expert: torch.Tensor, suh: torch.Tensor, stream=None) -> torch.Tensor:

@@ -158,9 +158,21 @@ int gfr_moe_token_static(hipStream_t stream, const gfr_exl3_experts* w, int rout
 /* The layer's router gate: bias == NULL (default) the softmax gate of gfr_route_topk; else GLM's gate of
  * gfr_route_topk_biased with this bias [routed] (device, fp32; must outlive the runs) and scale (2.5 for GLM). */
 int gfr_moe_set_router(gfr_moe* m, const float* bias, float scale);
+/* The layer's gate: the general one of gfr_route_gate (copied; its bias must outlive the runs) in a launch of its own
+ * before the grouping, until gate = NULL goes back to the gate of gfr_moe_set_router. */
+typedef struct gfr_gate {
+    int score;          /* GFR_SCORE_* */
+    int groups;
+    int kept_groups;
+    int group_score;    /* GFR_GROUP_* */
+    int renormalise;
+    float scale;
+    const float* bias;  /* [routed] or NULL */
+} gfr_gate;
+int gfr_moe_set_gate(gfr_moe* m, const gfr_gate* gate);
 /* Measurement aid, no reference counterpart: a one-row run issues only its first `launches` launches (1: the gate/up
  * GEMV with the router; 2: and the down GEMV; 0 or 3: all three), so that a caller can time each launch inside the
- * layer's own sequence. Outputs of a shortened run are incomplete. */
+ * layer's own sequence. Outputs of a shortened run are incomplete. (Not under gfr_moe_set_gate: all launches.) */
 int gfr_moe_set_launches(gfr_moe* m, int launches);
 int gfr_moe_destroy(gfr_moe* m);
 
@@ -213,6 +225,22 @@ int gfr_moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, c
 int gfr_moe_run_router_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                            const uint16_t* router_weight, const gfr_fp8_shared_weights* sw, int rows);
 float* gfr_moe_shared_output(const gfr_moe* m);
+/* The layer with a bf16 shared expert (no reference counterpart: a checkpoint that leaves it unquantised), for a layer
+ * made with gfr_moe_create_shared(..., shared_exl3 = 0): act = bf16(silu(min(g, limit)) * clamp(u, -limit, limit)) of
+ * g, u = input . gu^T (limit 0: none), shared = act . down^T in fp32 (gfr_dense_run twice, fp32 sums), then
+ * gfr_moe_run_shared with it. gu [2 inter][hidden], down [hidden][inter] bf16; inter at most the layer's. _router_bf16
+ * computes the router logits first, as gfr_moe_run_router. Uses the buffers of gfr_moe_run_fp8's shared expert. */
+typedef struct gfr_bf16_shared_weights {
+    int hidden;
+    int inter;
+    const uint16_t* gu;
+    const uint16_t* down;
+    float limit;
+} gfr_bf16_shared_weights;
+int gfr_moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
+                     const float* logits, const gfr_bf16_shared_weights* sw, int rows);
+int gfr_moe_run_router_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
+                            const uint16_t* router_weight, const gfr_bf16_shared_weights* sw, int rows);
 
 /* ---- The router alone (the reference's Triton topk, moe.rs:89-100; source absent, semantics of the benchmark):
  * logits [rows][routed] fp32 -> picks / weights [rows][topk + 1]: top-k by logit (ties: lower id), weights the
@@ -236,6 +264,69 @@ int gfr_route_topk(hipStream_t stream, const float* logits, int rows, int routed
  * 16 bytes at a time). */
 int gfr_router_logits(hipStream_t stream, const uint16_t* input, int input_stride, const uint16_t* router_weight,
                       int hidden, int routed, int rows, float* logits);
+
+/* ---- The general router gate (no reference counterpart; its two gates are gfr_route_topk and gfr_route_topk_biased) --
+ * logits [rows][logits_stride] fp32, bf16 or fp16 (logits_type) -> picks / weights [rows][topk + shared]; shared = 1
+ * appends the shared expert (id `routed`, weight 1), 0 does not:
+ *   score[e]  = exp(l[e]) / sum of exp(l) over all experts (GFR_SCORE_SOFTMAX), or 1 / (1 + exp(-l[e])) (GFR_SCORE_SIGMOID)
+ *   choice[e] = score[e] + bias[e] (bias [routed] fp32, or NULL: the scores' order, which is the logits')
+ *   groups    : routed / groups neighbouring experts each. A group's value is its largest choice (GFR_GROUP_MAX) or the sum
+ *               of its two largest (GFR_GROUP_TOP2; of scores where there is no bias); the kept_groups groups of the
+ *               largest values stay (equal values: the lower group). groups = kept_groups = 1: no groups.
+ *   picks     : the topk largest choices in the groups that stay, descending (equal choices: the lower id)
+ *   weights   : score[pick], with renormalise divided by (the picks' sum in slot order + 1e-20), times scale
+ * Choices and group values are compared as 64-bit arithmetic orders them; weights are fp32.
+ * Masked experts: one whose logit is -inf or NaN, or whose choice is (a bias of -inf or NaN), is picked only when the
+ * kept groups have fewer than topk others, by lower id and with weight 0. The softmax leaves out masked logits, group
+ * values leave out masked experts (a group with one other has that one's choice as its sum; one with none comes last).
+ * A row of masked experts only gets the lowest ids, all with weight 0. Several logits of +inf share a softmax equally.
+ * routed <= 1024, groups <= 64 (a divisor of routed), topk <= 31 and at most the kept groups' experts, scale > 0. */
+#define GFR_BF16 0
+#define GFR_F16 1
+#define GFR_F32 2
+#define GFR_SCORE_SOFTMAX 0
+#define GFR_SCORE_SIGMOID 1
+#define GFR_GROUP_MAX 0
+#define GFR_GROUP_TOP2 1
+int gfr_route_gate(hipStream_t stream, const void* logits, int logits_type, int64_t logits_stride, int rows, int routed,
+                   int topk, const gfr_gate* gate, int shared, int32_t* picks, float* weights);
+
+/* ---- 16-bit matrix products with their epilogue (dense MLP layers, 16-bit shared experts, projections) ----------
+ *   out[r][c] = act(sum over k of x[r][k] * w[c][k] + bias[c]) + residual[r][c]                          (gated = 0)
+ *   out[r][c] = act(min(g, limit)) * clamp(u, -limit, limit) + residual[r][c],                           (gated = 1)
+ *               g = x[r] . w[c] + bias[c], u = x[r] . w[n + c] + bias[n + c] (gate rows, then up rows; limit 0: none)
+ * x [rows][x_stride] and w [n or 2 n][w_stride] in `type` (GFR_BF16 or GFR_F16), out, bias and residual each in that
+ * type or GFR_F32; bias and residual may be NULL. Sums, bias, activation and residual in fp32, one rounding to out's
+ * type. GFR_ACT_GELU is x times the normal distribution's cumulative function (erf), GFR_ACT_GELU_TANH its tanh form.
+ * Strides count elements; any size, stride and element-aligned address works, rows at 16-byte aligned addresses (16-byte
+ * aligned pointers, strides a multiple of 8) are the fast ones. Columns of x and w from k on are not read. residual may
+ * be out itself; out must not overlap x or w otherwise. A row's sums do not depend on the other rows' values, but windows
+ * of other sizes may take them in another order (all in fp32). No scratch: calls may overlap on any streams. */
+#define GFR_ACT_NONE 0
+#define GFR_ACT_RELU 1
+#define GFR_ACT_GELU 2
+#define GFR_ACT_GELU_TANH 3
+#define GFR_ACT_SILU 4
+typedef struct gfr_dense {
+    int rows, n, k;
+    int type;
+    const uint16_t* x;
+    int64_t x_stride;
+    const uint16_t* w;
+    int64_t w_stride;
+    int gated;
+    int act;
+    float limit;
+    int bias_type;
+    const void* bias;
+    int residual_type;
+    int out_type;
+    const void* residual;
+    int64_t residual_stride;
+    void* out;
+    int64_t out_stride;
+} gfr_dense;
+int gfr_dense_run(hipStream_t stream, const gfr_dense* d);
 
 /* ---- Single EXL3 linear (benchmark config 1; the decode path's GEMV with rot_in / down-epilogue formulas) ----
  * y [n] fp32 = svh * had(W^T xh) / sqrt(128), xh = fp16(had(x * suh) / sqrt(128)), x [kin] fp16. */
