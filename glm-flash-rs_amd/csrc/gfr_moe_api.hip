@@ -391,7 +391,7 @@ int gfr_route_gate(hipStream_t stream, const void* logits, int logits_type, int6
     if (!logits || !picks || !weights) return fail(GFR_EINVAL, "null argument");
     int rc = check_gate(gate, routed, topk);
     if (rc) return rc;
-    if (rows <= 0) return fail(GFR_EINVAL, "gate rows %d", rows);
+    if (rows <= 0 || rows > 1 << 24) return fail(GFR_EINVAL, "gate rows %d outside 1..%d", rows, 1 << 24);
     if (!known_type(logits_type)) return fail(GFR_EINVAL, "gate logits type %d", logits_type);
     if (logits_stride < routed) return fail(GFR_EINVAL, "gate logits stride %lld < routed %d", (long long)logits_stride, routed);
     if (shared != 0 && shared != 1) return fail(GFR_EINVAL, "gate shared %d: 0 or 1", shared);
@@ -442,11 +442,12 @@ int gfr_dense_run(hipStream_t stream, const gfr_dense* d) {
         (d->bias && !aligned(d->bias, type_bytes(d->bias_type))) ||
         (d->residual && !aligned(d->residual, type_bytes(d->residual_type))))
         return fail(GFR_EINVAL, "dense: tensors must be aligned to their elements");
-    if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 31))
+    // the most tiles that a launch holds: 2^32 threads, 512 a tile
+    if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 23))
         return fail(GFR_EINVAL, "dense: %d rows of %d columns are too many tiles for a launch", d->rows, d->n);
     const gfr::DenseJob job{d->x, d->w, d->bias, d->residual, d->out, d->x_stride, d->w_stride, d->residual_stride,
                             d->out_stride, d->rows, d->n, d->k, d->type, d->bias_type, d->residual_type, d->out_type,
-                            d->act, d->limit > 0.f ? d->limit : __builtin_inff(), d->gated != 0, 0, false};
+                            d->act, d->limit > 0.f ? d->limit : __builtin_inff(), d->gated != 0, 0, 0, false};
     hipError_t e = gfr::launch_dense(stream, job);
     if (e != hipSuccess) return hip_fail(e, "dense");
     return 0;

@@ -157,7 +157,8 @@ struct DenseJob {
     float limit;                    // infinity: none
     bool gated;
     int n_tiles;                    // set by launch_dense: tiles along the columns
-    bool vector;                    // set by launch_dense: residual and out are read and written four columns at a time (residual, out)
+    int cols;                       // set by launch_dense: columns a workgroup (dense_thin_kernel)
+    bool vector;                    // set by launch_dense: residual and out take eight columns at a time (residual, out)
 };
 hipError_t launch_dense(hipStream_t s, DenseJob d);
 

@@ -18,6 +18,7 @@ def gate(gfr, **kw):
     (dict(scale=float("inf")), {}, "scale"), (dict(bias=18), {}, "bias must be"),
     (dict(groups=8, kept_groups=1), dict(topk=9), "8 experts of the kept groups"), ({}, dict(topk=0), "topk 0"),
     ({}, dict(topk=32), "topk 32"), ({}, dict(rows=0), "rows 0"), ({}, dict(rows=-1), "rows -1"),
+    ({}, dict(rows=(1 << 24) + 1), "outside 1..16777216"),
     ({}, dict(routed=0), "routed 0"), ({}, dict(routed=1025, stride=2000), "routed 1025"), ({}, dict(type=3), "logits type 3"),
     ({}, dict(stride=63), "stride 63"), ({}, dict(shared=2), "shared 2"), ({}, dict(logits=18), "aligned"),
     ({}, dict(logits=17, type=0), "aligned"), ({}, dict(picks=17), "aligned"), ({}, dict(logits=None), "null"),
