@@ -155,7 +155,7 @@ gfr::GateJob gate_job(const gfr_gate& g, const void* logits, int type, int64_t s
                       int shared, int32_t* picks, float* weights) {
     return {logits,      type,     stride, rows,    routed, topk,  topk + (shared ? 1 : 0), g.score == GFR_SCORE_SOFTMAX,
             g.group_score == GFR_GROUP_TOP2, g.renormalise != 0, g.groups, g.kept_groups, g.scale, g.bias, picks, weights,
-            0, 0, 0};
+            0, 0, 0, false, false};
 }
 }  // namespace
 

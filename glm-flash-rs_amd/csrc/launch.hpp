@@ -137,7 +137,9 @@ struct GateJob {
     const float* bias;
     int* picks;
     float* weights;
-    int lpg, per_group, per_lane;   // set by launch_gate: lanes a group, experts a group, experts a lane
+    // set by launch_gate: lanes a group, experts a group, experts a lane, logits and bias in aligned groups of four
+    int lpg, per_group, per_lane;
+    bool four, four_bias;
 };
 hipError_t launch_gate(hipStream_t s, GateJob g);
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -104,9 +105,9 @@ def _load() -> ctypes.CDLL:
         "gfr_prefetch_capturing": ([P, ctypes.POINTER(I)], I),
         "gfr_prefetch_segments": ([P, I, I, P], I),
         "gfr_prefetch_experts": ([P, P, I, P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, I, P], I),
-        "gfr_route_gate": ([P, P, I, ctypes.c_int64, I, I, I, ctypes.POINTER(_GateStruct), I, P, P], I),
-        "gfr_moe_set_gate": ([VP, ctypes.POINTER(_GateStruct)], I),
-        "gfr_dense_run": ([P, ctypes.POINTER(_DenseStruct)], I),
+        "gfr_route_gate": ([P, P, I, ctypes.c_int64, I, I, I, P, I, P, P], I),
+        "gfr_moe_set_gate": ([VP, P], I),
+        "gfr_dense_run": ([P, P], I),
         "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_tensor_extent": ([ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64), I, I,
@@ -355,30 +356,25 @@ class Gate:
     renormalise: bool = True
     scale: float = 1.0
 
-    def struct(self, routed: int) -> "_GateStruct":
+    def pack(self, routed: int) -> bytes:
+        """gfr_gate's bytes."""
         bias = self.bias
         if bias is not None and not (bias.dtype is torch.float32 and bias.shape == (routed,) and bias.is_contiguous()
                                      and bias.is_cuda):
             raise ValueError(f"gate bias: {tuple(bias.shape)} {bias.dtype}, want ({routed},) float32 contiguous on GPU")
-        if self.score not in _SCORES or self.group_score not in _GROUP_SCORES:
+        score, group_score = _SCORES.get(self.score), _GROUP_SCORES.get(self.group_score)
+        if score is None or group_score is None:
             raise ValueError(f"gate: score {self.score!r} of {list(_SCORES)}, group score {self.group_score!r} of "
                              f"{list(_GROUP_SCORES)}")
-        return _GateStruct(_SCORES[self.score], self.groups, self.groups if self.kept_groups is None else self.kept_groups,
-                           _GROUP_SCORES[self.group_score], bool(self.renormalise), self.scale, _ptr(bias))
+        kept = self.kept_groups
+        return _GATE.pack(score, self.groups, self.groups if kept is None else kept, group_score, bool(self.renormalise),
+                          self.scale, 0 if bias is None else bias.data_ptr())
 
 
-class _GateStruct(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int) for n in ("score", "groups", "kept_groups", "group_score", "renormalise")] + [
-        ("scale", ctypes.c_float), ("bias", ctypes.c_void_p)]
-
-
-class _DenseStruct(ctypes.Structure):
-    _fields_ = [("rows", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("type", ctypes.c_int),
-                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("w", ctypes.c_void_p),
-                ("w_stride", ctypes.c_int64), ("gated", ctypes.c_int), ("act", ctypes.c_int),
-                ("limit", ctypes.c_float), ("bias_type", ctypes.c_int), ("bias", ctypes.c_void_p),
-                ("residual_type", ctypes.c_int), ("out_type", ctypes.c_int), ("residual", ctypes.c_void_p),
-                ("residual_stride", ctypes.c_int64), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64)]
+# gfr_gate and gfr_dense as bytes in the machine's layout: packed anew for every call, which a ctypes structure of as many
+# fields takes about three times as long for
+_GATE = struct.Struct("@5ifP")
+_DENSE = struct.Struct("@4iPqPq2ifiP2iPqPq")
 
 
 class _Engine:
@@ -541,7 +537,7 @@ class Moe(_Engine):
         """The general gate (gfr_moe_set_gate) instead of set_router's, in a launch of its own; None: back to that one.
         The gate's bias must outlive the runs (this object holds it)."""
         self._gate = gate
-        _check(lib().gfr_moe_set_gate(self._h, None if gate is None else ctypes.byref(gate.struct(self.routed))))
+        _check(lib().gfr_moe_set_gate(self._h, None if gate is None else gate.pack(self.routed)))
 
     def run_bf16(self, w: Exl3Experts, input: torch.Tensor, logits: torch.Tensor, sw: Bf16SharedWeights, rows: int,
                  stream=None):
@@ -851,21 +847,22 @@ def route_biased(logits: torch.Tensor, bias: torch.Tensor, topk: int, scale: flo
 
 _TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _here(*tensors):
-    """The tensors' device has to be the current one: a launch goes to the current device's stream."""
+def _elsewhere(*tensors):
+    """A launch goes to the current device's stream, so that every tensor's device has to be the current one."""
     here = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != here:
             raise ValueError(f"tensor on {t.device}, the current device is cuda:{here}")
 
 
-def _empty(shape, dtype, device, stream):
+def _empty(shape, dtype, like, stream):
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):       # memory of the stream it is written on
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _row_stride(t) -> int:
@@ -874,46 +871,74 @@ def _row_stride(t) -> int:
     stride, step = t.stride()
     if step != 1 and cols > 1:
         raise ValueError(f"tensor {tuple(t.shape)} strides {tuple(t.stride())}: columns must be neighbours")
-    return stride if rows > 1 else max(stride, cols)
+    return stride if rows > 1 or stride > cols else cols
 
 
 def route_gate(logits: torch.Tensor, gate: Gate, topk: int, shared: bool = True, stream=None):
     """gfr_route_gate: (picks [rows, topk + 1] int32, weights [rows, topk + 1] fp32) of logits [rows, routed] (fp32, bf16
     or fp16), the shared expert's id = routed last; shared=False: [rows, topk] without it."""
     rows, routed = logits.shape
-    if logits.dtype not in _TYPE:
+    kind = _TYPE.get(logits.dtype)
+    if kind is None:
         raise ValueError(f"gate logits {logits.dtype}: fp32, bf16 or fp16")
-    _here(logits, gate.bias)
+    packed, bias = gate.pack(routed), gate.bias
+    here = _get_device()
+    if logits.get_device() != here or (bias is not None and bias.get_device() != here):
+        _elsewhere(logits, bias)
     slots = topk + 1 if shared else topk
-    st = gate.struct(routed)
-    picks = _empty((rows, slots), torch.int32, logits.device, stream)
-    weights = _empty((rows, slots), torch.float32, logits.device, stream)
-    _check(lib().gfr_route_gate(_stream(stream), logits.data_ptr(), _TYPE[logits.dtype], _row_stride(logits), rows, routed,
-                                topk, ctypes.byref(st), int(shared), picks.data_ptr(), weights.data_ptr()))
+    picks = _empty((rows, slots), torch.int32, logits, stream)
+    weights = _empty((rows, slots), torch.float32, logits, stream)
+    handle = _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)
+    rc = (_lib or lib()).gfr_route_gate(handle, logits.data_ptr(), kind, _row_stride(logits), rows, routed, topk,
+                                        packed, 1 if shared else 0, picks.data_ptr(), weights.data_ptr())
+    if rc:
+        _check(rc)
     return picks, weights
 
 
 def _dense(x, w, n, gated, bias, activation, limit, residual, out, out_dtype, stream):
-    if w.dtype is not x.dtype or x.shape[1] != w.shape[1] or activation not in _ACTIVATIONS:
-        raise ValueError(f"x {tuple(x.shape)} {x.dtype}, w {tuple(w.shape)} {w.dtype}, activation {activation!r}: want the "
-                         f"same 16-bit type and columns, an activation of {[a for a in _ACTIVATIONS if a]}")
+    dtype, act = x.dtype, _ACTIVATIONS.get(activation)
     rows, k = x.shape
-    _here(x, w, bias, residual, out)
-    if bias is not None and (bias.shape != (w.shape[0],) or not bias.is_contiguous()):
-        raise ValueError(f"bias {tuple(bias.shape)}: want ({w.shape[0]},) contiguous")
-    if out is None:
-        out = _empty((rows, n), x.dtype if out_dtype is None else out_dtype, x.device, stream)
-    elif out.shape != (rows, n) or (out_dtype is not None and out.dtype is not out_dtype):
-        raise ValueError(f"out {tuple(out.shape)} {out.dtype}: want ({rows}, {n})")
-    if residual is not None and residual.shape != (rows, n):
-        raise ValueError(f"residual {tuple(residual.shape)}: want ({rows}, {n})")
+    wrows, wk = w.shape
+    if w.dtype is not dtype or wk != k or act is None:
+        raise ValueError(f"x {tuple(x.shape)} {dtype}, w {tuple(w.shape)} {w.dtype}, activation {activation!r}: want the "
+                         f"same 16-bit type and columns, an activation of {[a for a in _ACTIVATIONS if a]}")
+    here = _get_device()
+    if x.get_device() != here or w.get_device() != here:
+        _elsewhere(x, w)
     types = _TYPE
-    st = _DenseStruct(rows, n, k, types.get(x.dtype, -1), x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w),
-                      gated, _ACTIVATIONS[activation], limit or 0.0,
-                      0 if bias is None else types.get(bias.dtype, -1), _ptr(bias),
-                      0 if residual is None else types.get(residual.dtype, -1), types.get(out.dtype, -1), _ptr(residual),
-                      0 if residual is None else _row_stride(residual), out.data_ptr(), _row_stride(out))
-    _check(lib().gfr_dense_run(_stream(stream), ctypes.byref(st)))
+    bias_at = bias_type = residual_at = residual_type = residual_stride = 0
+    if bias is not None:
+        if bias.shape != (wrows,) or not bias.is_contiguous():
+            raise ValueError(f"bias {tuple(bias.shape)}: want ({wrows},) contiguous")
+        if bias.get_device() != here:
+            _elsewhere(bias)
+        bias_at, bias_type = bias.data_ptr(), types.get(bias.dtype, -1)
+    if residual is not None:
+        if residual.shape != (rows, n):
+            raise ValueError(f"residual {tuple(residual.shape)}: want ({rows}, {n})")
+        if residual.get_device() != here:
+            _elsewhere(residual)
+        residual_at, residual_type = residual.data_ptr(), types.get(residual.dtype, -1)
+        residual_stride = _row_stride(residual)
+    if out is None:
+        if out_dtype is None:
+            out_dtype = dtype
+        out = _empty((rows, n), out_dtype, x, stream)
+        out_stride = n
+    else:
+        if out.shape != (rows, n) or (out_dtype is not None and out.dtype is not out_dtype):
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype}: want ({rows}, {n})")
+        if out.get_device() != here:
+            _elsewhere(out)
+        out_dtype, out_stride = out.dtype, _row_stride(out)
+    handle = _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)
+    rc = (_lib or lib()).gfr_dense_run(
+        handle, _DENSE.pack(rows, n, k, types.get(dtype, -1), x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w),
+                            gated, act, limit or 0.0, bias_type, bias_at, residual_type, types.get(out_dtype, -1),
+                            residual_at, residual_stride, out.data_ptr(), out_stride))
+    if rc:
+        _check(rc)
     return out
 
 

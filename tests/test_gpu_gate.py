@@ -213,10 +213,8 @@ def test_gate_strides_and_untouched_rows(gfr):
     l = logits_of(rows, E, 3)
     picks = torch.full((rows + 2, topk + 1), -7, dtype=torch.int32, device="cuda")
     weights = torch.full((rows + 2, topk + 1), -7.0, device="cuda")
-    import ctypes
-    st = gfr.Gate().struct(E)
     L = gfr.lib()
-    assert L.gfr_route_gate(gfr._stream(), l.data_ptr(), 2, E, rows, E, topk, ctypes.byref(st), 1, picks.data_ptr(),
+    assert L.gfr_route_gate(gfr._stream(), l.data_ptr(), 2, E, rows, E, topk, gfr.Gate().pack(E), 1, picks.data_ptr(),
                             weights.data_ptr()) == 0
     torch.cuda.synchronize()
     assert (picks[:rows] >= 0).all() and (picks[rows:] == -7).all() and (weights[rows:] == -7).all()

@@ -1,13 +1,11 @@
 """What the general gate and the 16-bit products refuse: host checks before any launch (no GPU needed)."""
-import ctypes
-
 import pytest
 
 
 def gate(gfr, **kw):
     g = dict(score=1, groups=1, kept_groups=1, group_score=0, renormalise=1, scale=1.0, bias=None)
     g.update(kw)
-    return gfr._GateStruct(**g)
+    return gfr._GATE.pack(*[g[n] or 0 for n in ("score", "groups", "kept_groups", "group_score", "renormalise", "scale", "bias")])
 
 
 @pytest.mark.parametrize("kw,args,needle", [
@@ -30,7 +28,7 @@ def test_route_gate_refuses(kw, args, needle):
     a = dict(logits=16, type=2, stride=64, rows=4, routed=64, topk=4, shared=1, picks=16, weights=16)   # never read
     a.update(args)
     st = gate(gfr_moe, **kw)
-    rc = L.gfr_route_gate(None, a["logits"], a["type"], a["stride"], a["rows"], a["routed"], a["topk"], ctypes.byref(st),
+    rc = L.gfr_route_gate(None, a["logits"], a["type"], a["stride"], a["rows"], a["routed"], a["topk"], st,
                           a["shared"], a["picks"], a["weights"])
     assert rc == gfr_moe.GFR_EINVAL and needle in L.gfr_last_error().decode()
 
@@ -40,7 +38,7 @@ def test_null_gate_and_layer():
     L = gfr_moe.lib()
     assert L.gfr_route_gate(None, 16, 2, 64, 4, 64, 4, None, 1, 16, 16) == gfr_moe.GFR_EINVAL
     st = gate(gfr_moe)
-    assert L.gfr_moe_set_gate(None, ctypes.byref(st)) == gfr_moe.GFR_EINVAL
+    assert L.gfr_moe_set_gate(None, st) == gfr_moe.GFR_EINVAL
     assert L.gfr_moe_run_bf16(None, None, None, None, None, None, 1) == gfr_moe.GFR_EINVAL
     assert L.gfr_moe_run_router_bf16(None, None, None, None, None, None, 1) == gfr_moe.GFR_EINVAL
     assert L.gfr_dense_run(None, None) == gfr_moe.GFR_EINVAL
@@ -62,9 +60,11 @@ def test_dense_refuses(kw, needle):
     import gfr_moe
     a = dict(rows=4, n=16, k=32, type=0, x=16, x_stride=32, w=16, w_stride=32, out=16, out_stride=16, residual_stride=16)
     a.update(kw)
-    st = gfr_moe._DenseStruct(**a)
+    names = ("rows n k type x x_stride w w_stride gated act limit bias_type bias residual_type out_type residual "
+             "residual_stride out out_stride").split()
+    st = gfr_moe._DENSE.pack(*[a.get(n) or 0 for n in names])
     L = gfr_moe.lib()
-    assert L.gfr_dense_run(None, ctypes.byref(st)) == gfr_moe.GFR_EINVAL
+    assert L.gfr_dense_run(None, st) == gfr_moe.GFR_EINVAL
     assert needle in L.gfr_last_error().decode()
 
 
@@ -86,10 +86,10 @@ def test_python_refusals():
     with pytest.raises(ValueError, match="gate logits"):
         gfr_moe.route_gate(torch.zeros(2, 8, dtype=torch.float64), gfr_moe.Gate(), 2)
     with pytest.raises(ValueError, match="gate: score"):
-        gfr_moe.Gate(score="max").struct(8)
+        gfr_moe.Gate(score="max").pack(8)
     with pytest.raises(ValueError, match="group score"):
-        gfr_moe.Gate(group_score="sum").struct(8)
+        gfr_moe.Gate(group_score="sum").pack(8)
     with pytest.raises(ValueError, match="gate bias"):
-        gfr_moe.Gate(bias=torch.zeros(7)).struct(8)
+        gfr_moe.Gate(bias=torch.zeros(7)).pack(8)
     with pytest.raises(ValueError, match="bf16"):
         gfr_moe.Bf16SharedWeights(w, w).struct()
