@@ -167,14 +167,33 @@ __device__ __forceinline__ void finish_some(const DenseJob& d, int r, int c, f8_
 
 // The epilogue of a wave's RB x COLS results (COLS columns from c0 on, rows from r0 on), which lie in LDS as RB rows of LD
 // floats (a gated tile's 16 gate and 16 up columns in turn): eight columns a lane, so that the residual and out are read
-// and written in whole lines, the residual a pass ahead.
+// and written in whole lines. Plain sums: all passes' residuals in flight at once; else one pass ahead, in a loop (the
+// activations' code once: unrolled it spilled the sums).
 template <bool GATED, int COLS, int RB, int LD>
 __device__ __forceinline__ void finish_rows(const DenseJob& d, const float* ep, int r0, int c0) {
     constexpr int LANES = COLS / 8, ROWS = 64 / LANES, PASSES = RB / ROWS;
     static_assert(RB % ROWS == 0, "passes");
     const int lane = threadIdx.x & 63, row = lane / LANES, cc = lane % LANES * 8, c = c0 + cc;
     const float* p = ep + row * LD + (GATED ? (cc >> 4) * 32 + (cc & 15) : cc);
-    const bool whole = d.vector && c0 + COLS <= d.n;
+    const bool whole = d.vector && c0 + COLS <= d.n, add = d.residual && whole;
+    const auto ask = [&](int i) {
+        return load_eight(d.residual, d.residual_type, (size_t)min(r0 + row + ROWS * i, d.rows - 1) * d.residual_stride + c);
+    };
+    if (!GATED && whole && !d.bias && d.act == ACT_NONE) {
+        Eight res[PASSES];
+        if (add) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) res[i] = ask(i);
+        }
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = r0 + row + ROWS * i;
+            f8_t v = *reinterpret_cast<const f8_t*>(p + i * ROWS * LD);
+            if (add) v += values(res[i], d.residual_type);
+            if (r < d.rows) store_eight(d.out, d.out_type, (size_t)r * d.out_stride + c, v);
+        }
+        return;
+    }
     f8_t bias = {0, 0, 0, 0, 0, 0, 0, 0}, bias_up = bias;
     if (d.bias && whole) {
 #pragma unroll
@@ -183,10 +202,6 @@ __device__ __forceinline__ void finish_rows(const DenseJob& d, const float* ep, 
             if constexpr (GATED) bias_up[j] = load_one(d.bias, d.bias_type, (size_t)d.n + c + j);
         }
     }
-    const auto ask = [&](int i) {
-        return load_eight(d.residual, d.residual_type, (size_t)min(r0 + row + ROWS * i, d.rows - 1) * d.residual_stride + c);
-    };
-    const bool add = d.residual && whole;
     Eight res{}, next{};
     if (add) res = ask(0);
 #pragma unroll 1
@@ -246,8 +261,9 @@ __device__ __forceinline__ void tile_of(const DenseJob& d, int block, int& tn, i
 // positions (lane l: row l / 8, position l % 8), so the lane reads chunk (l % 8) ^ (l / 8) of its row, and the fragment
 // reads of 8 neighbouring rows (ds_read_b128) meet 8 different positions, all banks once. LDS holds NSB steps of rows
 // and NSA (NSB, or one more) of weights.
-// Needs 16-byte aligned rows whose tile lies within 32-bit offsets; k past the last multiple of 64 is staged through
-// registers (load_chunk), so that nothing beyond k is read.
+// Needs a tile's rows within 32-bit offsets. DIRECT: the loads go straight to LDS, for 16-byte aligned rows; others go
+// through registers. k past the last multiple of 64 is staged element by element (load_chunk), so that nothing beyond k
+// is read.
 template <bool GATED, int NT, int RT, int WN, int WR, int NSA, int NSB>
 struct TileShape {
     static constexpr int COLS = GATED ? NT / 2 : NT;               // columns of out
@@ -264,7 +280,7 @@ struct TileShape {
     static_assert(NSB >= 2 && (NSA == NSB || NSA == NSB + 1) && LDS <= 163840, "stages");
 };
 
-template <int TYPE, bool GATED, int NT, int RT, int WN, int WR, int NSA, int NSB>
+template <int TYPE, bool GATED, bool DIRECT, int NT, int RT, int WN, int WR, int NSA, int NSB>
 __global__ void __launch_bounds__(64 * WN * WR) dense_tile_kernel(DenseJob d) {
     using S = TileShape<GATED, NT, RT, WN, WR, NSA, NSB>;
     extern __shared__ __align__(1024) char lds[];
@@ -362,30 +378,67 @@ __global__ void __launch_bounds__(64 * WN * WR) dense_tile_kernel(DenseJob d) {
         }
         lds_barrier();
     }
+    if constexpr (DIRECT) {
 #pragma unroll
-    for (int p = 0; p < NSB; ++p) {
-        if (p < NSA - 1) {
+        for (int p = 0; p < NSB; ++p) {
+            if (p < NSA - 1) {
 #pragma unroll
-            for (int j = 0; j < S::LA; ++j) issue_a(j, p, p);
+                for (int j = 0; j < S::LA; ++j) issue_a(j, p, p);
+            }
+#pragma unroll
+            for (int j = 0; j < S::LB; ++j) issue_b(j, p, p);
         }
-#pragma unroll
-        for (int j = 0; j < S::LB; ++j) issue_b(j, p, p);
-    }
-    wait_vmcnt<(NSB - 1) * S::LB + (NSA - 2) * S::LA>();
-    lds_barrier();
-#pragma unroll
-    for (int i = 0; i < S::MA + S::NB; ++i) read_one(i, 0, 0, 0, a0, b0);
-    int sa = 0, sb = 0, last = NSA - 1;
-    for (int t = 0; t < steps; ++t) {
-        half(a0, b0, a1, b1, sa, sb, 1, std::integral_constant<int, S::LA>{}, [&](int j) { issue_a(j, t + NSA - 1, last); });
-        wait_vmcnt<S::AHEAD>();
+        wait_vmcnt<(NSB - 1) * S::LB + (NSA - 2) * S::LA>();
         lds_barrier();
-        const int free_b = sb;
-        last = sa;
-        sa = sa + 1 == NSA ? 0 : sa + 1;
-        sb = sb + 1 == NSB ? 0 : sb + 1;
-        // the last step's read of the stage after it is of whatever lies there and is not used
-        half(a1, b1, a0, b0, sa, sb, 0, std::integral_constant<int, S::LB>{}, [&](int j) { issue_b(j, t + NSB, free_b); });
+#pragma unroll
+        for (int i = 0; i < S::MA + S::NB; ++i) read_one(i, 0, 0, 0, a0, b0);
+        int sa = 0, sb = 0, last = NSA - 1;
+        for (int t = 0; t < steps; ++t) {
+            half(a0, b0, a1, b1, sa, sb, 1, std::integral_constant<int, S::LA>{}, [&](int j) { issue_a(j, t + NSA - 1, last); });
+            wait_vmcnt<S::AHEAD>();
+            lds_barrier();
+            const int free_b = sb;
+            last = sa;
+            sa = sa + 1 == NSA ? 0 : sa + 1;
+            sb = sb + 1 == NSB ? 0 : sb + 1;
+            // the last step's read of the stage after it is of whatever lies there and is not used
+            half(a1, b1, a0, b0, sa, sb, 0, std::integral_constant<int, S::LB>{}, [&](int j) { issue_b(j, t + NSB, free_b); });
+        }
+    } else if (steps > 0) {
+        // Through registers, two stages: step t + 2's values are asked for in step t's first half and go to step t's place
+        // after its second (a step past the end is the last one again, and not read).
+        static_assert(DIRECT || (NSA == 2 && NSB == 2), "two stages");
+        uint4 rw[S::LA + S::LB];
+        auto ask = [&](int j, int step) {
+            const uint64_t base = j >= S::LA ? xbase : GATED && ((wave * S::LA + j) * 8 & 16) ? ubase : wbase;
+            uint4 v;
+            __builtin_memcpy(&v, reinterpret_cast<const char*>(base + (uint64_t)min(step, steps - 1) * 128) +
+                                     (j >= S::LA ? vb[j >= S::LA ? j - S::LA : 0] : va[j >= S::LA ? 0 : j]), 16);
+            rw[j] = v;
+        };
+        auto put = [&](int stage) {
+#pragma unroll
+            for (int j = 0; j < S::LA; ++j)
+                *reinterpret_cast<uint4*>(lds + stage * S::STAGE_A + (wave * S::LA + j) * 1024 + lane * 16) = rw[j];
+#pragma unroll
+            for (int j = 0; j < S::LB; ++j)
+                *reinterpret_cast<uint4*>(lds + S::B0 + stage * S::STAGE_B + (wave * S::LB + j) * 1024 + lane * 16) = rw[S::LA + j];
+        };
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+#pragma unroll
+            for (int j = 0; j < S::LA + S::LB; ++j) ask(j, p);
+            put(p);
+        }
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < S::MA + S::NB; ++i) read_one(i, 0, 0, 0, a0, b0);
+        for (int t = 0; t < steps; ++t) {
+            half(a0, b0, a1, b1, t & 1, t & 1, 1, std::integral_constant<int, S::LA + S::LB>{}, [&](int j) { ask(j, t + 2); });
+            lds_barrier();
+            half(a1, b1, a0, b0, (t + 1) & 1, (t + 1) & 1, 0, std::integral_constant<int, 0>{}, [](int) {});
+            put(t & 1);
+        }
     }
     // Epilogue, through the wave's part of LDS
     lds_barrier();
@@ -532,8 +585,8 @@ __global__ void __launch_bounds__(64 * WAVES) dense_thin_kernel(DenseJob d) {
 // workgroup a CU, each a fixed part and a time per 64 k that grows with the share of the CUs in use (they share the
 // caches). Light and full: a chunk's time with few and with all CUs at work, us; fixed: a round's start and epilogue.
 // Fitted to 190 sizes (rows 1 to 4096, 512 to 24576 weight rows, k 1024 to 12288, weights out of the caches), where the
-// form this picks takes 1.015 times the fastest one's time on average, 1.25 at worst. Times of the forms in this order
-// (us, bf16, plain form; -: not measured):
+// form this picks takes 1.015 times the fastest one's time on average, 1.25 at worst; rows off 16-byte alignment to 55 of
+// their own (k 1001 to 8191), 1.014 and 1.45. Times of the forms in this order (us, bf16, plain form; -: not measured):
 //   rows    n     k     16x16  32x16  32x32  32x64  64x64  128x128  128x256  256x256
 //      1   4096  4096     9.8   10.4   11.1   13.7   18.2      -        -        -
 //     16   5120 12288    34.5   27.8   29.2   35.4   46.2      -        -        -
@@ -546,9 +599,17 @@ struct Form {
     int cols, rows;
     float light, full, fixed;
 };
-constexpr Form FORMS[] = {{16, 16, .056f, .11f, .3f}, {32, 16, .075f, .136f, .4f}, {32, 32, .10f, .18f, .5f},
-                          {32, 64, .135f, .237f, .7f}, {64, 64, .20f, .275f, 1.2f}, {128, 128, .3625f, .53f, 2.2f},
-                          {128, 256, .615f, .90f, 3.3f}, {256, 256, 1.017f, 1.5f, 5.5f}};
+// and off alignment, the tiles through registers:
+//     12   4099  4099    18.1   16.1   17.0   19.1   28.0      -        -
+//    128   8191  2047    64.8   57.3   36.6   36.8   29.4     48.3     66.0
+//    512   4099  4099      -      -   103.6  106.1   89.1     71.8    104.1
+//   2000   8191  2047      -      -      -      -      -     146.7    134.5
+constexpr Form ALIGNED[] = {{16, 16, .056f, .11f, .3f},     {32, 16, .075f, .136f, .4f},     {32, 32, .10f, .18f, .5f},
+                            {32, 64, .135f, .237f, .7f},    {64, 64, .20f, .275f, 1.2f},     {128, 128, .3625f, .53f, 2.2f},
+                            {128, 256, .615f, .90f, 3.3f},  {256, 256, 1.017f, 1.5f, 5.5f}};
+constexpr Form UNALIGNED[] = {{16, 16, .067f, .14f, .3f},  {32, 16, .091f, .22f, .4f}, {32, 32, .112f, .25f, .5f},
+                              {32, 64, .153f, .42f, .7f},  {64, 64, .22f, .5f, 1.2f},  {128, 128, .71f, .92f, 5.f},
+                              {128, 256, 1.14f, 1.7f, 7.f}};
 constexpr int THIN_FORMS = 5;                                      // the first ones: dense_thin_kernel
 constexpr int CUS = 256;
 
@@ -559,11 +620,11 @@ int thin_cols(int n, int row_tiles, int most) {
     const int cols = (int)((n + per - 1) / per + 3) / 4 * 4;
     return cols < most ? cols : most;
 }
-int pick_form(const DenseJob& d, bool tiles_fit) {
+int pick_form(const DenseJob& d, bool aligned, bool tiles_fit) {
     int best = 0;
     double least = 0.;
-    for (int f = 0; f < (tiles_fit ? 8 : THIN_FORMS); ++f) {
-        const Form& o = FORMS[f];
+    for (int f = 0; f < (!tiles_fit ? THIN_FORMS : aligned ? 8 : 7); ++f) {
+        const Form& o = aligned ? ALIGNED[f] : UNALIGNED[f];
         const int row_tiles = (d.rows + o.rows - 1) / o.rows, most = d.gated ? o.cols / 2 : o.cols;
         const int cols = f < THIN_FORMS ? thin_cols(d.n, row_tiles, most) : most;
         const int64_t groups = (int64_t)((d.n + cols - 1) / cols) * row_tiles;
@@ -577,12 +638,12 @@ int pick_form(const DenseJob& d, bool tiles_fit) {
 
 bool multiple(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <int TYPE, bool GATED, int NT, int RT, int WN, int WR, int NSA, int NSB>
+template <int TYPE, bool GATED, bool DIRECT, int NT, int RT, int WN, int WR, int NSA, int NSB>
 hipError_t launch_tile(hipStream_t s, DenseJob d) {
     using S = TileShape<GATED, NT, RT, WN, WR, NSA, NSB>;
     d.n_tiles = (d.n + S::COLS - 1) / S::COLS;
     const int64_t tiles = (int64_t)d.n_tiles * ((d.rows + RT - 1) / RT);
-    dense_tile_kernel<TYPE, GATED, NT, RT, WN, WR, NSA, NSB><<<dim3((unsigned)tiles), S::THREADS, S::LDS, s>>>(d);
+    dense_tile_kernel<TYPE, GATED, DIRECT, NT, RT, WN, WR, NSA, NSB><<<dim3((unsigned)tiles), S::THREADS, S::LDS, s>>>(d);
     return hipGetLastError();
 }
 
@@ -599,18 +660,22 @@ hipError_t launch_thin(hipStream_t s, DenseJob d) {
 
 template <int TYPE, bool GATED>
 hipError_t launch(hipStream_t s, DenseJob d) {
-    // the tiles' direct loads take 16-byte aligned rows and a tile's rows within 32-bit offsets
-    const bool tiles_fit = multiple(d.x, 16) && multiple(d.w, 16) && d.x_stride % 8 == 0 && d.w_stride % 8 == 0 &&
-                           d.x_stride < 1 << 22 && d.w_stride < 1 << 22;
-    switch (pick_form(d, tiles_fit)) {
+    // the tiles take a tile's rows within 32-bit offsets, and directly to LDS at 16-byte aligned addresses
+    const bool aligned = multiple(d.x, 16) && multiple(d.w, 16) && d.x_stride % 8 == 0 && d.w_stride % 8 == 0;
+    const bool tiles_fit = d.x_stride < 1 << 22 && d.w_stride < 1 << 22;
+    switch (pick_form(d, aligned, tiles_fit)) {
         case 0: return launch_thin<TYPE, GATED, 1, 1, 8, 2>(s, d);
         case 1: return launch_thin<TYPE, GATED, 2, 1, 8, 2>(s, d);
         case 2: return launch_thin<TYPE, GATED, 2, 2, 8, 2>(s, d);
         case 3: return launch_thin<TYPE, GATED, 2, 4, 8, 2>(s, d);
         case 4: return launch_thin<TYPE, GATED, 4, 4, 8, 1>(s, d);
-        case 5: return launch_tile<TYPE, GATED, 128, 128, 2, 4, 4, 4>(s, d);
-        case 6: return launch_tile<TYPE, GATED, 128, 256, 2, 4, 3, 3>(s, d);
-        default: return launch_tile<TYPE, GATED, 256, 256, 4, 2, 3, 2>(s, d);
+        case 5:
+            return aligned ? launch_tile<TYPE, GATED, true, 128, 128, 2, 4, 4, 4>(s, d)
+                           : launch_tile<TYPE, GATED, false, 128, 128, 2, 4, 2, 2>(s, d);
+        case 6:
+            return aligned ? launch_tile<TYPE, GATED, true, 128, 256, 2, 4, 3, 3>(s, d)
+                           : launch_tile<TYPE, GATED, false, 128, 256, 2, 4, 2, 2>(s, d);
+        default: return launch_tile<TYPE, GATED, true, 256, 256, 4, 2, 3, 2>(s, d);
     }
 }
 

@@ -121,6 +121,15 @@ def test_dense_larger(gfr, rows, n, k, gated):
     one(gfr, rows, n, k, torch.float16, gated, "gelu" if gated else None, seed=rows + 1, out_dtype=torch.float32)
 
 
+@pytest.mark.parametrize("rows,n,k", [(1000, 2047, 1001), (2100, 2055, 999), (4100, 1031, 333), (2100, 2056, 1000),
+                                      (4099, 4104, 200), (700, 5000, 1032), (3000, 3001, 63), (2500, 2600, 72), (2600, 2700, 8)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_dense_large_odd(gfr, rows, n, k, gated):
+    """The tiles' own edges: rows, columns and k that end inside a tile, a step and a chunk, on and off alignment."""
+    one(gfr, rows, n, k, torch.bfloat16, gated, "silu" if gated else None, torch.bfloat16, None, seed=rows)
+    one(gfr, rows, n, k, torch.float16, gated, "gelu_tanh", None, torch.float32, torch.float32, seed=rows + 1)
+
+
 @pytest.mark.parametrize("rows", [1, 9, 70, 300])
 @pytest.mark.parametrize("gated", [False, True])
 def test_dense_strides_alignment_and_padding(gfr, rows, gated):
