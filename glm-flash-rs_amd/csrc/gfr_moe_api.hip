@@ -442,8 +442,8 @@ int gfr_dense_run(hipStream_t stream, const gfr_dense* d) {
         (d->bias && !aligned(d->bias, type_bytes(d->bias_type))) ||
         (d->residual && !aligned(d->residual, type_bytes(d->residual_type))))
         return fail(GFR_EINVAL, "dense: tensors must be aligned to their elements");
-    // the most tiles that a launch holds: 2^32 threads, 512 a tile
-    if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 23))
+    // the most tiles that a launch holds: 2^32 threads, 512 a tile (and up to 255 tiles from evening out)
+    if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 23) - 256)
         return fail(GFR_EINVAL, "dense: %d rows of %d columns are too many tiles for a launch", d->rows, d->n);
     const gfr::DenseJob job{d->x, d->w, d->bias, d->residual, d->out, d->x_stride, d->w_stride, d->residual_stride,
                             d->out_stride, d->rows, d->n, d->k, d->type, d->bias_type, d->residual_type, d->out_type,

@@ -536,12 +536,23 @@ class Moe(_Engine):
     def set_gate(self, gate: "Gate" = None):
         """The general gate (gfr_moe_set_gate) instead of set_router's, in a launch of its own; None: back to that one.
         The gate's bias must outlive the runs (this object holds it)."""
+        if gate is not None and gate.bias is not None and gate.bias.device != self.output.device:
+            raise ValueError(f"gate bias on {gate.bias.device}, the layer on {self.output.device}")
         self._gate = gate
         _check(lib().gfr_moe_set_gate(self._h, None if gate is None else gate.pack(self.routed)))
 
+    def _check_rows(self, t, dtype, columns: int, rows: int, what: str):
+        if t.dtype is not dtype or t.dim() != 2 or t.shape[1] != columns or t.shape[0] < rows or not t.is_contiguous() or (
+                t.device != self.output.device):
+            raise ValueError(f"{what} {tuple(t.shape)} {t.dtype} on {t.device}: want at least [{rows}, {columns}] {dtype}, "
+                             f"contiguous on {self.output.device}")
+
     def run_bf16(self, w: Exl3Experts, input: torch.Tensor, logits: torch.Tensor, sw: Bf16SharedWeights, rows: int,
                  stream=None):
-        """The layer with an unquantised shared expert (a layer made with shared_exl3=False): gfr_moe_run_bf16."""
+        """The layer with an unquantised shared expert (a layer made with shared_exl3=False): gfr_moe_run_bf16. input
+        [rows, hidden] bf16 and logits [rows, routed] fp32, contiguous."""
+        self._check_rows(input, torch.bfloat16, self.hidden, rows, "input")
+        self._check_rows(logits, torch.float32, self.routed, rows, "logits")
         ws, ss = w.struct(), sw.struct()
         _check(lib().gfr_moe_run_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input), _ptr(logits),
                                       ctypes.byref(ss), rows))
@@ -549,6 +560,8 @@ class Moe(_Engine):
     def run_router_bf16(self, w: Exl3Experts, input: torch.Tensor, router_weight: torch.Tensor, sw: Bf16SharedWeights,
                         rows: int, stream=None):
         """run_bf16 with the router logits computed from the hidden rows first (router_weight [routed, hidden])."""
+        self._check_rows(input, torch.bfloat16, self.hidden, rows, "input")
+        self._check_rows(router_weight, torch.bfloat16, self.hidden, self.routed, "router weight")
         ws, ss = w.struct(), sw.struct()
         _check(lib().gfr_moe_run_router_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input),
                                              _ptr(router_weight), ctypes.byref(ss), rows))
@@ -858,6 +871,15 @@ def _elsewhere(*tensors):
             raise ValueError(f"tensor on {t.device}, the current device is cuda:{here}")
 
 
+def _handle(stream, here: int) -> int:
+    """The stream's handle (None: the current one of device `here`)."""
+    if stream is None:
+        return _raw_stream(here) if _raw_stream is not None else _stream(None)
+    if stream.device_index != here:
+        raise ValueError(f"stream of cuda:{stream.device_index}, the current device is cuda:{here}")
+    return stream.cuda_stream
+
+
 def _empty(shape, dtype, like, stream):
     if stream is None:
         return like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
@@ -876,7 +898,8 @@ def _row_stride(t) -> int:
 
 def route_gate(logits: torch.Tensor, gate: Gate, topk: int, shared: bool = True, stream=None):
     """gfr_route_gate: (picks [rows, topk + 1] int32, weights [rows, topk + 1] fp32) of logits [rows, routed] (fp32, bf16
-    or fp16), the shared expert's id = routed last; shared=False: [rows, topk] without it."""
+    or fp16), the shared expert's id = routed last; shared=False: [rows, topk] without it. A stream other than the current
+    one is the caller's to order after the inputs' writes; they have to stay alive until it is done."""
     rows, routed = logits.shape
     kind = _TYPE.get(logits.dtype)
     if kind is None:
@@ -888,7 +911,7 @@ def route_gate(logits: torch.Tensor, gate: Gate, topk: int, shared: bool = True,
     slots = topk + 1 if shared else topk
     picks = _empty((rows, slots), torch.int32, logits, stream)
     weights = _empty((rows, slots), torch.float32, logits, stream)
-    handle = _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)
+    handle = _handle(stream, here)
     rc = (_lib or lib()).gfr_route_gate(handle, logits.data_ptr(), kind, _row_stride(logits), rows, routed, topk,
                                         packed, 1 if shared else 0, picks.data_ptr(), weights.data_ptr())
     if rc:
@@ -931,8 +954,10 @@ def _dense(x, w, n, gated, bias, activation, limit, residual, out, out_dtype, st
             raise ValueError(f"out {tuple(out.shape)} {out.dtype}: want ({rows}, {n})")
         if out.get_device() != here:
             _elsewhere(out)
+        if out.data_ptr() in (x.data_ptr(), w.data_ptr()):
+            raise ValueError("out must not be x or w")
         out_dtype, out_stride = out.dtype, _row_stride(out)
-    handle = _raw_stream(here) if stream is None and _raw_stream is not None else _stream(stream)
+    handle = _handle(stream, here)
     rc = (_lib or lib()).gfr_dense_run(
         handle, _DENSE.pack(rows, n, k, types.get(dtype, -1), x.data_ptr(), _row_stride(x), w.data_ptr(), _row_stride(w),
                             gated, act, limit or 0.0, bias_type, bias_at, residual_type, types.get(out_dtype, -1),
@@ -945,7 +970,8 @@ def _dense(x, w, n, gated, bias, activation, limit, residual, out, out_dtype, st
 def dense(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, activation: str = None,
           residual: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
     """gfr_dense_run: act(x w^T + bias) + residual for x [rows, k] and w [n, k] of one 16-bit type; bias [n], residual and
-    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself."""
+    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself. A stream other than the
+    current one is the caller's to order after the inputs' writes; they have to stay alive until it is done."""
     return _dense(x, w, w.shape[0], 0, bias, activation, 0.0, residual, out, out_dtype, stream)
 
 

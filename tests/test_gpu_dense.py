@@ -165,6 +165,27 @@ def test_dense_residual_in_place(gfr, rows, n, k):
         assert torch.equal(h, want)
 
 
+def test_dense_refuses_on_the_gpu(gfr):
+    x, w = randn(1, 8, 64), randn(2, 64, 64)
+    for kw, needle in ((dict(out=x), "must not be x or w"), (dict(out=w[:8]), "must not be x or w"),
+                       (dict(out=torch.empty(8, 63, dtype=torch.bfloat16, device="cuda")), "want \\(8, 64\\)"),
+                       (dict(residual=randn(3, 7, 64)), "residual"), (dict(residual=randn(3, 8, 64).cpu()), "current device"),
+                       (dict(bias=randn(3, 65)), "bias"), (dict(bias=randn(3, 64).cpu()), "current device"),
+                       (dict(out=torch.empty(8, 64, dtype=torch.bfloat16)), "current device"),
+                       (dict(out=torch.empty(64, 8, dtype=torch.bfloat16, device="cuda").t()), "neighbours")):
+        with pytest.raises(ValueError, match=needle):
+            gfr.dense(x, w, **kw)
+    for bad in ((x[:0], w), (x[:1].expand(8, 64), w), (x.float(), w.float())):
+        with pytest.raises((gfr.GfrError, ValueError)):
+            gfr.dense(*bad)
+    for kw in (dict(out_dtype=torch.float16), dict(residual=randn(3, 8, 64, dtype=torch.float16)),
+               dict(bias=randn(3, 64, dtype=torch.float16))):
+        with pytest.raises(gfr.GfrError, match="x's type or fp32"):
+            gfr.dense(x, w, **kw)
+    with pytest.raises(gfr.GfrError, match="limit"):
+        gfr.dense_gated(x, w, limit=-1.0)
+
+
 @pytest.mark.parametrize("rows", [2, 40, 300])
 def test_dense_special_values(gfr, rows):
     """Infinities and NaN stay in the rows and columns that they meet; fp16 results past its range are infinite."""

@@ -368,6 +368,26 @@ def test_moe_gate_graph(gfr, layer_weights, rows):
         assert torch.equal(m.output, eager)
 
 
+def test_moe_bf16_refuses(gfr, layer_weights):
+    import synth
+    w = layer_weights[1]
+    x, l = synth.activations(4, D, 1), synth.logits(4, E, 1)
+    sw = gfr.Bf16SharedWeights(torch.zeros(2 * N, D, dtype=torch.bfloat16, device="cuda"),
+                               torch.zeros(D, N, dtype=torch.bfloat16, device="cuda"))
+    m = gfr.Moe(D, N, E, TOPK, 4, shared_exl3=False)
+    for args in ((x.half(), l, sw, 4), (x[:, :D - 8], l, sw, 4), (x, l.half(), sw, 4), (x, l[:3], sw, 4), (x, l, sw, 5)):
+        with pytest.raises((ValueError, gfr.GfrError)):
+            m.run_bf16(w, *args)
+    wide = gfr.Bf16SharedWeights(torch.zeros(4 * N, D, dtype=torch.bfloat16, device="cuda"),
+                                 torch.zeros(D, 2 * N, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(gfr.GfrError, match="inter up to"):
+        m.run_bf16(w, x, l, wide, 4)
+    with pytest.raises(gfr.GfrError, match="EXL3"):
+        gfr.Moe(D, N, E, TOPK, 4).run_bf16(layer_weights[0], x, l, sw, 4)
+    with pytest.raises(gfr.GfrError, match="topk"):
+        m.set_gate(gfr.Gate(groups=12, kept_groups=1))
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 300])
 @pytest.mark.parametrize("hidden", [512, 768])
 def test_moe_bf16_shared(gfr, rows, hidden):
