@@ -333,23 +333,27 @@ __global__ void __launch_bounds__(64 * WN * WR) dense_tile_kernel(DenseJob d) {
         if (i < S::NB) frb[i] = *reinterpret_cast<const uint4*>(fb + sb * S::STAGE_B + at + i * 2048);
         else fra[i - S::NB] = *reinterpret_cast<const uint4*>(fa + sa * S::STAGE_A + at + (i - S::NB) * 2048);
     };
-    // A half step (32 k): its MFMAs on the fragments in hand, and between equal shares of them the reads of the next
-    // half's fragments and `loads` direct loads, one by one. In this order and no other: a wave issues in order, so
-    // that a burst of loads would hold back its MFMAs until the address units have taken them (16 cycles each, eight
-    // waves' worth of them).
+    // A half step (32 k): its MFMAs on the fragments in hand, and between equal shares of the first three quarters of
+    // them the reads of the next half's fragments and `loads` direct loads, one by one. In this order and no other: a
+    // wave issues in order, so that a burst of loads would hold back its MFMAs until the address units have taken them
+    // (16 cycles each, eight waves' worth of them).
     auto half = [&](const uint4 (&ca)[S::MA], const uint4 (&cb)[S::NB], uint4 (&na)[S::MA], uint4 (&nb)[S::NB], int sa, int sb,
                     int s, auto loads, auto&& load) {
-        constexpr int READS = S::MA + S::NB, MFMAS = S::MA * S::NB, L = decltype(loads)::value;
+        constexpr int READS = S::MA + S::NB, MFMAS = S::MA * S::NB, SPREAD = MFMAS * 3 / 4, L = decltype(loads)::value;
 #pragma unroll
         for (int i = 0; i < READS; ++i) {
             read_one(i, sa, sb, s, na, nb);
 #pragma unroll
             for (int j = (i * L + READS - 1) / READS; j < ((i + 1) * L + READS - 1) / READS; ++j) load(j);
 #pragma unroll
-            for (int f = i * MFMAS / READS; f < (i + 1) * MFMAS / READS; ++f)
+            for (int f = i * SPREAD / READS; f < (i + 1) * SPREAD / READS; ++f)
                 acc[f / S::NB][f % S::NB] = mfma<TYPE>(ca[f / S::NB], cb[f % S::NB], acc[f / S::NB][f % S::NB]);
             __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int f = SPREAD; f < MFMAS; ++f)
+            acc[f / S::NB][f % S::NB] = mfma<TYPE>(ca[f / S::NB], cb[f % S::NB], acc[f / S::NB][f % S::NB]);
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     // A step's first half loads the weights of step t + NSA - 1 (to the place of step t - 1), its second half the rows of
