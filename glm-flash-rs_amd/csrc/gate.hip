@@ -249,8 +249,8 @@ __device__ __forceinline__ void pick_exactly(const GateJob& g, size_t row_at, in
 // first that does not) differ by more than their errors: the 16 units in the last place that the low bits hide, and the
 // scores' own. Where it is not, and for equal choices, the picks and those after them that may belong before one are put
 // in order by their choices in 64 bits, one a lane; a wave with a row whose groups are in doubt, or with too few experts
-// that are not masked, goes to pick_exactly. With 16-bit logits and no bias the choices are the logits, whose low ten bits are zero: the expert's place
-// in the row stands there, and every order is certain.
+// that are not masked, goes to pick_exactly. With 16-bit logits and no bias the choices are the logits, whose low ten
+// bits are zero: the expert's place in the row stands there, and every order is certain.
 constexpr int MASKED = (int)0x80000100, ABSENT = (int)0x80000000;
 __device__ __forceinline__ int ordered(float v) {
     const int b = __builtin_bit_cast(int, v);
@@ -282,8 +282,8 @@ __device__ __forceinline__ void sort_down(int (&k)[N]) {           // Batcher's 
 
 template <int W, int PER>
 __device__ __forceinline__ bool pick_fast(const GateJob& g, const RowLanes<W>& r, const float (&l)[PER], float (&part)[PER],
-                                          const float (&bias)[PER], float top, float inverse, size_t row_at, int n, int group, int base, int* picked,
-                                          int& pick, bool& live) {
+                                          const float (&bias)[PER], float top, float inverse, size_t row_at, int n, int group,
+                                          int base, int* picked, int& pick, bool& live) {
     constexpr float NONE = -__builtin_inff(), LOG2E = 1.44269504088896341f;
     // keys
     const bool exact = !g.bias && g.type != TYPE_F32;              // every order is certain
@@ -465,7 +465,9 @@ __global__ void __launch_bounds__(THREADS) gate_kernel(GateJob g) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) part[j] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l[j] * -LOG2E));
         }
-        if constexpr (PER <= 16) certain = pick_fast<W, PER>(g, r, l, part, bias, top, g.softmax ? __builtin_amdgcn_rcpf(total) : 1.f, at, n, group, base, picked + (threadIdx.x & ~63), pick, live);
+        if constexpr (PER <= 16)
+            certain = pick_fast<W, PER>(g, r, l, part, bias, top, g.softmax ? __builtin_amdgcn_rcpf(total) : 1.f, at, n, group,
+                                        base, picked + (threadIdx.x & ~63), pick, live);
     }
     if (__any(!certain && real)) pick_exactly<W, PER>(g, at, n, group, base, pick, live);
 

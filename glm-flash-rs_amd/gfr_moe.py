@@ -535,11 +535,12 @@ class Moe(_Engine):
 
     def set_gate(self, gate: "Gate" = None):
         """The general gate (gfr_moe_set_gate) instead of set_router's, in a launch of its own; None: back to that one.
-        The gate's bias must outlive the runs (this object holds it)."""
+        The gate is copied; its bias must outlive the runs (this object holds it until the next gate)."""
         if gate is not None and gate.bias is not None and gate.bias.device != self.output.device:
             raise ValueError(f"gate bias on {gate.bias.device}, the layer on {self.output.device}")
-        self._gate = gate
+        bias = None if gate is None else gate.bias
         _check(lib().gfr_moe_set_gate(self._h, None if gate is None else gate.pack(self.routed)))
+        self._gate_bias = bias     # the tensor itself: the gate's field may change, and a refused gate leaves the last one's
 
     def _check_rows(self, t, dtype, columns: int, rows: int, what: str):
         if t.dtype is not dtype or t.dim() != 2 or t.shape[1] != columns or t.shape[0] < rows or not t.is_contiguous() or (

@@ -388,6 +388,23 @@ def test_moe_bf16_refuses(gfr, layer_weights):
         m.set_gate(gfr.Gate(groups=12, kept_groups=1))
 
 
+def test_moe_holds_the_gate_bias(gfr, layer_weights):
+    """The layer's gate is the one it was given: its bias stays alive when the caller's object gets another, and when a
+    later gate is refused; a later gate that is taken lets it go."""
+    import weakref
+    m = gfr.Moe(D, N, E, TOPK, 4)
+    gate = gfr.Gate(bias=torch.from_numpy(bias_of(E, 9)).cuda())
+    bias = weakref.ref(gate.bias)
+    m.set_gate(gate)
+    gate.bias = None
+    assert bias() is not None
+    with pytest.raises(gfr.GfrError, match="topk"):
+        m.set_gate(gfr.Gate(groups=12, kept_groups=1))
+    assert bias() is not None
+    m.set_gate(gate)
+    assert bias() is None
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 300])
 @pytest.mark.parametrize("hidden", [512, 768])
 def test_moe_bf16_shared(gfr, rows, hidden):
