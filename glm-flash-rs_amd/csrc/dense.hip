@@ -264,6 +264,13 @@ __device__ __forceinline__ void tile_of(const DenseJob& d, int block, int& tn, i
 // Needs a tile's rows within 32-bit offsets. DIRECT: the loads go straight to LDS, for 16-byte aligned rows; others go
 // through registers. k past the last multiple of 64 is staged element by element (load_chunk), so that nothing beyond k
 // is read.
+// Bound, large: the matrix core at the clock that full load leaves (8192 rows, 5120 -> 2 x 12288 gated 1470 us, 12288 ->
+// 5120 783 us: 1402 and 1317 TFLOP/s, where a library's product of 8192^3 runs at 1347). One round of 128 x 128 tiles: the
+// tiles' way from L2 (709 x 5120 x 12288 in 117 us; in copies for timing only, every step's loads from the same lines, in
+// L2, take 102, no loads 77, one fragment read of six 106): 32 KB a step and CU, 12.6 TB/s over the card. A larger tile asks for
+// less, and leaves CUs without one. A stage more or less, four waves instead of eight, waves of 32 x 64 instead of 64 x
+// 32, a barrier that waits for no reads and scalar-only addresses measured the same; with a step's loads in one burst the
+// first form of the 256 x 256 tiles took 1641 us of the gated product above.
 template <bool GATED, int NT, int RT, int WN, int WR, int NSA, int NSB>
 struct TileShape {
     static constexpr int COLS = GATED ? NT / 2 : NT;               // columns of out
@@ -466,6 +473,9 @@ __global__ void __launch_bounds__(64 * WN * WR) dense_tile_kernel(DenseJob d) {
 // lanes of 16 bytes a row: loads in the fragments' own layout, whose neighbouring lanes are different rows, ran at 16
 // bytes a cycle and CU), turns them into fragments through a stage of its own in LDS (the swizzle of the tiles; no
 // barrier, a wave's LDS operations complete in order), and has the next U chunks' loads in flight meanwhile.
+// Bound: HBM (weights out of the caches; the same read by a library's product in brackets): 1 row, 5120 -> 2 x 12288
+// gated 45.4 us, 5540 GB/s (49.8); 12288 -> 5120 26.6 us, 4723 GB/s (29.2); 16 rows of it 28.0 (31.1); 5120^2 12.5 us,
+// 4185 GB/s (13.4), where a round's start and end show.
 // EB tiles of 16 weight rows hold the columns: CC = 16 a tile, or 8 gate rows and the 8 up rows of the same columns. With
 // fewer than EB CC columns the last are read twice and dropped: `cols` is chosen so that every CU gets as much work.
 template <int TYPE, bool GATED, int EB, int RB, int WAVES, int U>
