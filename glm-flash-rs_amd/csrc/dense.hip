@@ -600,30 +600,36 @@ __global__ void __launch_bounds__(64 * WAVES) dense_thin_kernel(DenseJob d) {
 // caches). Light and full: a chunk's time with few and with all CUs at work, us; fixed: a round's start and epilogue.
 // Fitted to 190 sizes (rows 1 to 4096, 512 to 24576 weight rows, k 1024 to 12288, weights out of the caches), where the
 // form this picks takes 1.015 times the fastest one's time on average, 1.25 at worst; rows off 16-byte alignment to 55 of
-// their own (k 1001 to 8191), 1.014 and 1.45. Times of the forms in this order (us, bf16, plain form; -: not measured):
-//   rows    n     k     16x16  32x16  32x32  32x64  64x64  128x128  128x256  256x256
-//      1   4096  4096     9.8   10.4   11.1   13.7   18.2      -        -        -
-//     16   5120 12288    34.5   27.8   29.2   35.4   46.2      -        -        -
-//     64   4096  4096    20.3   16.7   14.7   18.0   20.8     33.1     47.4     82.2
-//    128   5120  1536      -    16.1   13.5   15.4   11.1     19.2     23.1     37.7
-//    512   4096  4096      -      -    58.0   58.4   38.8     38.4     53.6     86.2
-//   1536   4096  4096      -      -      -      -      -      71.2     58.1     86.3
-//   4096  16384  2048      -      -      -      -      -     360.4    285.8    227.1
+// their own (k 1001 to 8191), 1.014 and 1.45. 64 x 128, added to the others, to 84 and 40 (1.002 and 1.08, 1.002 and
+// 1.03); of 85 and 40 other sizes it made 18 and 8 faster by 5 to 27 %, none slower by more than 4.5 %.
+// Times of the forms in this order (us, bf16, plain form; -: not measured):
+//   rows    n     k     16x16  32x16  32x32  32x64  64x64  64x128  128x128  128x256  256x256
+//      1   4096  4096     9.8   10.4   11.1   13.7   18.2     -        -        -        -
+//     16   5120 12288    34.5   27.8   29.2   35.4   46.2     -        -        -        -
+//     64   4096  4096    20.3   16.7   14.7   18.0   20.8   23.8     33.1     47.4     82.2
+//    128   5120  1536      -    16.1   13.5   15.4   11.1   11.7     19.2     23.1     37.7
+//    384   5120  5120      -      -      -      -    51.8   39.1     51.0       -        -
+//   1536   1024  4096      -      -      -      -    37.0   25.5     30.8       -        -
+//    512   4096  4096      -      -    58.0   58.4   38.8   31.5     38.4     53.6     86.2
+//   1536   4096  4096      -      -      -      -      -      -      71.2     58.1     86.3
+//   4096  16384  2048      -      -      -      -      -      -     360.4    285.8    227.1
 struct Form {
     int cols, rows;
     float light, full, fixed;
 };
 // and off alignment, the tiles through registers:
-//     12   4099  4099    18.1   16.1   17.0   19.1   28.0      -        -
-//    128   8191  2047    64.8   57.3   36.6   36.8   29.4     48.3     66.0
-//    512   4099  4099      -      -   103.6  106.1   89.1     71.8    104.1
-//   2000   8191  2047      -      -      -      -      -     146.7    134.5
+//     12   4099  4099    18.1   16.1   17.0   19.1   28.0     -        -        -
+//    128   8191  2047    64.8   57.3   36.6   36.8   29.4     -      48.3     66.0
+//    375   5113  4093      -      -      -      -    74.1   59.3     75.3       -
+//   2492    506  4091      -      -      -      -    66.2   45.1     54.3       -
+//    512   4099  4099      -      -   103.6  106.1   89.1     -      71.8    104.1
+//   2000   8191  2047      -      -      -      -      -      -     146.7    134.5
 constexpr Form ALIGNED[] = {{16, 16, .056f, .11f, .3f},     {32, 16, .075f, .136f, .4f},     {32, 32, .10f, .18f, .5f},
-                            {32, 64, .135f, .237f, .7f},    {64, 64, .20f, .275f, 1.2f},     {128, 128, .3625f, .53f, 2.2f},
-                            {128, 256, .615f, .90f, 3.3f},  {256, 256, 1.017f, 1.5f, 5.5f}};
+                            {32, 64, .135f, .237f, .7f},    {64, 64, .20f, .275f, 1.2f},     {64, 128, .207f, .406f, 2.4f},
+                            {128, 128, .3625f, .53f, 2.2f}, {128, 256, .615f, .90f, 3.3f},   {256, 256, 1.017f, 1.5f, 5.5f}};
 constexpr Form UNALIGNED[] = {{16, 16, .067f, .14f, .3f},  {32, 16, .091f, .22f, .4f}, {32, 32, .112f, .25f, .5f},
-                              {32, 64, .153f, .42f, .7f},  {64, 64, .22f, .5f, 1.2f},  {128, 128, .71f, .92f, 5.f},
-                              {128, 256, 1.14f, 1.7f, 7.f}};
+                              {32, 64, .153f, .42f, .7f},  {64, 64, .22f, .5f, 1.2f},  {64, 128, .41f, .571f, 6.7f},
+                              {128, 128, .71f, .92f, 5.f}, {128, 256, 1.14f, 1.7f, 7.f}};
 constexpr int THIN_FORMS = 5;                                      // the first ones: dense_thin_kernel
 constexpr int CUS = 256;
 
@@ -637,7 +643,7 @@ int thin_cols(int n, int row_tiles, int most) {
 int pick_form(const DenseJob& d, bool aligned, bool tiles_fit) {
     int best = 0;
     double least = 0.;
-    for (int f = 0; f < (!tiles_fit ? THIN_FORMS : aligned ? 8 : 7); ++f) {
+    for (int f = 0; f < (!tiles_fit ? THIN_FORMS : aligned ? 9 : 8); ++f) {
         const Form& o = aligned ? ALIGNED[f] : UNALIGNED[f];
         const int row_tiles = (d.rows + o.rows - 1) / o.rows, most = d.gated ? o.cols / 2 : o.cols;
         const int cols = f < THIN_FORMS ? thin_cols(d.n, row_tiles, most) : most;
@@ -684,9 +690,12 @@ hipError_t launch(hipStream_t s, DenseJob d) {
         case 3: return launch_thin<TYPE, GATED, 2, 4, 8, 2>(s, d);
         case 4: return launch_thin<TYPE, GATED, 4, 4, 8, 1>(s, d);
         case 5:
+            return aligned ? launch_tile<TYPE, GATED, true, 64, 128, 2, 4, 5, 5>(s, d)
+                           : launch_tile<TYPE, GATED, false, 64, 128, 2, 4, 2, 2>(s, d);
+        case 6:
             return aligned ? launch_tile<TYPE, GATED, true, 128, 128, 2, 4, 4, 4>(s, d)
                            : launch_tile<TYPE, GATED, false, 128, 128, 2, 4, 2, 2>(s, d);
-        case 6:
+        case 7:
             return aligned ? launch_tile<TYPE, GATED, true, 128, 256, 2, 4, 3, 3>(s, d)
                            : launch_tile<TYPE, GATED, false, 128, 256, 2, 4, 2, 2>(s, d);
         default: return launch_tile<TYPE, GATED, true, 256, 256, 4, 2, 3, 2>(s, d);

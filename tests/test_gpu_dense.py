@@ -130,6 +130,16 @@ def test_dense_large_odd(gfr, rows, n, k, gated):
     one(gfr, rows, n, k, torch.float16, gated, "gelu_tanh", None, torch.float32, torch.float32, seed=rows + 1)
 
 
+@pytest.mark.parametrize("rows,n,k,gated", [(200, 4100, 520, False), (300, 4100, 1000, False), (1100, 1030, 200, False),
+                                            (200, 5128, 72, False), (500, 2063, 1001, False), (300, 5131, 999, False),
+                                            (500, 1030, 1000, True), (300, 2060, 200, True), (1100, 517, 1003, True),
+                                            (200, 2061, 999, True), (384, 2560, 448, True)])
+def test_dense_middle_odd(gfr, rows, n, k, gated):
+    """Sizes between the thin forms' and the large tiles', on and off alignment."""
+    one(gfr, rows, n, k, torch.bfloat16, gated, "silu" if gated else None, torch.bfloat16, torch.bfloat16, seed=rows)
+    one(gfr, rows, n, k, torch.float16, gated, "gelu_tanh", None, None, torch.float32, seed=rows + 1)
+
+
 @pytest.mark.parametrize("rows", [1, 9, 70, 300])
 @pytest.mark.parametrize("gated", [False, True])
 def test_dense_strides_alignment_and_padding(gfr, rows, gated):
