@@ -33,7 +33,9 @@ __device__ __forceinline__ f4_t mfma(uint4 a, uint4 b, f4_t c) {
 }
 
 // ---- epilogue -------------------------------------------------------------------------------------------------------
-typedef float f8_t __attribute__((ext_vector_type(8)));
+// (16: rows in LDS and out are no further aligned)
+typedef float f8_t __attribute__((ext_vector_type(8), aligned(16)));
+static_assert(alignof(f8_t) == 16, "f8_t's accesses");
 __device__ __forceinline__ float bf16_to_f(uint32_t h) { return __builtin_bit_cast(float, h << 16); }
 __device__ __forceinline__ float f16_to_f(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
 __device__ __forceinline__ uint32_t f_to_16(float v, int type) {
