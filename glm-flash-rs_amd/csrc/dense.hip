@@ -680,12 +680,16 @@ hipError_t launch_thin(hipStream_t s, DenseJob d) {
     return hipGetLastError();
 }
 
+// the tiles take rows directly to LDS at 16-byte aligned addresses, and a tile's rows within 32-bit offsets
+bool aligned_rows(const DenseJob& d) {
+    return multiple(d.x, 16) && multiple(d.w, 16) && d.x_stride % 8 == 0 && d.w_stride % 8 == 0;
+}
+int form_of(const DenseJob& d, bool aligned) { return pick_form(d, aligned, d.x_stride < 1 << 22 && d.w_stride < 1 << 22); }
+
 template <int TYPE, bool GATED>
 hipError_t launch(hipStream_t s, DenseJob d) {
-    // the tiles take a tile's rows within 32-bit offsets, and directly to LDS at 16-byte aligned addresses
-    const bool aligned = multiple(d.x, 16) && multiple(d.w, 16) && d.x_stride % 8 == 0 && d.w_stride % 8 == 0;
-    const bool tiles_fit = d.x_stride < 1 << 22 && d.w_stride < 1 << 22;
-    switch (pick_form(d, aligned, tiles_fit)) {
+    const bool aligned = aligned_rows(d);
+    switch (form_of(d, aligned)) {
         case 0: return launch_thin<TYPE, GATED, 1, 1, 8, 2>(s, d);
         case 1: return launch_thin<TYPE, GATED, 2, 1, 8, 2>(s, d);
         case 2: return launch_thin<TYPE, GATED, 2, 2, 8, 2>(s, d);
@@ -705,6 +709,11 @@ hipError_t launch(hipStream_t s, DenseJob d) {
 }
 
 }  // namespace
+
+int dense_form(const DenseJob& d) {
+    const bool aligned = aligned_rows(d);
+    return form_of(d, aligned) + (aligned ? 0 : 16);
+}
 
 hipError_t launch_dense(hipStream_t s, DenseJob d) {
     const auto eight = [](const void* p, int type, int64_t stride) {

@@ -415,7 +415,10 @@ int gfr_moe_set_gate(gfr_moe* m, const gfr_gate* gate) {
 }
 
 // ---- 16-bit products ----------------------------------------------------------------------------------------------
-int gfr_dense_run(hipStream_t stream, const gfr_dense* d) {
+}  // extern "C"
+namespace {
+// A product's checks, and its launch's arguments
+int dense_job(const gfr_dense* d, gfr::DenseJob& job) {
     if (!d || !d->x || !d->w || !d->out) return fail(GFR_EINVAL, "dense: null argument");
     const int limit = 1 << 24;
     if (d->rows <= 0 || d->n <= 0 || d->k <= 0 || d->rows > limit || d->n > limit || d->k > limit)
@@ -445,12 +448,27 @@ int gfr_dense_run(hipStream_t stream, const gfr_dense* d) {
     // the most tiles that a launch holds: 2^32 threads, 512 a tile (and up to 255 tiles from evening out)
     if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 23) - 256)
         return fail(GFR_EINVAL, "dense: %d rows of %d columns are too many tiles for a launch", d->rows, d->n);
-    const gfr::DenseJob job{d->x, d->w, d->bias, d->residual, d->out, d->x_stride, d->w_stride, d->residual_stride,
-                            d->out_stride, d->rows, d->n, d->k, d->type, d->bias_type, d->residual_type, d->out_type,
-                            d->act, d->limit > 0.f ? d->limit : __builtin_inff(), d->gated != 0, 0, 0, false};
+    job = {d->x, d->w, d->bias, d->residual, d->out, d->x_stride, d->w_stride, d->residual_stride,
+           d->out_stride, d->rows, d->n, d->k, d->type, d->bias_type, d->residual_type, d->out_type,
+           d->act, d->limit > 0.f ? d->limit : __builtin_inff(), d->gated != 0, 0, 0, false};
+    return 0;
+}
+}  // namespace
+extern "C" {
+
+int gfr_dense_run(hipStream_t stream, const gfr_dense* d) {
+    gfr::DenseJob job;
+    int rc = dense_job(d, job);
+    if (rc) return rc;
     hipError_t e = gfr::launch_dense(stream, job);
     if (e != hipSuccess) return hip_fail(e, "dense");
     return 0;
+}
+
+int gfr_dense_form(const gfr_dense* d) {
+    gfr::DenseJob job;
+    int rc = dense_job(d, job);
+    return rc ? rc : gfr::dense_form(job);
 }
 
 // ---- debug rotation ---------------------------------------------------------------------------------------------

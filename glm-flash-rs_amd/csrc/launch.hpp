@@ -163,6 +163,8 @@ struct DenseJob {
     bool vector;                    // set by launch_dense: residual and out take eight columns at a time (residual, out)
 };
 hipError_t launch_dense(hipStream_t s, DenseJob d);
+// The form that launch_dense takes (gfr_dense_form's numbers); host only.
+int dense_form(const DenseJob& d);
 
 // shared_fp8.hip
 // The reference's FP8 shared expert (moe.rs:132-167) for rows [rows][x_stride] bf16: gate/up (8 K slices, bf16 gu

@@ -108,6 +108,7 @@ def _load() -> ctypes.CDLL:
         "gfr_route_gate": ([P, P, I, ctypes.c_int64, I, I, I, P, I, P, P], I),
         "gfr_moe_set_gate": ([VP, P], I),
         "gfr_dense_run": ([P, P], I),
+        "gfr_dense_form": ([P], I),
         "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_tensor_extent": ([ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64), I, I,

@@ -327,6 +327,11 @@ typedef struct gfr_dense {
     int64_t out_stride;
 } gfr_dense;
 int gfr_dense_run(hipStream_t stream, const gfr_dense* d);
+/* The kernel that gfr_dense_run takes for a call, for measurements and tests: its checks on the host and nothing launched
+ * (no memory is read, so the pointers stand for their alignment only). 0 .. 4: the thin forms of 16 x 16, 32 x 16, 32 x 32,
+ * 32 x 64 and 64 x 64 weight rows x rows a workgroup; 5 .. 8: the tiles of 64 x 128, 128 x 128, 128 x 256 and 256 x 256;
+ * + 16 where x's or w's rows are off 16-byte alignment. Negative: refused. */
+int gfr_dense_form(const gfr_dense* d);
 
 /* ---- Single EXL3 linear (benchmark config 1; the decode path's GEMV with rot_in / down-epilogue formulas) ----
  * y [n] fp32 = svh * had(W^T xh) / sqrt(128), xh = fp16(had(x * suh) / sqrt(128)), x [kin] fp16. */
