@@ -9,6 +9,7 @@
 #include <string.h>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include "../../include/gfr_moe.h"
 #include "launch.hpp"
@@ -129,6 +130,29 @@ struct gfr_shared_fp8 {
 };
 
 namespace {
+// `rows` rows of `bytes` bytes, `pitch` bytes apart (pitch >= bytes: rows do not overlap each other).
+struct RowBytes {
+    uintptr_t at;
+    int64_t bytes, pitch, rows;
+};
+// Whether two such sets of rows share a byte; slices side by side in one buffer do not.
+bool overlap(RowBytes a, RowBytes b) {
+    const auto end = [](const RowBytes& r) { return r.at + (uint64_t)(r.rows - 1) * r.pitch + r.bytes; };
+    if (end(a) <= b.at || end(b) <= a.at) return false;
+    if (a.rows > b.rows) std::swap(a, b);
+    if (a.rows == 1) a.pitch = b.pitch;
+    if (a.pitch == b.pitch) {
+        // the distance of a row of b from a row of a is delta + d pitch, d their numbers' difference: the largest such
+        // distance below a's length has to end b's row past a's start
+        const int64_t delta = (int64_t)(b.at - a.at), room = a.bytes - 1 - delta, p = a.pitch;
+        const int64_t below = room >= 0 ? room / p : -((-room + p - 1) / p), d = below < b.rows - 1 ? below : b.rows - 1;
+        return d >= -(a.rows - 1) && delta + d * p > -b.bytes;
+    }
+    for (int64_t i = 0; i < a.rows; ++i)
+        if (overlap({a.at + (uint64_t)(i * a.pitch), a.bytes, b.pitch, 1}, b)) return true;
+    return false;
+}
+
 // The general gate's checks, and its launch's arguments
 bool known_type(int t) { return t == GFR_BF16 || t == GFR_F16 || t == GFR_F32; }
 size_t type_bytes(int t) { return t == GFR_F32 ? 4 : 2; }
@@ -448,6 +472,23 @@ int dense_job(const gfr_dense* d, gfr::DenseJob& job) {
     // the most tiles that a launch holds: 2^32 threads, 512 a tile (and up to 255 tiles from evening out)
     if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 23) - 256)
         return fail(GFR_EINVAL, "dense: %d rows of %d columns are too many tiles for a launch", d->rows, d->n);
+    // a workgroup stores its part of out while others still read theirs of the operands
+    const auto rows_of = [](const void* p, int type, int64_t rows, int64_t columns, int64_t stride) {
+        const int64_t e = (int64_t)type_bytes(type);
+        return RowBytes{reinterpret_cast<uintptr_t>(p), columns * e, stride * e, rows};
+    };
+    const int64_t wrows = (int64_t)d->n * (1 + d->gated);
+    const RowBytes out = rows_of(d->out, d->out_type, d->rows, d->n, d->out_stride);
+    const bool in_place = d->residual == d->out && d->residual_type == d->out_type &&
+                          (d->rows == 1 || d->residual_stride == d->out_stride);
+    const char* met = overlap(out, rows_of(d->x, d->type, d->rows, d->k, d->x_stride))     ? "x"
+                      : overlap(out, rows_of(d->w, d->type, wrows, d->k, d->w_stride))     ? "w"
+                      : d->bias && overlap(out, rows_of(d->bias, d->bias_type, 1, wrows, wrows)) ? "bias"
+                      : d->residual && !in_place &&
+                              overlap(out, rows_of(d->residual, d->residual_type, d->rows, d->n, d->residual_stride))
+                          ? "the residual, and is not the residual itself"
+                          : nullptr;
+    if (met) return fail(GFR_EINVAL, "dense: out overlaps %s", met);
     job = {d->x, d->w, d->bias, d->residual, d->out, d->x_stride, d->w_stride, d->residual_stride,
            d->out_stride, d->rows, d->n, d->k, d->type, d->bias_type, d->residual_type, d->out_type,
            d->act, d->limit > 0.f ? d->limit : __builtin_inff(), d->gated != 0, 0, 0, false};

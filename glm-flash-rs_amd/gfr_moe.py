@@ -972,7 +972,8 @@ def _dense(x, w, n, gated, bias, activation, limit, residual, out, out_dtype, st
 def dense(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, activation: str = None,
           residual: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
     """gfr_dense_run: act(x w^T + bias) + residual for x [rows, k] and w [n, k] of one 16-bit type; bias [n], residual and
-    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself. No gradient is recorded.
+    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself; any other
+    memory that out shares with an operand is refused. No gradient is recorded.
     A stream other than the current one is the caller's to order after the inputs' writes; they have to stay alive until it
     is done."""
     return _dense(x, w, w.shape[0], 0, bias, activation, 0.0, residual, out, out_dtype, stream)

@@ -300,8 +300,9 @@ int gfr_route_gate(hipStream_t stream, const void* logits, int logits_type, int6
  * type. GFR_ACT_GELU is x times the normal distribution's cumulative function (erf), GFR_ACT_GELU_TANH its tanh form.
  * Strides count elements; any size, stride and element-aligned address works, rows at 16-byte aligned addresses (16-byte
  * aligned pointers, strides a multiple of 8) are the fast ones. Columns of x and w from k on are not read. residual may
- * be out itself; out must not overlap x or w otherwise. A row's sums do not depend on the other rows' values, but windows
- * of other sizes may take them in another order (all in fp32). No scratch: calls may overlap on any streams. */
+ * be out itself (address, type and stride); an out that shares memory with an operand in any other way is refused. A row's
+ * sums do not depend on the other rows' values, but windows of other sizes may take them in another order (all in fp32).
+ * No scratch: calls may overlap on any streams. */
 #define GFR_ACT_NONE 0
 #define GFR_ACT_RELU 1
 #define GFR_ACT_GELU 2
