@@ -658,9 +658,9 @@ int gfr_moe_set_decode_rows(gfr_moe* m, int decode_rows) {
 }
 
 namespace {
-int moe_run(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input, const float* logits,
-            const float* shared, int shared_stride, int rows, hipEvent_t shared_ready = nullptr,
-            const gfr::Fp8Shared* fp8 = nullptr) {
+// A run's checks, all before the first launch of any part of it
+int moe_ready(const gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input, const float* logits, const float* shared,
+              int shared_stride, int rows) {
     if (!m) return fail(GFR_EINVAL, "null moe");
     int rc = check_weights(w, m->hidden, m->inter);
     if (rc) return rc;
@@ -676,6 +676,13 @@ int moe_run(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uin
     if (shared && (shared_stride % 4 || reinterpret_cast<uintptr_t>(shared) % 16))
         return fail(GFR_EINVAL, "shared output: stride %d must be a multiple of 4 and the pointer 16-byte aligned",
                     shared_stride);
+    return 0;
+}
+int moe_run(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input, const float* logits,
+            const float* shared, int shared_stride, int rows, hipEvent_t shared_ready = nullptr,
+            const gfr::Fp8Shared* fp8 = nullptr) {
+    int rc = moe_ready(m, w, input, logits, shared, shared_stride, rows);
+    if (rc) return rc;
     if (shared_ready && !shared) return fail(GFR_EINVAL, "a shared-ready event without a shared output");
     hipError_t e;
     const gfr::GateJob gate = m->has_gate ? gate_job(m->gate, logits, GFR_F32, m->routed, rows, m->routed, m->topk, 1,
@@ -931,12 +938,16 @@ int shared_fp8_run(gfr_shared_fp8* sh, hipStream_t stream, const gfr_fp8_shared_
     if (e != hipSuccess) return hip_fail(e, "FP8 shared expert");
     return 0;
 }
-int moe_fp8_ready(gfr_moe* m, const gfr_fp8_shared_weights* sw) {
+int moe_fp8_ready(gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input, const float* logits,
+                  const gfr_fp8_shared_weights* sw, int rows) {
     if (!m) return fail(GFR_EINVAL, "null moe");
     if (m->shared_exl3 || !m->sfp8)
         return fail(GFR_EINVAL, "the layer has no FP8 shared expert (made with shared_exl3 = 1, or hidden %d is not "
                     "a multiple of 512)", m->hidden);
-    return check_fp8_weights(sw, m->hidden, m->inter);
+    int rc = check_fp8_weights(sw, m->hidden, m->inter);
+    if (rc) return rc;
+    if (input && !al16(input)) return fail(GFR_EINVAL, "input rows must be 16-byte aligned");
+    return moe_ready(m, w, input, logits, m->shared_out, m->hidden, rows);
 }
 }  // namespace
 
@@ -1005,15 +1016,11 @@ int gfr_shared_fp8_destroy(gfr_shared_fp8* sh) {
 
 namespace {
 // The layer with its FP8 shared expert. A one-token window whose launches have the shared slot's workgroups (the
-// grid's last unit exists: the weights hold at least `slots` experts; not under gfr_moe_set_gate) runs the shared expert inside the gate/up and
-// down launches (three launches in all), a prefill-engine window of at most 16 rows inside its route + group + rotation
-// and gate/up epilogue launches; other windows run its two launches first.
+// grid's last unit exists: the weights hold at least `slots` experts) runs the shared expert inside the gate/up and down
+// launches (three launches in all), a prefill-engine window of at most 16 rows inside its route + group + rotation and
+// gate/up epilogue launches; other windows, and every window under gfr_moe_set_gate, run its two launches first.
 int moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                 const float* logits, const gfr_fp8_shared_weights* sw, int rows) {
-    if (rows <= 0 || rows > m->max_rows) return fail(GFR_EINVAL, "rows %d outside 1..%d", rows, m->max_rows);
-    if (!w || !input) return fail(GFR_EINVAL, "null weights or input");
-    if (!al16(input)) return fail(GFR_EINVAL, "input rows must be 16-byte aligned");
-    // (the weights' other checks follow in moe_run, before any launch)
     const bool fused = m->has_gate ? false
                        : rows <= m->decode_rows
                            ? rows == 1 && w->experts >= m->slots && gfr::gemv_gateup_splits(m->hidden) <= 16
@@ -1032,17 +1039,16 @@ int moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const
 
 int gfr_moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                     const float* logits, const gfr_fp8_shared_weights* sw, int rows) {
-    int rc = moe_fp8_ready(m, sw);
+    int rc = moe_fp8_ready(m, w, input, logits, sw, rows);
     if (rc) return rc;
     return moe_run_fp8(m, stream, w, input, logits, sw, rows);
 }
 
 int gfr_moe_run_router_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                            const uint16_t* router_weight, const gfr_fp8_shared_weights* sw, int rows) {
-    int rc = moe_fp8_ready(m, sw);
+    int rc = moe_fp8_ready(m, w, input, m ? m->logits : nullptr, sw, rows);
     if (rc) return rc;
-    if (!input || !router_weight) return fail(GFR_EINVAL, "null input or router weight");
-    if (rows <= 0 || rows > m->max_rows) return fail(GFR_EINVAL, "rows %d outside 1..%d", rows, m->max_rows);
+    if (!router_weight) return fail(GFR_EINVAL, "null router weight");
     if ((rc = gfr_router_logits(stream, input, m->hidden, router_weight, m->hidden, m->routed, rows, m->logits)))
         return rc;
     return moe_run_fp8(m, stream, w, input, m->logits, sw, rows);
@@ -1050,8 +1056,9 @@ int gfr_moe_run_router_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_expert
 
 // ---- the bf16 shared expert -------------------------------------------------------------------------------------
 namespace {
-int moe_bf16_ready(gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input, const gfr_bf16_shared_weights* sw,
-                   int rows) {
+// The shared expert's two products (job), checked with the rest of the run
+int moe_bf16_ready(gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input, const float* logits,
+                   const gfr_bf16_shared_weights* sw, int rows, gfr::DenseJob (&job)[2]) {
     if (!m) return fail(GFR_EINVAL, "null moe");
     if (m->shared_exl3) return fail(GFR_EINVAL, "the layer's shared expert is EXL3: no bf16 shared expert");
     if (!sw || !sw->gu || !sw->down) return fail(GFR_EINVAL, "null bf16 shared weights");
@@ -1059,12 +1066,8 @@ int moe_bf16_ready(gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input,
         return fail(GFR_EINVAL, "bf16 shared weights %dx%d: the layer's hidden %d, inter up to %d", sw->hidden, sw->inter,
                     m->hidden, m->inter);
     if (!(sw->limit >= 0.f)) return fail(GFR_EINVAL, "bf16 shared limit %g must not be negative", (double)sw->limit);
-    if (!input) return fail(GFR_EINVAL, "null input");
-    if (rows <= 0 || rows > m->max_rows) return fail(GFR_EINVAL, "rows %d outside 1..%d", rows, m->max_rows);
-    return check_weights(w, m->hidden, m->inter);
-}
-int moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
-                 const float* logits, const gfr_bf16_shared_weights* sw, int rows) {
+    int rc = moe_ready(m, w, input, logits, m->bf16_out, m->hidden, rows);
+    if (rc) return rc;
     const int H = m->hidden, I = sw->inter;
     gfr_dense up{};
     up.rows = rows, up.n = I, up.k = H;
@@ -1077,28 +1080,36 @@ int moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, cons
     down.x = m->bf16_act, down.x_stride = I;
     down.w = sw->down, down.w_stride = I;
     down.out = m->bf16_out, down.out_stride = H, down.out_type = GFR_F32;
-    int rc;
-    if ((rc = gfr_dense_run(stream, &up)) || (rc = gfr_dense_run(stream, &down))) return rc;
-    return moe_run(m, stream, w, input, logits, m->bf16_out, H, rows);
+    if ((rc = dense_job(&up, job[0]))) return rc;
+    return dense_job(&down, job[1]);
+}
+int moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
+                 const float* logits, const gfr::DenseJob (&job)[2], int rows) {
+    for (const gfr::DenseJob& j : job) {
+        hipError_t e = gfr::launch_dense(stream, j);
+        if (e != hipSuccess) return hip_fail(e, "bf16 shared expert");
+    }
+    return moe_run(m, stream, w, input, logits, m->bf16_out, m->hidden, rows);
 }
 }  // namespace
 
 int gfr_moe_run_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                      const float* logits, const gfr_bf16_shared_weights* sw, int rows) {
-    int rc = moe_bf16_ready(m, w, input, sw, rows);
+    gfr::DenseJob job[2];
+    int rc = moe_bf16_ready(m, w, input, logits, sw, rows, job);
     if (rc) return rc;
-    if (!logits) return fail(GFR_EINVAL, "null logits");
-    return moe_run_bf16(m, stream, w, input, logits, sw, rows);
+    return moe_run_bf16(m, stream, w, input, logits, job, rows);
 }
 
 int gfr_moe_run_router_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                             const uint16_t* router_weight, const gfr_bf16_shared_weights* sw, int rows) {
-    int rc = moe_bf16_ready(m, w, input, sw, rows);
+    gfr::DenseJob job[2];
+    int rc = moe_bf16_ready(m, w, input, m ? m->logits : nullptr, sw, rows, job);
     if (rc) return rc;
     if (!router_weight) return fail(GFR_EINVAL, "null router weight");
     if ((rc = gfr_router_logits(stream, input, m->hidden, router_weight, m->hidden, m->routed, rows, m->logits)))
         return rc;
-    return moe_run_bf16(m, stream, w, input, m->logits, sw, rows);
+    return moe_run_bf16(m, stream, w, input, m->logits, job, rows);
 }
 
 float* gfr_moe_shared_output(const gfr_moe* m) { return m ? m->shared_out : nullptr; }

@@ -1,0 +1,70 @@
+"""The layer with a shared expert that is not EXL3: what its runs leave behind, refused ones among them."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D, N, E, TOPK, BITS = 512, 256, 24, 4, 4
+
+
+@pytest.fixture(scope="module")
+def layer_weights():
+    import synth
+    return synth.experts(E + 1, D, N, BITS, seed=5), synth.experts(E, D, N, BITS, seed=6)
+
+
+def bf16_shared(gfr, hidden, inter, seed=3, limit=2.0):
+    g = torch.Generator().manual_seed(seed)
+    return gfr.Bf16SharedWeights((torch.randn((2 * inter, hidden), generator=g) * 3 / hidden ** 0.5).to(torch.bfloat16).cuda(),
+                                 (torch.randn((hidden, inter), generator=g) / inter ** 0.5).to(torch.bfloat16).cuda(), limit)
+
+
+def router_weight(hidden, seed=4):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((E, hidden), generator=g) / hidden ** 0.5).to(torch.bfloat16).cuda()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20, 300])
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+@pytest.mark.parametrize("router", [False, True])
+def test_refused_run_launches_nothing(gfr, layer_weights, rows, kind, router):
+    """Weights of another number of experts: refused before the shared expert's launches, the outputs of the run before
+    still in place."""
+    import synth
+    wrong, w = layer_weights
+    x, l, rw = synth.activations(rows, D, rows), synth.logits(rows, E, rows), router_weight(D)
+    sw = synth.fp8_shared(D, N) if kind == "fp8" else bf16_shared(gfr, D, N)
+    m = gfr.Moe(D, N, E, TOPK, rows, shared_exl3=False)
+    run = getattr(m, f"run_{'router_' if router else ''}{kind}")
+    run(w, x, rw if router else l, sw, rows)
+    torch.cuda.synchronize()
+    before = [t.clone() for t in (m.output, m.shared_output, m.picks, m.weights)]
+    x2 = synth.activations(rows, D, rows + 50)
+    with pytest.raises(gfr.GfrError, match="weights hold 25 experts"):
+        run(wrong, x2, rw if router else l, sw, rows)
+    torch.cuda.synchronize()
+    for a, b in zip(before, (m.output, m.shared_output, m.picks, m.weights)):
+        assert torch.equal(a, b)
+    m.output.zero_()
+    run(w, x, rw if router else l, sw, rows)
+    torch.cuda.synchronize()
+    assert torch.equal(m.output, before[0])
+
+
+def test_refused_down_matrix_launches_nothing(gfr, layer_weights):
+    """The down matrix at an odd address (through the C interface): refused before the gate and up matrices' product."""
+    import ctypes
+    import synth
+    w = layer_weights[1]
+    rows = 3
+    x, l, sw = synth.activations(rows, D, 1), synth.logits(rows, E, 1), bf16_shared(gfr, D, N)
+    m = gfr.Moe(D, N, E, TOPK, rows, shared_exl3=False)
+    m.run_bf16(w, x, l, sw, rows)
+    torch.cuda.synchronize()
+    before = m.output.clone(), m.shared_output.clone()
+    ws, ss = w.struct(), sw.struct()
+    ss.down += 1
+    rc = gfr.lib().gfr_moe_run_bf16(m._h, gfr._stream(), ctypes.byref(ws), x.data_ptr(), l.data_ptr(), ctypes.byref(ss), rows)
+    assert rc == gfr.GFR_EINVAL
+    torch.cuda.synchronize()
+    assert torch.equal(m.output, before[0]) and torch.equal(m.shared_output, before[1])
