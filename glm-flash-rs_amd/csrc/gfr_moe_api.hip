@@ -1112,7 +1112,8 @@ int gfr_moe_run_router_bf16(gfr_moe* m, hipStream_t stream, const gfr_exl3_exper
     return moe_run_bf16(m, stream, w, input, m->logits, job, rows);
 }
 
-float* gfr_moe_shared_output(const gfr_moe* m) { return m ? m->shared_out : nullptr; }
+// (bf16_out is shared_out where the layer has the FP8 shared expert's buffers)
+float* gfr_moe_shared_output(const gfr_moe* m) { return m ? m->bf16_out : nullptr; }
 
 int gfr_router_logits(hipStream_t stream, const uint16_t* input, int input_stride, const uint16_t* router_weight,
                       int hidden, int routed, int rows, float* logits) {

@@ -570,10 +570,10 @@ class Moe(_Engine):
 
     @property
     def shared_output(self) -> torch.Tensor:
-        """[max_rows, hidden] fp32: the FP8 shared expert's output of the last run_fp8 (shared_exl3=False)."""
+        """[max_rows, hidden] fp32: the shared expert's output of the last run_fp8 or run_bf16 (shared_exl3=False)."""
         p = lib().gfr_moe_shared_output(self._h)
         if not p:
-            raise ValueError("the layer has no FP8 shared expert")
+            raise ValueError("the layer's shared expert is EXL3")
         return _view(p, (self.max_rows, self.hidden), torch.float32, self.output.device)
 
     def run_router(self, w: Exl3Experts, input: torch.Tensor, router_weight: torch.Tensor, rows: int, stream=None,

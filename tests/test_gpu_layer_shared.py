@@ -68,3 +68,20 @@ def test_refused_down_matrix_launches_nothing(gfr, layer_weights):
     assert rc == gfr.GFR_EINVAL
     torch.cuda.synchronize()
     assert torch.equal(m.output, before[0]) and torch.equal(m.shared_output, before[1])
+
+
+@pytest.mark.parametrize("hidden", [512, 768])
+def test_shared_output_of_a_bf16_run(gfr, hidden):
+    """gfr_moe_shared_output after gfr_moe_run_bf16: the two products' output, where the layer can have an FP8 shared
+    expert (hidden a multiple of 512) and where it cannot."""
+    import synth
+    rows, inter = 20, 192
+    w, sw = synth.experts(E, hidden, N, BITS, seed=6), bf16_shared(gfr, hidden, inter)
+    x, l = synth.activations(rows, hidden, rows), synth.logits(rows, E, rows)
+    m = gfr.Moe(hidden, N, E, TOPK, rows, shared_exl3=False)
+    m.run_bf16(w, x, l, sw, rows)
+    want = gfr.dense(gfr.dense_gated(x, sw.gu, limit=2.0), sw.down, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    assert torch.equal(m.shared_output[:rows], want)
+    with pytest.raises(ValueError, match="EXL3"):
+        gfr.Moe(hidden, N, E, TOPK, rows).shared_output
