@@ -118,7 +118,7 @@ struct gfr_moe {
     bool has_gate;             // the general gate (gfr_moe_set_gate) instead of route_bias / route_scale
     gfr_gate gate;
     uint16_t* bf16_act;        // shared_exl3 = 0: the bf16 shared expert's activations [max_rows][inter] and output
-    float* bf16_out;           // (gfr_moe_run_bf16)
+    float* bf16_out;           // (gfr_moe_run_bf16): the FP8 one's, or gfr_moe_reserve_bf16's
 };
 
 struct gfr_shared_fp8 {
@@ -627,14 +627,10 @@ int gfr_moe_create_shared(gfr_moe** out, int hidden, int inter, int routed, int 
         return rc;
     }
     // the bf16 shared expert's activations and output: the FP8 one's buffers where the layer has them (one shared expert
-    // a run)
-    if (!shared_exl3 && m->sfp8) {
+    // a run), else gfr_moe_reserve_bf16's
+    if (m->sfp8) {
         m->bf16_act = m->sfp8->act;
         m->bf16_out = m->shared_out;
-    } else if (!shared_exl3 && ((rc = alloc_zero(&m->bf16_act, (size_t)max_rows * inter, "moe shared activations")) ||
-                                (rc = alloc_zero(&m->bf16_out, (size_t)max_rows * hidden, "moe shared output")))) {
-        gfr_moe_destroy(m);
-        return rc;
     }
     if (max_rows > m->decode_rows &&
         ((rc = gfr_grouping_create(&m->group_pre, routed + 1, m->slots, max_rows)) ||
@@ -644,6 +640,20 @@ int gfr_moe_create_shared(gfr_moe** out, int hidden, int inter, int routed, int 
     }
     *out = m;
     return 0;
+}
+
+int gfr_moe_reserve_bf16(gfr_moe* m) {
+    if (!m) return fail(GFR_EINVAL, "null moe");
+    if (m->shared_exl3) return fail(GFR_EINVAL, "the layer's shared expert is EXL3: no bf16 shared expert");
+    if (m->bf16_out) return 0;
+    int rc;
+    if ((rc = alloc_zero(&m->bf16_act, (size_t)m->max_rows * m->inter, "moe shared activations")) ||
+        (rc = alloc_zero(&m->bf16_out, (size_t)m->max_rows * m->hidden, "moe shared output"))) {
+        free_all({m->bf16_act, m->bf16_out});
+        m->bf16_act = nullptr;
+        m->bf16_out = nullptr;
+    }
+    return rc;
 }
 
 int gfr_moe_set_decode_rows(gfr_moe* m, int decode_rows) {
@@ -1061,6 +1071,7 @@ int moe_bf16_ready(gfr_moe* m, const gfr_exl3_experts* w, const uint16_t* input,
                    const gfr_bf16_shared_weights* sw, int rows, gfr::DenseJob (&job)[2]) {
     if (!m) return fail(GFR_EINVAL, "null moe");
     if (m->shared_exl3) return fail(GFR_EINVAL, "the layer's shared expert is EXL3: no bf16 shared expert");
+    if (!m->bf16_out) return fail(GFR_EINVAL, "the bf16 shared expert's buffers: gfr_moe_reserve_bf16 first");
     if (!sw || !sw->gu || !sw->down) return fail(GFR_EINVAL, "null bf16 shared weights");
     if (sw->hidden != m->hidden || sw->inter <= 0 || sw->inter > m->inter)
         return fail(GFR_EINVAL, "bf16 shared weights %dx%d: the layer's hidden %d, inter up to %d", sw->hidden, sw->inter,

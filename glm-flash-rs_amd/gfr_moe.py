@@ -109,6 +109,7 @@ def _load() -> ctypes.CDLL:
         "gfr_moe_set_gate": ([VP, P], I),
         "gfr_dense_run": ([P, P], I),
         "gfr_dense_form": ([P], I),
+        "gfr_moe_reserve_bf16": ([VP], I),
         "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_tensor_extent": ([ctypes.c_char_p, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64), I, I,
@@ -477,6 +478,7 @@ class Moe(_Engine):
         _check(lib().gfr_moe_create_shared(ctypes.byref(self._h), hidden, inter, routed, topk, max_rows,
                                            int(shared_exl3)))
         self.hidden, self.routed, self.topk, self.max_rows = hidden, routed, topk, max_rows
+        self._bf16_reserved = False
         L = lib()
         self.output = _view(L.gfr_moe_output(self._h), (max_rows, hidden), torch.float32, device)
         self.picks = _view(L.gfr_moe_picks(self._h), (max_rows, topk + 1), torch.int32, device)
@@ -549,12 +551,22 @@ class Moe(_Engine):
             raise ValueError(f"{what} {tuple(t.shape)} {t.dtype} on {t.device}: want at least [{rows}, {columns}] {dtype}, "
                              f"contiguous on {self.output.device}")
 
+    def reserve_bf16(self):
+        """The buffers of run_bf16 (gfr_moe_reserve_bf16): a layer whose hidden is no multiple of 512 allocates them here,
+        or in its first run, which must not be captured then."""
+        if not self._bf16_reserved:
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("the bf16 shared expert's buffers are not allocated inside a capture: reserve_bf16 before it")
+            _check(lib().gfr_moe_reserve_bf16(self._h))
+            self._bf16_reserved = True
+
     def run_bf16(self, w: Exl3Experts, input: torch.Tensor, logits: torch.Tensor, sw: Bf16SharedWeights, rows: int,
                  stream=None):
         """The layer with an unquantised shared expert (a layer made with shared_exl3=False): gfr_moe_run_bf16. input
-        [rows, hidden] bf16 and logits [rows, routed] fp32, contiguous."""
+        [rows, hidden] bf16 and logits [rows, routed] fp32, contiguous. The first run may allocate (reserve_bf16)."""
         self._check_rows(input, torch.bfloat16, self.hidden, rows, "input")
         self._check_rows(logits, torch.float32, self.routed, rows, "logits")
+        self.reserve_bf16()
         ws, ss = w.struct(), sw.struct()
         _check(lib().gfr_moe_run_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input), _ptr(logits),
                                       ctypes.byref(ss), rows))
@@ -564,6 +576,7 @@ class Moe(_Engine):
         """run_bf16 with the router logits computed from the hidden rows first (router_weight [routed, hidden])."""
         self._check_rows(input, torch.bfloat16, self.hidden, rows, "input")
         self._check_rows(router_weight, torch.bfloat16, self.hidden, self.routed, "router weight")
+        self.reserve_bf16()
         ws, ss = w.struct(), sw.struct()
         _check(lib().gfr_moe_run_router_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input),
                                              _ptr(router_weight), ctypes.byref(ss), rows))
@@ -573,7 +586,7 @@ class Moe(_Engine):
         """[max_rows, hidden] fp32: the shared expert's output of the last run_fp8 or run_bf16 (shared_exl3=False)."""
         p = lib().gfr_moe_shared_output(self._h)
         if not p:
-            raise ValueError("the layer's shared expert is EXL3")
+            raise ValueError("no shared output: the layer's shared expert is EXL3, or reserve_bf16 has not run")
         return _view(p, (self.max_rows, self.hidden), torch.float32, self.output.device)
 
     def run_router(self, w: Exl3Experts, input: torch.Tensor, router_weight: torch.Tensor, rows: int, stream=None,

@@ -229,7 +229,11 @@ float* gfr_moe_shared_output(const gfr_moe* m);
  * made with gfr_moe_create_shared(..., shared_exl3 = 0): act = bf16(silu(min(g, limit)) * clamp(u, -limit, limit)) of
  * g, u = input . gu^T (limit 0: none), shared = act . down^T in fp32 (gfr_dense_run twice, fp32 sums), then
  * gfr_moe_run_shared with it. gu [2 inter][hidden], down [hidden][inter] bf16; inter at most the layer's. _router_bf16
- * computes the router logits first, as gfr_moe_run_router. The shared output is gfr_moe_shared_output, at any hidden. */
+ * computes the router logits first, as gfr_moe_run_router. The shared output is gfr_moe_shared_output.
+ * A layer whose hidden is a multiple of 512 has the buffers (those of gfr_moe_run_fp8's shared expert); any other takes
+ * max_rows * (2 inter + 4 hidden) bytes more, which gfr_moe_reserve_bf16 allocates: once, before the first run, as the
+ * create calls outside a stream capture. Where the buffers are there it does nothing. */
+int gfr_moe_reserve_bf16(gfr_moe* m);
 typedef struct gfr_bf16_shared_weights {
     int hidden;
     int inter;

@@ -85,3 +85,57 @@ def test_shared_output_of_a_bf16_run(gfr, hidden):
     assert torch.equal(m.shared_output[:rows], want)
     with pytest.raises(ValueError, match="EXL3"):
         gfr.Moe(hidden, N, E, TOPK, rows).shared_output
+
+
+@pytest.mark.parametrize("hidden", [512, 768])
+def test_bf16_buffers_are_allocated_when_asked_for(gfr, hidden):
+    """A layer that never runs a bf16 shared expert holds no buffers for one; reserve_bf16 allocates them once, and a
+    layer with the FP8 shared expert's buffers has them."""
+    rows = 8192
+    m = gfr.Moe(hidden, N, E, TOPK, rows, shared_exl3=False)
+    torch.cuda.synchronize()
+    free = [torch.cuda.mem_get_info()[0]]
+    for _ in range(2):
+        m.reserve_bf16()
+        assert gfr.lib().gfr_moe_reserve_bf16(m._h) == 0
+        free.append(torch.cuda.mem_get_info()[0])
+    want = 0 if hidden % 512 == 0 else rows * (2 * N + 4 * hidden)
+    assert free[1] == free[2] and want <= free[0] - free[1] <= want + (8 << 20)
+    assert m.shared_output.shape == (rows, hidden)
+
+
+def test_bf16_run_without_its_buffers(gfr):
+    """Refused in C before reserve, and in Python inside a capture (where nothing may be allocated)."""
+    import ctypes
+    import synth
+    hidden, rows = 768, 3
+    w, sw = synth.experts(E, hidden, N, BITS, seed=6), bf16_shared(gfr, hidden, N)
+    x, l = synth.activations(rows, hidden, rows), synth.logits(rows, E, rows)
+    m = gfr.Moe(hidden, N, E, TOPK, rows, shared_exl3=False)
+    with pytest.raises(ValueError, match="reserve_bf16"):
+        m.shared_output
+    ws, ss = w.struct(), sw.struct()
+    L = gfr.lib()
+    assert L.gfr_moe_run_bf16(m._h, gfr._stream(), ctypes.byref(ws), x.data_ptr(), l.data_ptr(), ctypes.byref(ss),
+                              rows) == gfr.GFR_EINVAL and b"gfr_moe_reserve_bf16" in L.gfr_last_error()
+    other = gfr.Moe(hidden, N, E, TOPK, rows, shared_exl3=False)
+    other.run_bf16(w, x, l, sw, rows)                      # (its kernels are loaded before the capture)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="capture"):
+            m.run_bf16(w, x, l, sw, rows)
+        other.run_bf16(w, x, l, sw, rows)
+    m.run_bf16(w, x, l, sw, rows)
+    torch.cuda.synchronize()
+    want = m.output.clone()
+    for _ in range(3):
+        other.output.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(other.output, want)
+
+
+def test_no_bf16_buffers_for_an_exl3_shared_expert(gfr):
+    with pytest.raises(gfr.GfrError, match="EXL3"):
+        gfr.Moe(D, N, E, TOPK, 4).reserve_bf16()
