@@ -91,10 +91,25 @@ __device__ __forceinline__ void store_eight(void* p, int type, size_t i, f8_t v)
 __device__ __forceinline__ float times_logistic(float v, float z) {
     return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
+// v times the normal distribution's cumulative function: v h for v < 0 and v (1 - h) else, h = erfc(|v| / sqrt 2) / 2 the tail
+// beyond |v|. (0.5 v (1 + erf) cancels below v = -3.) h = exp(-v^2 / 2) t p(t) with t = 1 / (1 + 0.35 |v|): p is a
+// polynomial of degree 8 fitted to the scaled complement exp(x^2) erfc(x), within 2^-24.9 of it for |v| to 14, past where h
+// is a normal float. The exponential's argument is off by up to 1.5 v^2 2^-24: results below zero by v^2 2^-23 + 2^-20 of
+// themselves, others by 2^-20. 4096 x 16384 x 2048 (SiLU 233 us) takes 253 us, 298 with erfcf, 270 with the sum and erff.
+__device__ __forceinline__ float gelu(float v) {
+    constexpr float P[9] = {0.139621407f, 0.139861867f, 0.119832858f, 0.105508044f, -0.0231099185f,
+                            0.159174263f, -0.255714327f, 0.143971726f, -0.0291459356f};
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, fabsf(v), 1.f));
+    float p = P[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) p = fmaf(p, t, P[i]);
+    const float h = p * t * __builtin_amdgcn_exp2f(v * v * -0.72134752044448170f);
+    return v * (v < 0.f ? h : 1.f - h);
+}
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
     if constexpr (ACT == ACT_SILU) return times_logistic(v, v);
-    if constexpr (ACT == ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    if constexpr (ACT == ACT_GELU) return gelu(v);
     // 0.5 (1 + tanh(z)) = 1 / (1 + exp(-2 z))
     if constexpr (ACT == ACT_GELU_TANH) return times_logistic(v, 1.59576912160573072f * (v + 0.044715f * v * v * v));
     if constexpr (ACT == ACT_RELU) return v < 0.f ? 0.f : v;
@@ -103,10 +118,7 @@ __device__ __forceinline__ float activate(float v) {
 template <int ACT>
 __device__ __forceinline__ void activate_eight(f8_t& v) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        v[j] = activate<ACT>(v[j]);
-        if constexpr (ACT == ACT_GELU) __builtin_amdgcn_sched_barrier(0);   // eight of them at once would take many registers
-    }
+    for (int j = 0; j < 8; ++j) v[j] = activate<ACT>(v[j]);
 }
 // Sums with their bias (and the up matrix's, with its own) to the values before the residual. Comparisons that keep a NaN.
 template <bool GATED>

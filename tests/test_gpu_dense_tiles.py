@@ -106,3 +106,36 @@ def test_far_apart_rows(gfr, far, rows, n, k, gated, off):
         assert (taken >= 16) == bool(off) and (taken % 16 < 5) == (stride > 1 << 22)
         check(f(a, b, out_dtype=torch.float32), want, f"{far} {stride} form {taken}")
         del buf, view, a, b
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300, 2000])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_where_they_vanish(gfr, rows, gated, act):
+    """Single products (exact in fp32) through each activation from -13 to 13, relative to the value itself, fp32 out.
+
+    gelu = v / 2 erfc(t), t = -v / sqrt 2: erfc falls by the factor 1 - 2 t^2 e (t > 1) where t is off by a share e of it,
+    here two roundings, 2^-23: v^2 2^-23; the rest within 2^-20. silu = v / (1 +
+    exp(-v)): the exponential's argument is off by two roundings, |v| 2^-23; exp2, the sum, the quotient and a product (one
+    unit each) within 2^-21. gelu_tanh the same with 2 z = 2 sqrt(2 / pi) (v + 0.044715 v^3) in the place of v, which takes
+    seven roundings more: |2 z| 2^-21. Values below 2^-100 may be flushed."""
+    v = torch.cat((torch.arange(-13 * 64, 13 * 64, device="cuda") / 64, torch.tensor([-0.001, 0.001, 0.0], device="cuda")))
+    v = v.to(torch.float16)
+    n, k = v.numel(), 64
+    w = torch.zeros(2 * n if gated else n, k, dtype=torch.float16, device="cuda")
+    x = torch.zeros(rows, k, dtype=torch.float16, device="cuda")
+    x[:, 3] = 1
+    w[:n, 3] = v
+    if gated:
+        w[n:, 3] = 1
+    y = (gfr.dense_gated if gated else gfr.dense)(x, w, activation=act, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    d = v.double()
+    if act == "gelu":
+        want, rel = 0.5 * d * torch.special.erfc(-d / 2 ** 0.5), d * d * 2.0 ** -23 + 2.0 ** -20
+    else:
+        z = d if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (d + 0.044715 * d ** 3)
+        want, rel = d / (1 + torch.exp(-z)), z.abs() * 2.0 ** (-23 if act == "silu" else -21) + 2.0 ** -21
+    over = (y.double() - want).abs() - (rel * want.abs() + 2.0 ** -100)
+    i = int(over.max(0).values.argmax())
+    assert (over <= 0).all(), f"{act}({d[i].item()}): {y[0, i].item():.6g}, want {want[i].item():.6g}"
