@@ -19,10 +19,6 @@ __device__ __forceinline__ void load_lds16_s(uint64_t sbase, uint32_t voff, uint
     __asm__ volatile("s_mov_b64 exec, %3\n\ts_mov_b64 vcc, %1\n\tglobal_load_lds_dwordx4 %0, vcc\n\ts_mov_b64 exec, -1"
                      :: "v"(voff), "s"(sbase), "{m0}"(m0), "s"(mask) : "memory", "vcc");
 }
-// The same with every lane loading.
-__device__ __forceinline__ void load_lds16(uint64_t sbase, uint32_t voff, uint32_t m0) {
-    __asm__ volatile("s_mov_b64 vcc, %1\n\tglobal_load_lds_dwordx4 %0, vcc" :: "v"(voff), "s"(sbase), "{m0}"(m0) : "memory", "vcc");
-}
 // The LDS address (m0's unit) of shared memory.
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
