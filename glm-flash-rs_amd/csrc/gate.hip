@@ -302,9 +302,13 @@ __device__ __forceinline__ bool pick_fast(const GateJob& g, const RowLanes<W>& r
     }
     sort_down<PER>(k);
 
-    // The error of a choice: 32 units of the largest score (its exponential, the sum of up to 1024 of them in at most 38
-    // additions of positive terms, whose roundings mostly cancel but are all counted, and the quotient) and 20 of the
-    // choice itself (its sum's rounding and the low bits).
+    // The error of a choice, in units of 2^-24. A score is off by at most 48 of the row's largest (softmax) or 8 (sigmoid):
+    //   softmax: an exponential's argument l - top = -d takes three roundings and its value two units, 3 d + 2 of itself,
+    //   at most 3.1 of the largest (d exp(-d) < 0.37); the sum of up to 1024 of them the exponentials' own, 3 x 4.4 + 2
+    //   (the mean d, weighted with exp(-d), is below 4.4), and 22 additions of positive terms (16 in a lane, 6 over the
+    //   lanes); the reciprocal and two products 4; sigmoid: s (1 - s) (3 |l| + 2) + 4 < 6.
+    // The choice adds its sum's rounding and the 15 units in the last place that the low bits hide: 31 of itself, at
+    // most 36 of its neighbour. Two such errors meet, and twice that is taken.
     constexpr float UNIT = 0x1p-24f;
     const float score_error = g.bias ? (g.softmax ? 48.f * inverse : 8.f) * UNIT : 0.f;
     const auto doubt = [&](float x) { return exact ? -1.f : 4.f * (score_error + 36.f * UNIT * fabsf(x)); };
@@ -324,7 +328,8 @@ __device__ __forceinline__ bool pick_fast(const GateJob& g, const RowLanes<W>& r
                     if (g.softmax) return (x == top ? 1.f : __builtin_amdgcn_exp2f((x - top) * LOG2E)) * inverse;
                     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -LOG2E));
                 };
-                // a key's hidden bits move the score by its slope (at most the score, a sigmoid's a quarter) times them
+                // of two scores a group, two groups: a key's hidden bits (30 units of the logit) move a score by its slope
+                // (at most the score, a sigmoid's a quarter) times them
                 error = 4.f * UNIT * (g.softmax ? (48.f + 36.f * fmaxf(fabsf(va), fabsf(vb))) * inverse
                                                 : 8.f + 9.f * fmaxf(fabsf(va), fabsf(vb)));
                 va = score(va), vb = score(vb);
