@@ -913,7 +913,8 @@ def _row_stride(t) -> int:
 
 def route_gate(logits: torch.Tensor, gate: Gate, topk: int, shared: bool = True, stream=None):
     """gfr_route_gate: (picks [rows, topk + 1] int32, weights [rows, topk + 1] fp32) of logits [rows, routed] (fp32, bf16
-    or fp16), the shared expert's id = routed last; shared=False: [rows, topk] without it. A stream other than the current
+    or fp16), the shared expert's id = routed last; shared=False: [rows, topk] without it. In windows of other sizes a row's
+    softmax weights may differ in their last bits (the order of the sum); its picks do not. A stream other than the current
     one is the caller's to order after the inputs' writes; they have to stay alive until it is done."""
     rows, routed = logits.shape
     kind = _TYPE.get(logits.dtype)

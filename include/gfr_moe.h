@@ -279,7 +279,9 @@ int gfr_router_logits(hipStream_t stream, const uint16_t* input, int input_strid
  *               largest values stay (equal values: the lower group). groups = kept_groups = 1: no groups.
  *   picks     : the topk largest choices in the groups that stay, descending (equal choices: the lower id)
  *   weights   : score[pick], with renormalise divided by (the picks' sum in slot order + 1e-20), times scale
- * Choices and group values are compared as 64-bit arithmetic orders them; weights are fp32.
+ * Choices and group values are compared as 64-bit arithmetic orders them; weights are fp32. A row's picks and a sigmoid
+ * gate's weights do not depend on the other rows; a softmax's sum is taken in an order that follows the window's size, so
+ * that the same row in another window may have weights that differ in their last bits.
  * Masked experts: one whose logit is -inf or NaN, or whose choice is (a bias of -inf or NaN), is picked only when the
  * kept groups have fewer than topk others, by lower id and with weight 0. The softmax leaves out masked logits, group
  * values leave out masked experts (a group with one other has that one's choice as its sum; one with none comes last).
