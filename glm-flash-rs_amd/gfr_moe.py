@@ -560,15 +560,24 @@ class Moe(_Engine):
             _check(lib().gfr_moe_reserve_bf16(self._h))
             self._bf16_reserved = True
 
+    def _bf16_stream(self, sw: Bf16SharedWeights, stream) -> int:
+        """The checks of a run_bf16 that the library cannot make, its buffers, and the stream's handle."""
+        here = _get_device()
+        for t in (self.output, sw.gu, sw.down):
+            if t.get_device() != here:
+                raise ValueError(f"layer or shared expert on {t.device}, the current device is cuda:{here}")
+        handle = _handle(stream, here)
+        self.reserve_bf16()
+        return handle
+
     def run_bf16(self, w: Exl3Experts, input: torch.Tensor, logits: torch.Tensor, sw: Bf16SharedWeights, rows: int,
                  stream=None):
         """The layer with an unquantised shared expert (a layer made with shared_exl3=False): gfr_moe_run_bf16. input
         [rows, hidden] bf16 and logits [rows, routed] fp32, contiguous. The first run may allocate (reserve_bf16)."""
         self._check_rows(input, torch.bfloat16, self.hidden, rows, "input")
         self._check_rows(logits, torch.float32, self.routed, rows, "logits")
-        self.reserve_bf16()
-        ws, ss = w.struct(), sw.struct()
-        _check(lib().gfr_moe_run_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input), _ptr(logits),
+        handle, ws, ss = self._bf16_stream(sw, stream), w.struct(), sw.struct()
+        _check(lib().gfr_moe_run_bf16(self._h, handle, ctypes.byref(ws), _ptr(input), _ptr(logits),
                                       ctypes.byref(ss), rows))
 
     def run_router_bf16(self, w: Exl3Experts, input: torch.Tensor, router_weight: torch.Tensor, sw: Bf16SharedWeights,
@@ -576,9 +585,8 @@ class Moe(_Engine):
         """run_bf16 with the router logits computed from the hidden rows first (router_weight [routed, hidden])."""
         self._check_rows(input, torch.bfloat16, self.hidden, rows, "input")
         self._check_rows(router_weight, torch.bfloat16, self.hidden, self.routed, "router weight")
-        self.reserve_bf16()
-        ws, ss = w.struct(), sw.struct()
-        _check(lib().gfr_moe_run_router_bf16(self._h, _stream(stream), ctypes.byref(ws), _ptr(input),
+        handle, ws, ss = self._bf16_stream(sw, stream), w.struct(), sw.struct()
+        _check(lib().gfr_moe_run_router_bf16(self._h, handle, ctypes.byref(ws), _ptr(input),
                                              _ptr(router_weight), ctypes.byref(ss), rows))
 
     @property

@@ -139,3 +139,25 @@ def test_bf16_run_without_its_buffers(gfr):
 def test_no_bf16_buffers_for_an_exl3_shared_expert(gfr):
     with pytest.raises(gfr.GfrError, match="EXL3"):
         gfr.Moe(D, N, E, TOPK, 4).reserve_bf16()
+
+
+def test_bf16_run_on_another_device_is_refused(gfr, layer_weights, monkeypatch):
+    """A launch goes to the current device's stream: the layer, the shared expert's weights and a given stream have to be
+    on it."""
+    import synth
+    w, rows = layer_weights[1], 2
+    x, l, rw, sw = synth.activations(rows, D, 1), synth.logits(rows, E, 1), router_weight(D), bf16_shared(gfr, D, N)
+    m = gfr.Moe(D, N, E, TOPK, rows, shared_exl3=False)
+    host = gfr.Bf16SharedWeights(sw.gu, sw.down.cpu())
+    with pytest.raises(ValueError, match="shared expert on cpu"):
+        m.run_bf16(w, x, l, host, rows)
+
+    class Elsewhere:
+        device_index, cuda_stream = 1, 0
+
+    with pytest.raises(ValueError, match="stream of cuda:1"):
+        m.run_bf16(w, x, l, sw, rows, stream=Elsewhere())
+    monkeypatch.setattr(gfr, "_get_device", lambda: 1)
+    for run, arg in ((m.run_bf16, l), (m.run_router_bf16, rw)):
+        with pytest.raises(ValueError, match="current device is cuda:1"):
+            run(w, x, arg, sw, rows)
