@@ -11,9 +11,11 @@
 // An expert whose logit or choice is -inf or NaN is masked: no group value counts it, the softmax leaves out its logit,
 // and it is picked only where a row's kept groups have too few others, by lower id, with weight 0.
 //
-// Bound by its operations, not by the logits it reads: 32768 rows of 256 (the first gate above) take 29 us, 7 of them the
-// bytes' at a copy's rate, with about 300 VALU operations a row: a fifth the scores, a fifth the keys and their sort, a
-// third the rounds. In 64-bit arithmetic throughout, a wave a row, they took 65.
+// 32768 rows of 256 (the first gate above) take 29 us, the bytes 7 of them at a copy's rate. Half of the 29 does not grow
+// with the rows: a launch, one wave's chain of loads, sort and rounds, and behind it the 64-bit order of near choices (one
+// wave of 27; one of 320 decides everything again). The other half, 13 to 14 us per 32768 rows, is about the issue of 316
+// VALU instructions a row: a fifth the scores, a fifth the keys and their sort, a third the rounds. A third of the wave
+// cycles wait. In 64-bit arithmetic throughout, a wave a row, they took 65 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

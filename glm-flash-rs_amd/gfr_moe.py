@@ -994,10 +994,9 @@ def _dense(x, w, n, gated, bias, activation, limit, residual, out, out_dtype, st
 def dense(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, activation: str = None,
           residual: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
     """gfr_dense_run: act(x w^T + bias) + residual for x [rows, k] and w [n, k] of one 16-bit type; bias [n], residual and
-    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself; any other
-    memory that out shares with an operand is refused. No gradient is recorded.
-    A stream other than the current one is the caller's to order after the inputs' writes; they have to stay alive until it
-    is done."""
+    out [rows, n] in that type or fp32 (out: x's type by default). residual may be out itself; an out that
+    shares memory with an operand in any other way is refused, as are zero rows. No gradient is recorded. A stream other
+    than the current one is the caller's to order after the inputs' writes; they have to stay alive until it is done."""
     return _dense(x, w, w.shape[0], 0, bias, activation, 0.0, residual, out, out_dtype, stream)
 
 
@@ -1005,7 +1004,8 @@ def dense_gated(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, act
                 limit: float = None, residual: torch.Tensor = None, out: torch.Tensor = None,
                 out_dtype: torch.dtype = None, stream=None):
     """gfr_dense_run, gated: act(min(g, limit)) * clamp(u, -limit, limit) + residual, g and u the halves of x w^T + bias
-    for w [2 n, k] (gate rows, then up rows); limit None or 0: none. Otherwise as dense."""
+    for w [2 n, k] (gate rows, then up rows); limit None or 0: none. Otherwise as dense. An MLP's activations between
+    this and dense are rounded to x's type, as dense takes 16-bit rows."""
     if w.shape[0] % 2:
         raise ValueError(f"w {tuple(w.shape)}: want an even number of rows, the gate's and the up matrix's")
     return _dense(x, w, w.shape[0] // 2, 1, bias, activation, limit, residual, out, out_dtype, stream)

@@ -218,7 +218,7 @@ int gfr_shared_fp8_destroy(gfr_shared_fp8* sh);
 /* Moe::run_prefetched with its FP8 shared expert (moe.rs:66-182), for a layer made with gfr_moe_create_shared(...,
  * shared_exl3 = 0) and hidden a multiple of 512: the shared expert into the layer's own buffer
  * (gfr_moe_shared_output, [max_rows][hidden] fp32), then gfr_moe_run_shared with it, in the same launches where these
- * have room (one token; up to 16 rows on the prefill engine). _router_fp8 computes the router
+ * have room (one token; up to 16 rows on the prefill engine; not under gfr_moe_set_gate). _router_fp8 computes the router
  * logits first, as gfr_moe_run_router. Input rows [rows][hidden] bf16, 16-byte aligned. */
 int gfr_moe_run_fp8(gfr_moe* m, hipStream_t stream, const gfr_exl3_experts* w, const uint16_t* input,
                     const float* logits, const gfr_fp8_shared_weights* sw, int rows);
@@ -286,7 +286,8 @@ int gfr_router_logits(hipStream_t stream, const uint16_t* input, int input_strid
  * kept groups have fewer than topk others, by lower id and with weight 0. The softmax leaves out masked logits, group
  * values leave out masked experts (a group with one other has that one's choice as its sum; one with none comes last).
  * A row of masked experts only gets the lowest ids, all with weight 0. Several logits of +inf share a softmax equally.
- * routed <= 1024, groups <= 64 (a divisor of routed), topk <= 31 and at most the kept groups' experts, scale > 0. */
+ * At least one row; routed <= 1024, groups <= 64 (a divisor of routed), topk <= 31 and at most the kept groups' experts,
+ * scale > 0. */
 #define GFR_BF16 0
 #define GFR_F16 1
 #define GFR_F32 2
@@ -308,7 +309,8 @@ int gfr_route_gate(hipStream_t stream, const void* logits, int logits_type, int6
  * aligned pointers, strides a multiple of 8) are the fast ones. Columns of x and w from k on are not read. residual may
  * be out itself (address, type and stride); an out that shares memory with an operand in any other way is refused. A row's
  * sums do not depend on the other rows' values, but windows of other sizes may take them in another order (all in fp32).
- * No scratch: calls may overlap on any streams. */
+ * No scratch: calls may overlap on any streams. At least one row, column and k. Two products in turn, as an MLP's, round
+ * the rows between them to `type`, half a step, since x is 16 bits wide. */
 #define GFR_ACT_NONE 0
 #define GFR_ACT_RELU 1
 #define GFR_ACT_GELU 2
