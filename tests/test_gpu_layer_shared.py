@@ -161,3 +161,65 @@ def test_bf16_run_on_another_device_is_refused(gfr, layer_weights, monkeypatch):
     for run, arg in ((m.run_bf16, l), (m.run_router_bf16, rw)):
         with pytest.raises(ValueError, match="current device is cuda:1"):
             run(w, x, arg, sw, rows)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20, 40, 300])
+def test_gate_with_the_shared_expert_on_a_branch(gfr, layer_weights, rows):
+    """The bf16 shared expert's products on the branch stream (dense_gated and dense with its stream) beside the layer
+    under the general gate: byte-equal to run_bf16, eagerly and in every replay of a graph."""
+    import synth
+    w, sw = layer_weights[1], bf16_shared(gfr, D, N)
+    x, l = synth.activations(rows, D, rows), synth.logits(rows, E, rows)
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(5)).cuda() * 0.02
+    m = gfr.Moe(D, N, E, TOPK, rows, shared_exl3=False)
+    m.set_gate(gfr.Gate(bias=bias, groups=6, kept_groups=3, scale=2.5))
+    m.run_bf16(w, x, l, sw, rows)
+    torch.cuda.synchronize()
+    want = m.output.clone()
+    shared = torch.empty(rows, D, device="cuda")
+    branch, main = gfr.SharedBranch(), torch.cuda.Stream()
+
+    def layer():
+        shared.fill_(float("nan"))
+
+        def shared_fn(side):
+            gfr.dense(gfr.dense_gated(x, sw.gu, limit=2.0, stream=side), sw.down, out=shared, stream=side)
+
+        branch.run(main, shared_fn, lambda ready: m.run(w, x, l, rows, stream=main, shared=shared, shared_ready=ready))
+
+    with torch.cuda.stream(main):
+        m.output.zero_()
+        layer()
+    torch.cuda.synchronize()
+    assert torch.equal(m.output, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(main):
+        with torch.cuda.graph(graph, stream=main):
+            layer()
+    for _ in range(3):
+        m.output.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(main):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(m.output, want)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 20, 300])
+def test_router_logits_then_the_gate(gfr, layer_weights, rows):
+    """run_router under the general gate: the picks and weights of route_gate on the router's logits."""
+    import synth
+    w, rw = layer_weights[0], router_weight(D)
+    x = synth.activations(rows, D, rows)
+    gate = gfr.Gate(score="softmax", groups=4, kept_groups=2, group_score="max", renormalise=False, scale=1.5)
+    m = gfr.Moe(D, N, E, TOPK, rows)
+    m.set_gate(gate)
+    m.run_router(w, x, rw, rows)
+    logits = gfr.router_logits(x, rw)
+    p, wt = gfr.route_gate(logits, gate, TOPK)
+    torch.cuda.synchronize()
+    assert torch.equal(m.picks, p) and torch.equal(m.weights, wt)
+    got = m.output.clone()
+    m.run(w, x, logits, rows)
+    torch.cuda.synchronize()
+    assert torch.equal(m.output, got)
