@@ -42,8 +42,10 @@ int alloc_zero(T** p, size_t count, const char* what) {
     if (count == 0) count = 1;
     hipError_t e = hipMalloc((void**)p, count * sizeof(T));
     if (e != hipSuccess) return hip_fail(e, what);
-    e = hipMemset(*p, 0, count * sizeof(T));
-    if (e != hipSuccess) return hip_fail(e, what);
+    // waited for: a fill of device memory may return before it is done, and a stream that does not wait for the null stream
+    // (torch's do not) could have a first run's results cleared
+    if ((e = hipMemset(*p, 0, count * sizeof(T))) != hipSuccess || (e = hipStreamSynchronize(nullptr)) != hipSuccess)
+        return hip_fail(e, what);
     return 0;
 }
 

@@ -223,3 +223,25 @@ def test_router_logits_then_the_gate(gfr, layer_weights, rows):
     m.run(w, x, logits, rows)
     torch.cuda.synchronize()
     assert torch.equal(m.output, got)
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+def test_first_run_right_after_the_buffers(gfr, layer_weights, rows):
+    """A layer made, its buffers reserved and run at once on a stream of the caller's: the buffers' clearing is over by
+    then (the bytes of a run after a synchronization)."""
+    import synth
+    hidden = 768
+    w, sw = synth.experts(E, hidden, N, BITS, seed=6), bf16_shared(gfr, hidden, N)
+    x, l = synth.activations(rows, hidden, rows), synth.logits(rows, E, rows)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(3):
+        m = gfr.Moe(hidden, N, E, TOPK, 8192, shared_exl3=False)
+        m.run_bf16(w, x, l, sw, rows, stream=s)
+        s.synchronize()
+        first = m.output[:rows].clone(), m.shared_output[:rows].clone(), m.picks[:rows].clone(), m.weights[:rows].clone()
+        torch.cuda.synchronize()
+        m.run_bf16(w, x, l, sw, rows)
+        torch.cuda.synchronize()
+        for a, b in zip(first, (m.output, m.shared_output, m.picks, m.weights)):
+            assert torch.equal(a, b[:rows])
