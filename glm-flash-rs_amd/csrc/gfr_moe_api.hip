@@ -158,6 +158,11 @@ bool overlap(RowBytes a, RowBytes b) {
 // The general gate's checks, and its launch's arguments
 bool known_type(int t) { return t == GFR_BF16 || t == GFR_F16 || t == GFR_F32; }
 size_t type_bytes(int t) { return t == GFR_F32 ? 4 : 2; }
+constexpr int64_t FAR = (int64_t)1 << 31;                         // the widest stride of the row operators
+RowBytes rows_of(const void* p, int type, int64_t rows, int64_t columns, int64_t stride) {
+    const int64_t e = (int64_t)type_bytes(type);
+    return RowBytes{reinterpret_cast<uintptr_t>(p), columns * e, stride * e, rows};
+}
 bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 int check_gate(const gfr_gate* g, int routed, int topk) {
     if (!g) return fail(GFR_EINVAL, "null gate");
@@ -464,8 +469,7 @@ int dense_job(const gfr_dense* d, gfr::DenseJob& job) {
     if (d->out_stride < d->n || (d->residual && d->residual_stride < d->n))
         return fail(GFR_EINVAL, "dense: strides of out %lld and residual %lld below n %d", (long long)d->out_stride,
                     (long long)d->residual_stride, d->n);
-    const int64_t far = (int64_t)1 << 31;
-    if (d->x_stride > far || d->w_stride > far || d->out_stride > far || (d->residual && d->residual_stride > far))
+    if (d->x_stride > FAR || d->w_stride > FAR || d->out_stride > FAR || (d->residual && d->residual_stride > FAR))
         return fail(GFR_EINVAL, "dense: a stride above 2^31");
     if (!aligned(d->x, 2) || !aligned(d->w, 2) || !aligned(d->out, type_bytes(d->out_type)) ||
         (d->bias && !aligned(d->bias, type_bytes(d->bias_type))) ||
@@ -475,10 +479,6 @@ int dense_job(const gfr_dense* d, gfr::DenseJob& job) {
     if (((int64_t)d->rows + 63) / 64 * (((int64_t)d->n + 31) / 32) >= ((int64_t)1 << 23) - 256)
         return fail(GFR_EINVAL, "dense: %d rows of %d columns are too many tiles for a launch", d->rows, d->n);
     // a workgroup stores its part of out while others still read theirs of the operands
-    const auto rows_of = [](const void* p, int type, int64_t rows, int64_t columns, int64_t stride) {
-        const int64_t e = (int64_t)type_bytes(type);
-        return RowBytes{reinterpret_cast<uintptr_t>(p), columns * e, stride * e, rows};
-    };
     const int64_t wrows = (int64_t)d->n * (1 + d->gated);
     const RowBytes out = rows_of(d->out, d->out_type, d->rows, d->n, d->out_stride);
     const bool in_place = d->residual == d->out && d->residual_type == d->out_type &&
@@ -512,6 +512,86 @@ int gfr_dense_form(const gfr_dense* d) {
     gfr::DenseJob job;
     int rc = dense_job(d, job);
     return rc ? rc : gfr::dense_form(job);
+}
+
+// ---- norms around a block -----------------------------------------------------------------------------------------
+}  // extern "C"
+namespace {
+int norm_part(const gfr_norm& g, const char* which, gfr::NormPart& p) {
+    if (g.kind < GFR_NORM_NONE || g.kind > GFR_NORM_LAYER) return fail(GFR_EINVAL, "norm: %s kind %d", which, g.kind);
+    p = {g.kind == GFR_NORM_LAYER, g.weight_type, g.bias_type, g.weight, g.bias, g.eps, g.offset};
+    if (g.kind == GFR_NORM_NONE) {
+        if (g.weight || g.bias) return fail(GFR_EINVAL, "norm: %s has a weight or bias and no kind", which);
+        return 0;
+    }
+    if (!(g.eps >= 0.f) || g.eps > 3.4e38f) return fail(GFR_EINVAL, "norm: %s eps %g", which, (double)g.eps);
+    if (!(g.offset >= -3.4e38f && g.offset <= 3.4e38f)) return fail(GFR_EINVAL, "norm: %s offset %g", which, (double)g.offset);
+    if ((g.weight && !known_type(g.weight_type)) || (g.bias && !known_type(g.bias_type)))
+        return fail(GFR_EINVAL, "norm: %s types %d and %d of weight and bias", which, g.weight_type, g.bias_type);
+    if ((g.weight && !aligned(g.weight, type_bytes(g.weight_type))) || (g.bias && !aligned(g.bias, type_bytes(g.bias_type))))
+        return fail(GFR_EINVAL, "norm: tensors must be aligned to their elements");
+    return 0;
+}
+int norm_job(const gfr_block_norm* d, gfr::NormJob& job) {
+    if (!d) return fail(GFR_EINVAL, "norm: null argument");
+    if (d->rows <= 0 || d->n <= 0 || d->n > 32768) return fail(GFR_EINVAL, "norm: rows %d, n %d (1..32768)", d->rows, d->n);
+    if (!d->x || (!d->h && !d->y)) return fail(GFR_EINVAL, "norm: null argument");
+    gfr::NormPart post, pre;
+    int rc = norm_part(d->post, "post", post);
+    if (rc || (rc = norm_part(d->pre, "pre", pre))) return rc;
+    if ((d->pre.kind != GFR_NORM_NONE) != (d->y != nullptr)) return fail(GFR_EINVAL, "norm: y and pre go together");
+    if (d->gate_column != 0 && d->gate_column != 1) return fail(GFR_EINVAL, "norm: gate column %d: 0 or 1", d->gate_column);
+    if (d->sigmoid != 0 && d->sigmoid != 1) return fail(GFR_EINVAL, "norm: sigmoid %d: 0 or 1", d->sigmoid);
+    if (!(d->scale >= -3.4e38f && d->scale <= 3.4e38f && d->residual_scale >= -3.4e38f && d->residual_scale <= 3.4e38f))
+        return fail(GFR_EINVAL, "norm: scales %g and %g must be finite", (double)d->scale, (double)d->residual_scale);
+    struct Operand {
+        const char* name;
+        const void* at;
+        int type;
+        int64_t stride, columns, rows;
+    };
+    const int64_t rows = d->rows, n = d->n;
+    const Operand all[] = {{"x", d->x, d->x_type, d->x_stride, n, rows},
+                           {"residual", d->residual, d->residual_type, d->residual_stride, n, rows},
+                           {"gate", d->gate, d->gate_type, d->gate_row ? d->gate_row : n, d->gate_column ? n : 1,
+                            d->gate_row ? rows : 1},
+                           {"h", d->h, d->h_type, d->h_stride, n, rows},
+                           {"y", d->y, d->y_type, d->y_stride, n, rows},
+                           {"post weight", d->post.weight, d->post.weight_type, n, n, 1},
+                           {"post bias", d->post.bias, d->post.bias_type, n, n, 1},
+                           {"pre weight", d->pre.weight, d->pre.weight_type, n, n, 1},
+                           {"pre bias", d->pre.bias, d->pre.bias_type, n, n, 1}};
+    for (const Operand& o : all) {
+        if (!o.at) continue;
+        if (!known_type(o.type)) return fail(GFR_EINVAL, "norm: %s type %d", o.name, o.type);
+        if (o.stride < o.columns || o.stride > FAR)
+            return fail(GFR_EINVAL, "norm: %s stride %lld outside %lld..2^31", o.name, (long long)o.stride, (long long)o.columns);
+        if (!aligned(o.at, type_bytes(o.type))) return fail(GFR_EINVAL, "norm: tensors must be aligned to their elements");
+    }
+    // a lane stores the columns that it has read, and other lanes' rows and columns may still be read after that
+    for (int out = 3; out <= 4; ++out)
+        for (int i = 0; i < 9; ++i) {
+            const Operand &a = all[out], &b = all[i];
+            if (i == out || !a.at || !b.at) continue;
+            const bool itself = i < 2 && b.at == a.at && b.type == a.type && (rows == 1 || b.stride == a.stride);
+            if (!itself && overlap(rows_of(a.at, a.type, a.rows, a.columns, a.stride), rows_of(b.at, b.type, b.rows, b.columns, b.stride)))
+                return fail(GFR_EINVAL, "norm: %s overlaps %s", a.name, b.name);
+        }
+    job = {d->x, d->residual, d->gate, d->h, d->y, d->x_stride, d->residual_stride, d->gate_row, d->h_stride, d->y_stride,
+           d->rows, d->n, d->x_type, d->residual_type, d->gate_type, d->h_type, d->y_type, d->gate_column, d->sigmoid != 0,
+           d->post.kind != GFR_NORM_NONE, d->scale, d->residual_scale, post, pre, 0.f};
+    return 0;
+}
+}  // namespace
+extern "C" {
+
+int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d) {
+    gfr::NormJob job;
+    int rc = norm_job(d, job);
+    if (rc) return rc;
+    hipError_t e = gfr::launch_norm(stream, job);
+    if (e != hipSuccess) return hip_fail(e, "norm");
+    return 0;
 }
 
 // ---- debug rotation ---------------------------------------------------------------------------------------------

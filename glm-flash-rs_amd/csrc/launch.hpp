@@ -166,6 +166,34 @@ hipError_t launch_dense(hipStream_t s, DenseJob d);
 // The form that launch_dense takes (gfr_dense_form's numbers); host only.
 int dense_form(const DenseJob& d);
 
+// norm.hip
+// A norm: (z - mean) / sqrt(mean of squares + eps) * (weight + offset) + bias; layer false: the mean is taken as 0.
+struct NormPart {
+    bool layer;
+    int weight_type, bias_type;
+    const void* weight;
+    const void* bias;
+    float eps, offset;
+};
+// v = post(x) * gate (gate_col 1: an element a column, 0: one a row; gate_row: elements between rows, 0 for one row of
+// them); h = residual_scale * residual + scale * v; y = pre(h). n <= 32768.
+struct NormJob {
+    const void* x;
+    const void* residual;
+    const void* gate;
+    void* h;
+    void* y;
+    int64_t x_stride, residual_stride, gate_row, h_stride, y_stride;
+    int rows, n;
+    int x_type, residual_type, gate_type, h_type, y_type;
+    int gate_col;
+    bool sigmoid, has_post;
+    float scale, residual_scale;
+    NormPart post, pre;
+    float per_column;               // set by launch_norm: 1 / n
+};
+hipError_t launch_norm(hipStream_t s, NormJob d);
+
 // shared_fp8.hip
 // The reference's FP8 shared expert (moe.rs:132-167) for rows [rows][x_stride] bf16: gate/up (8 K slices, bf16 gu
 // [rows][2 inter], limited SwiGLU -> act [rows][inter] bf16), then down -> out [rows][out_stride] fp32. hidden a

@@ -109,6 +109,7 @@ def _load() -> ctypes.CDLL:
         "gfr_moe_set_gate": ([VP, P], I),
         "gfr_dense_run": ([P, P], I),
         "gfr_dense_form": ([P], I),
+        "gfr_block_norm_run": ([P, P], I),
         "gfr_moe_reserve_bf16": ([VP], I),
         "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
@@ -373,10 +374,43 @@ class Gate:
                           self.scale, 0 if bias is None else bias.data_ptr())
 
 
-# gfr_gate and gfr_dense as bytes in the machine's layout: packed anew for every call, which a ctypes structure of as many
-# fields takes about three times as long for
+_NORMS = {"rms": 1, "layer": 2}
+
+
+@dataclass
+class Norm:
+    """A norm over a row's columns (gfr_norm): kind "rms" or "layer" (which takes the mean off first), then times
+    weight + offset and plus bias; weight and bias [n], bf16, fp16 or fp32 (None: 1 and 0). offset 1 is for weights that are
+    stored less one."""
+
+    kind: str = "rms"
+    weight: torch.Tensor = None
+    bias: torch.Tensor = None
+    eps: float = 1e-6
+    offset: float = 0.0
+
+    def fields(self, n: int, here: int):
+        """gfr_norm's values."""
+        kind, w, b = _NORMS.get(self.kind), self.weight, self.bias
+        if kind is None:
+            raise ValueError(f"norm kind {self.kind!r} of {list(_NORMS)}")
+        for t in (w, b):
+            if t is None:
+                continue
+            if t.shape != (n,) or t.dtype not in _TYPE or not t.is_contiguous():
+                raise ValueError(f"norm weight or bias {tuple(t.shape)} {t.dtype}: want ({n},) bf16, fp16 or fp32, contiguous")
+            if t.get_device() != here:
+                _elsewhere(t)
+        return (kind, 0 if w is None else _TYPE[w.dtype], 0 if b is None else _TYPE[b.dtype], self.eps, self.offset,
+                0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr())
+
+
+_NO_NORM = (0, 0, 0, 0.0, 0.0, 0, 0)
+# gfr_gate, gfr_dense and gfr_block_norm as bytes in the machine's layout: packed anew for every call, which a ctypes
+# structure of as many fields takes about three times as long for
 _GATE = struct.Struct("@5ifP")
 _DENSE = struct.Struct("@4iPqPq2ifiP2iPqPq")
+_BLOCK_NORM = struct.Struct("@9i2fPqPqPqPqPq3i2f2P3i2f2P")
 
 
 class _Engine:
@@ -1009,6 +1043,88 @@ def dense_gated(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, act
     if w.shape[0] % 2:
         raise ValueError(f"w {tuple(w.shape)}: want an even number of rows, the gate's and the up matrix's")
     return _dense(x, w, w.shape[0] // 2, 1, bias, activation, limit, residual, out, out_dtype, stream)
+
+
+def _result(out, shape, dtype, like, stream, here, name="out"):
+    """A new output, or the caller's own after its checks."""
+    if out is None:
+        return _empty(shape, dtype, like, stream)
+    if out.shape != shape or out.dtype not in _TYPE:
+        raise ValueError(f"{name} {tuple(out.shape)} {out.dtype}: want {tuple(shape)} in bf16, fp16 or fp32")
+    if out.get_device() != here:
+        _elsewhere(out)
+    return out
+
+
+def _block_norm(x, residual, pre, post, gate, gate_activation, scale, residual_scale, keep, h, out, out_dtype, stream):
+    rows, n = x.shape
+    shape, types, here = x.shape, _TYPE, _get_device()
+    x_type = types.get(x.dtype)
+    if x_type is None:
+        raise ValueError(f"x {x.dtype}: bf16, fp16 or fp32")
+    if x.get_device() != here:
+        _elsewhere(x)
+    residual_at = residual_type = residual_stride = 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype not in types:
+            raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype}: want ({rows}, {n}) in bf16, fp16 or fp32")
+        if residual.get_device() != here:
+            _elsewhere(residual)
+        residual_at, residual_type, residual_stride = residual.data_ptr(), types[residual.dtype], _row_stride(residual)
+    gate_at = gate_type = gate_row = gate_column = 0
+    if gate is not None:
+        if gate.dtype not in types or gate.dim() > 2:
+            raise ValueError(f"gate {tuple(gate.shape)} {gate.dtype}: [n], [rows, 1], [1, n] or [rows, n] in bf16, fp16 or fp32")
+        if gate.get_device() != here:
+            _elsewhere(gate)
+        g = gate if gate.dim() == 2 else gate.reshape(1, -1)
+        if g.shape[0] not in (1, rows) or g.shape[1] not in (1, n):
+            raise ValueError(f"gate {tuple(gate.shape)}: [n], [rows, 1], [1, n] or [rows, n] of ({rows}, {n})")
+        gate_at, gate_type, gate_column = gate.data_ptr(), types[gate.dtype], int(g.shape[1] == n and n > 1)
+        gate_row = _row_stride(g) if g.shape[0] > 1 else 0
+    if gate_activation not in (None, "none", "sigmoid"):
+        raise ValueError(f"gate activation {gate_activation!r} of ['none', 'sigmoid']")
+    h_at = h_type = h_stride = y_at = y_type = y_stride = 0
+    if keep:
+        h = _result(h, shape, x.dtype if residual is None else residual.dtype, x, stream, here, "h")
+        h_at, h_type, h_stride = h.data_ptr(), types[h.dtype], _row_stride(h)
+    if pre is not None:
+        if out is not None and out_dtype is not None and out.dtype is not out_dtype:
+            raise ValueError(f"out {out.dtype}: want {out_dtype}")
+        if out_dtype is not None and out_dtype not in types:
+            raise ValueError(f"out {out_dtype}: bf16, fp16 or fp32")
+        out = _result(out, shape, out_dtype or x.dtype, x, stream, here)
+        y_at, y_type, y_stride = out.data_ptr(), types[out.dtype], _row_stride(out)
+    elif out is not None or out_dtype is not None:
+        raise ValueError("out is the pre norm's: want pre")
+    handle = _handle(stream, here)
+    rc = (_lib or lib()).gfr_block_norm_run(
+        handle, _BLOCK_NORM.pack(rows, n, x_type, residual_type, gate_type, h_type, y_type, gate_column,
+                                 int(gate_activation == "sigmoid"), scale, residual_scale, x.data_ptr(), _row_stride(x),
+                                 residual_at, residual_stride, gate_at, gate_row, h_at, h_stride, y_at, y_stride,
+                                 *(_NO_NORM if post is None else post.fields(n, here)),
+                                 *(_NO_NORM if pre is None else pre.fields(n, here))))
+    if rc:
+        _check(rc)
+    return h, out
+
+
+def block_norm(x: torch.Tensor, residual: torch.Tensor = None, pre: Norm = None, post: Norm = None,
+               gate: torch.Tensor = None, gate_activation: str = None, scale: float = 1.0, residual_scale: float = 1.0,
+               h: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
+    """gfr_block_norm_run, from a block's output x [rows, n] to the stream and the next block's rows: (h, y) with
+    h = residual_scale * residual + scale * gate * post(x) in the residual's type (x's where there is none) and y = pre(h) in
+    out_dtype (x's type by default; None without pre). gate: [n], [rows, 1], [1, n] or [rows, n], by its logistic function
+    where gate_activation is "sigmoid". bf16, fp16 or fp32 each. h and out may each be x or the residual itself; ones that
+    share memory with an operand in any other way are refused, as are zero rows. pre takes h before its rounding. No gradient
+    is recorded. A stream other than the current one is the caller's to order after the inputs' writes; they have to stay
+    alive until it is done."""
+    return _block_norm(x, residual, pre, post, gate, gate_activation, scale, residual_scale, True, h, out, out_dtype, stream)
+
+
+def norm(x: torch.Tensor, norm: Norm, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
+    """The norm alone: rows [rows, n] (a token's, or its heads') to out (x's type by default; may be x itself)."""
+    return _block_norm(x, None, norm, None, None, None, 1.0, 1.0, False, None, out, out_dtype, stream)[1]
 
 
 def rotate(x: torch.Tensor, expert: torch.Tensor, suh: torch.Tensor, stream=None) -> torch.Tensor:

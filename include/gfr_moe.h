@@ -342,6 +342,50 @@ int gfr_dense_run(hipStream_t stream, const gfr_dense* d);
  * + 16 where x's or w's rows are off 16-byte alignment. Negative: refused. */
 int gfr_dense_form(const gfr_dense* d);
 
+/* ---- The norms around a block, with its gate and residual -----------------------------------------------------
+ *   v = post(x) * f(gate);  h = residual_scale * residual + scale * v;  y = pre(h)
+ * a norm: (z - mean) / sqrt(mean of (z - mean)^2 + eps) * (weight + offset) + bias over a row's n columns, the mean 0 for
+ * GFR_NORM_RMS; f the identity, or the logistic function. x, residual, gate, h, y, the weights and biases each in any of
+ * GFR_BF16, GFR_F16, GFR_F32. post.kind GFR_NORM_NONE, gate, residual, weights and biases NULL: not there (a residual that
+ * is not there is 0, a weight that is not there 1). h or y may be NULL, and y is exactly where pre.kind is not
+ * GFR_NORM_NONE. The gate's element of row r and column c is gate[r * gate_row + c * gate_column], gate_column 0 or 1,
+ * gate_row 0 or any (at least n, or 1 where gate_column is 0). Values and statistics in fp32 (pre takes h before its rounding), one rounding an
+ * output. Strides count elements; any size, stride and element-aligned address works. h and y may each be x or the residual
+ * itself (address, type and stride); one that shares memory with another operand, or with the other, in any other way is
+ * refused. A row's results do not depend on the other rows, nor on how many there are. No scratch: calls may overlap on
+ * any streams. At least one row; n from 1 to 32768, eps >= 0, scales finite. */
+#define GFR_NORM_NONE 0
+#define GFR_NORM_RMS 1
+#define GFR_NORM_LAYER 2
+typedef struct gfr_norm {
+    int kind;
+    int weight_type;
+    int bias_type;
+    float eps;
+    float offset;
+    const void* weight;
+    const void* bias;
+} gfr_norm;
+typedef struct gfr_block_norm {
+    int rows, n;
+    int x_type, residual_type, gate_type, h_type, y_type;
+    int gate_column;
+    int sigmoid;
+    float scale, residual_scale;
+    const void* x;
+    int64_t x_stride;
+    const void* residual;
+    int64_t residual_stride;
+    const void* gate;
+    int64_t gate_row;
+    void* h;
+    int64_t h_stride;
+    void* y;
+    int64_t y_stride;
+    gfr_norm post, pre;
+} gfr_block_norm;
+int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d);
+
 /* ---- Single EXL3 linear (benchmark config 1; the decode path's GEMV with rot_in / down-epilogue formulas) ----
  * y [n] fp32 = svh * had(W^T xh) / sqrt(128), xh = fp16(had(x * suh) / sqrt(128)), x [kin] fp16. */
 typedef struct gfr_linear gfr_linear;

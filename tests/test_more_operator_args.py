@@ -1,0 +1,42 @@
+"""What the norms, the 16-bit experts and the log probabilities refuse: host checks before any launch (no GPU needed)."""
+import pytest
+
+
+def refused(rc, needle):
+    import gfr_moe
+    said = gfr_moe.lib().gfr_last_error().decode()
+    assert rc == gfr_moe.GFR_EINVAL and needle in said, said
+
+
+NORM = ("rows n x_type residual_type gate_type h_type y_type gate_column sigmoid scale residual_scale x x_stride residual "
+        "residual_stride gate gate_row h h_stride y y_stride").split()
+PART = "kind weight_type bias_type eps offset weight bias".split()
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(x=0), "null"), (dict(h=0, y=0, pre=dict(kind=0)), "null"), (dict(rows=0), "rows 0"), (dict(rows=-3), "rows -3"),
+    (dict(n=0), "n 0"), (dict(n=32769, x_stride=40000, h_stride=40000, y_stride=40000), "n 32769"),
+    (dict(pre=dict(kind=3)), "pre kind 3"), (dict(post=dict(kind=-1)), "post kind -1"),
+    (dict(post=dict(kind=0, weight=16)), "no kind"), (dict(pre=dict(eps=-1.0)), "eps"),
+    (dict(pre=dict(eps=float("nan"))), "eps"), (dict(pre=dict(offset=float("inf"))), "offset"),
+    (dict(pre=dict(weight=16, weight_type=3)), "types 3"), (dict(pre=dict(bias=18, bias_type=2)), "aligned"),
+    (dict(y=0), "go together"), (dict(pre=dict(kind=0)), "go together"), (dict(gate_column=2), "gate column 2"),
+    (dict(sigmoid=2), "sigmoid 2"), (dict(scale=float("inf")), "finite"), (dict(residual_scale=float("nan")), "finite"),
+    (dict(x_type=3), "x type 3"), (dict(h_type=-1), "h type -1"), (dict(x_stride=31), "x stride 31"),
+    (dict(y_stride=31), "y stride 31"), (dict(h_stride=(1 << 31) + 1), "h stride"),
+    (dict(residual=1 << 33, residual_stride=16), "residual stride 16"), (dict(gate=1 << 33, gate_row=16, gate_column=1), "gate stride"),
+    (dict(gate=1 << 33, gate_row=-1, gate_column=0), "gate stride"), (dict(x=17), "aligned"), (dict(h=(1 << 30) + 2, h_type=2), "aligned"),
+    (dict(h=64, h_stride=32), "h overlaps x"), (dict(x=1 << 20, h=1 << 20, h_type=2), "h overlaps x"),
+    (dict(x=1 << 20, y=1 << 20, y_stride=33), "y overlaps x"), (dict(y=1 << 30), "h overlaps y"),
+    (dict(gate=1 << 31, gate_row=32, gate_column=1), "y overlaps gate"),
+    (dict(pre=dict(weight=1 << 30)), "h overlaps pre weight"), (dict(post=dict(kind=2, bias=1 << 31)), "y overlaps post bias"),
+])
+def test_block_norm_refuses(kw, needle):
+    import gfr_moe
+    a = dict(rows=4, n=32, scale=1.0, residual_scale=1.0, x=16, x_stride=32, h=1 << 30, h_stride=32, y=1 << 31, y_stride=32)
+    parts = dict(post=dict(kind=0, eps=0.0, offset=0.0), pre=dict(kind=1, eps=1e-5, offset=0.0))
+    for k, v in kw.items():
+        parts[k].update(v) if k in parts else a.update({k: v})
+    st = gfr_moe._BLOCK_NORM.pack(*[a.get(n, 0) for n in NORM], *[parts[p].get(n, 0) for p in ("post", "pre") for n in PART])
+    refused(gfr_moe.lib().gfr_block_norm_run(None, st), needle)
+    refused(gfr_moe.lib().gfr_block_norm_run(None, None), "null")
