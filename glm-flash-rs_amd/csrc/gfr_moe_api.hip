@@ -594,6 +594,58 @@ int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d) {
     return 0;
 }
 
+// ---- log probabilities --------------------------------------------------------------------------------------------
+int64_t gfr_logprobs_workspace(int rows, int vocab, int top) {
+    if (rows <= 0 || vocab <= 0 || vocab > gfr::LOGPROBS_VOCAB || top < 0 || top > 32 || top > vocab)
+        return fail(GFR_EINVAL, "logprobs: rows %d, vocab %d (1..%d), top %d (0..32, at most vocab)", rows, vocab,
+                    gfr::LOGPROBS_VOCAB, top);
+    if ((int64_t)rows * gfr::logprobs_chunks(rows, vocab) >= 1 << 23)  // a launch's threads: 2^32, 512 a chunk
+        return fail(GFR_EINVAL, "logprobs: %d rows of %d logits are too many for a launch", rows, vocab);
+    return (int64_t)gfr::logprobs_workspace(rows, vocab, top);
+}
+
+int gfr_logprobs_run(hipStream_t stream, const gfr_logprobs* d) {
+    if (!d) return fail(GFR_EINVAL, "logprobs: null argument");
+    const int64_t need = gfr_logprobs_workspace(d->rows, d->vocab, d->top);
+    if (need < 0) return GFR_EINVAL;
+    if (d->tokens < 0 || d->tokens > 1 << 24) return fail(GFR_EINVAL, "logprobs: tokens %d outside 0..%d", d->tokens, 1 << 24);
+    if (!d->logits || !d->entropy || !d->workspace || (d->tokens && (!d->token || !d->logprobs)) ||
+        (d->top && (!d->top_ids || !d->top_logprobs)))
+        return fail(GFR_EINVAL, "logprobs: null argument");
+    if (!known_type(d->type)) return fail(GFR_EINVAL, "logprobs: logits type %d", d->type);
+    if (d->wide_tokens != 0 && d->wide_tokens != 1) return fail(GFR_EINVAL, "logprobs: wide tokens %d: 0 or 1", d->wide_tokens);
+    if (!(d->temperature >= 1e-6f && d->temperature <= 1e6f))
+        return fail(GFR_EINVAL, "logprobs: temperature %g outside 1e-6..1e6", (double)d->temperature);
+    if (d->stride < d->vocab || d->stride > FAR || (d->tokens && (d->tokens_stride < d->tokens || d->tokens_stride > FAR)))
+        return fail(GFR_EINVAL, "logprobs: stride %lld below vocab %d, or the tokens' %lld below %d", (long long)d->stride,
+                    d->vocab, (long long)d->tokens_stride, d->tokens);
+    if (d->workspace_bytes < need)
+        return fail(GFR_EINVAL, "logprobs: workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes, (long long)need);
+    const int64_t rows = d->rows;
+    const size_t token_bytes = d->wide_tokens ? 8 : 4;
+    if (!aligned(d->logits, type_bytes(d->type)) || !aligned(d->token, token_bytes) || !aligned(d->logprobs, 4) ||
+        !aligned(d->entropy, 4) || !aligned(d->top_ids, 4) || !aligned(d->top_logprobs, 4) || !aligned(d->workspace, 8))
+        return fail(GFR_EINVAL, "logprobs: tensors must be aligned to their elements");
+    // what is read after the first store: everything
+    const auto span_of = [](const void* p, int64_t bytes) { return RowBytes{reinterpret_cast<uintptr_t>(p), bytes, bytes, 1}; };
+    const RowBytes all[] = {rows_of(d->logits, d->type, rows, d->vocab, d->stride),
+                            {reinterpret_cast<uintptr_t>(d->token), (int64_t)(d->tokens * token_bytes),
+                             (int64_t)(d->tokens_stride * token_bytes), rows},
+                            span_of(d->logprobs, rows * d->tokens * 4), span_of(d->entropy, rows * 4),
+                            span_of(d->top_ids, rows * d->top * 4), span_of(d->top_logprobs, rows * d->top * 4),
+                            span_of(d->workspace, need)};
+    for (int i = 2; i < 7; ++i)
+        for (int j = 0; j < i; ++j)
+            if (all[i].at && all[j].at && all[i].bytes && all[j].bytes && overlap(all[i], all[j]))
+                return fail(GFR_EINVAL, "logprobs: an output or the workspace overlaps another tensor");
+    gfr::LogprobsJob job = {d->logits, d->token, d->logprobs, d->entropy, d->top_ids, d->top_logprobs, d->stride,
+                            d->tokens_stride, d->type, d->rows, d->vocab, d->tokens, d->top, d->wide_tokens != 0,
+                            1.f / d->temperature, 0, 0, nullptr, nullptr};
+    hipError_t e = gfr::launch_logprobs(stream, job, d->workspace);
+    if (e != hipSuccess) return hip_fail(e, "logprobs");
+    return 0;
+}
+
 // ---- debug rotation ---------------------------------------------------------------------------------------------
 int gfr_exl3_rotate(hipStream_t stream, const uint16_t* x, int x_stride, int x_f16, const int32_t* expert,
                     const uint16_t* suh, int k, int rows, uint16_t* out) {

@@ -194,6 +194,31 @@ struct NormJob {
 };
 hipError_t launch_norm(hipStream_t s, NormJob d);
 
+// logprobs.hip
+// logits [rows][stride], token [rows][tokens_stride] int32 or int64 -> logprob [rows][tokens], entropy [rows], top_ids and
+// top_logprobs [rows][top]. vocab <= LOGPROBS_VOCAB, top <= 32 and vocab.
+constexpr int LOGPROBS_VOCAB = 1 << 21;
+struct LogprobsJob {
+    const void* logits;
+    const void* token;
+    float* logprob;
+    float* entropy;
+    int* top_ids;
+    float* top_logprobs;
+    int64_t stride, tokens_stride;
+    int type, rows, vocab, tokens, top;
+    bool wide_tokens;
+    float by;                       // 1 / temperature
+    // set by launch_logprobs: chunks a row, logits a chunk, the chunks' sums and places in the workspace
+    int chunks;
+    int64_t span;
+    void* shares;
+    void* places;
+};
+size_t logprobs_workspace(int rows, int vocab, int top);
+int logprobs_chunks(int rows, int vocab);
+hipError_t launch_logprobs(hipStream_t s, LogprobsJob d, void* workspace);
+
 // shared_fp8.hip
 // The reference's FP8 shared expert (moe.rs:132-167) for rows [rows][x_stride] bf16: gate/up (8 K slices, bf16 gu
 // [rows][2 inter], limited SwiGLU -> act [rows][inter] bf16), then down -> out [rows][out_stride] fp32. hidden a

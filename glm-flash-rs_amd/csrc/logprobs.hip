@@ -1,0 +1,271 @@
+// Log probabilities of given tokens under rows of logits, the rows' entropies and their most likely tokens. With z = l / T,
+// m = max z and S = sum of exp(z - m):
+//   log p(t) = z_t - m - log S,   H = log S - (sum of (z - m) exp(z - m)) / S
+// Masked logits (-inf, NaN) have probability 0; several of +inf share it equally.
+//
+// A row is cut into chunks of a workgroup each, whose logits stay in registers as they were loaded: their maximum first, then
+// the sums against it, so that the row is read once and nothing is rescaled. S is held as C, the number of logits that equal
+// the maximum, and R, the sum over the others: where one token has nearly all of the probability, log S = log(1 + R) keeps
+// what 1 + R would round off. A second launch joins a row's chunks.
+// The most likely tokens of a chunk: with the lanes in G groups (G at least as many as are asked for) the least of the
+// groups' maxima is a threshold that G logits reach, and few more. These go to LDS, each counts those before it in the order
+// (larger logits first, the lower token first among equal ones), and that is its place. Where more reach it than LDS has
+// room for (rows of one value, rows in order), the places are filled one by one.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "lanes.hpp"
+#include "launch.hpp"
+#include "values.hpp"
+
+namespace gfr {
+namespace {
+
+constexpr int THREADS = 512, WAVES = THREADS / 64, ROOM = 1024;
+constexpr float LOG2E = 1.44269504088896341f;
+
+// A chunk's share of its row: the largest logit, how many equal it, the sums of the others' exponentials and of
+// (l - largest) times these (logits before they are divided by the temperature).
+struct Share {
+    float most, count, rest, slope;
+};
+
+// A place in the order: larger logits first, the lower token first among equal ones, as integers (0: an empty place).
+__device__ __forceinline__ uint64_t place_of(float logit, int token) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, logit + 0.f);     // (-0 is 0)
+    return (uint64_t)(b ^ (b >> 31 ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ int token_of(uint64_t place) { return (int)~(uint32_t)place; }
+__device__ __forceinline__ float logit_of(uint64_t place) {
+    const uint32_t b = (uint32_t)(place >> 32);
+    return __builtin_bit_cast(float, b ^ (b >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// Eight logits of a chunk from column c on, -inf from column end on.
+template <int TYPE>
+__device__ __forceinline__ Eight load_logits(const void* row, int64_t c, int64_t end) {
+    if (c + 8 <= end) return load_some(row, TYPE, c, 8);
+    constexpr uint32_t MASKED = TYPE == TYPE_BF16 ? 0xff80 : TYPE == TYPE_F16 ? 0xfc00 : 0xff800000;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        w[j] = MASKED;
+        if (c + j < end) w[j] = TYPE == TYPE_F32 ? static_cast<const uint32_t*>(row)[c + j] : static_cast<const uint16_t*>(row)[c + j];
+    }
+    Eight e;
+    if constexpr (TYPE == TYPE_F32) {
+        e.a = make_uint4(w[0], w[1], w[2], w[3]), e.b = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+        e.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        e.b = make_uint4(0, 0, 0, 0);
+    }
+    return e;
+}
+
+// V groups of eight logits a thread: group g of thread i starts at the chunk's column 8 (g THREADS + i).
+template <int TYPE, int V>
+__global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) {
+    __shared__ float maxima[32];
+    __shared__ float sums[WAVES][3];
+    __shared__ uint64_t places[ROOM];
+    __shared__ int found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x / d.chunks, chunk = blockIdx.x % d.chunks;
+    const int64_t c0 = (int64_t)chunk * d.span, end = c0 + d.span < d.vocab ? c0 + d.span : d.vocab;
+    const char* logits = static_cast<const char*>(d.logits) + (int64_t)row * d.stride * (TYPE == TYPE_F32 ? 4 : 2);
+    Eight raw[V];
+#pragma unroll
+    for (int g = 0; g < V; ++g) raw[g] = load_logits<TYPE>(logits, c0 + 8 * (g * THREADS + tid), end);
+    if (tid == 0) found = 0;
+    float most = -INFINITY;                                           // fmaxf leaves NaN out
+#pragma unroll
+    for (int g = 0; g < V; ++g) {
+        const f8_t l = values(raw[g], TYPE);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, l[j]);
+    }
+    // maxima of 16 neighbouring lanes, or of more where fewer places are asked for
+    const float near = max_over(d.top <= 8 ? 64 : d.top <= 16 ? 32 : 16, most);
+    if ((lane & 15) == 0) maxima[wave * 4 + lane / 16] = near;
+    __syncthreads();
+    const float one = maxima[lane & 31], M = max_over(32, one), least = -max_over(32, -one);
+
+    float rest = 0.f, slope = 0.f, count = 0.f;
+    const float k = LOG2E * d.by;
+#pragma unroll
+    for (int g = 0; g < V; ++g) {
+        const f8_t l = values(raw[g], TYPE);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = fmaxf(l[j] - M, -1e30f);                  // -1e30: masked, and exp2 of it is 0
+            const float e = __builtin_amdgcn_exp2f(x * k);
+            rest += e, slope = fmaf(x, e, slope);
+        }
+    }
+    if (most == M) {                                                  // few threads: again without the largest
+        rest = 0.f;
+#pragma unroll
+        for (int g = 0; g < V; ++g) {
+            const f8_t l = values(raw[g], TYPE);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float e = __builtin_amdgcn_exp2f(fmaxf(l[j] - M, -1e30f) * k);
+                if (l[j] == M) count += 1.f;
+                else rest += e;
+            }
+        }
+        if (M == -INFINITY) count = 0.f;
+    }
+    rest = sum_over(64, rest), slope = sum_over(64, slope), count = sum_over(64, count);
+    if (lane == 0) sums[wave][0] = rest, sums[wave][1] = slope, sums[wave][2] = count;
+    if (d.top && most >= least) {
+#pragma unroll
+        for (int g = 0; g < V; ++g) {
+            const f8_t l = values(raw[g], TYPE);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (l[j] >= least && l[j] > -INFINITY) {
+                    const int at = atomicAdd(&found, 1);
+                    if (at < ROOM) places[at] = place_of(l[j], (int)(c0 + 8 * (g * THREADS + tid) + j));
+                }
+        }
+    }
+    __syncthreads();
+    const int64_t part = (int64_t)row * d.chunks + chunk;
+    if (tid == 0) {
+        Share s = {M, 0.f, 0.f, 0.f};
+        for (int w = 0; w < WAVES; ++w) s.rest += sums[w][0], s.slope += sums[w][1], s.count += sums[w][2];
+        static_cast<Share*>(d.shares)[part] = s;
+    }
+    if (!d.top) return;
+    uint64_t* out = static_cast<uint64_t*>(d.places) + part * d.top;
+    const int n = found;
+    if (n <= ROOM) {
+        if (tid >= n && tid < d.top) out[tid] = 0;
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t p = places[i];
+            int place = 0;
+            for (int o = 0; o < n; ++o) place += places[o] > p;
+            if (place < d.top) out[place] = p;
+        }
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int i = 0; i < d.top; ++i) {                                 // (more than ROOM: none of them stays empty)
+        uint64_t best = 0;
+#pragma unroll
+        for (int g = 0; g < V; ++g) {
+            const f8_t l = values(raw[g], TYPE);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint64_t p = place_of(l[j], (int)(c0 + 8 * (g * THREADS + tid) + j));
+                if (l[j] > -INFINITY && p < last && p > best) best = p;
+            }
+        }
+        best = max_over(64, best);
+        __syncthreads();
+        if (lane == 0) places[wave] = best;
+        __syncthreads();
+        last = places[0];
+        for (int w = 1; w < WAVES; ++w) last = larger(last, places[w]);
+        if (tid == 0) out[i] = last;
+    }
+}
+
+// A wave a row: the chunks' shares against the row's largest logit, the tokens, the places.
+__global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsJob d) {
+    const int lane = threadIdx.x, row = blockIdx.x;
+    const Share* shares = static_cast<const Share*>(d.shares) + (int64_t)row * d.chunks;
+    Share s = {-INFINITY, 0.f, 0.f, 0.f};
+    if (lane < d.chunks) s = shares[lane];
+    const float M = max_over(64, s.most);
+    float count = s.count, rest = s.rest, slope = s.slope;
+    if (s.most < M) {
+        const float x = fmaxf(s.most - M, -1e30f), e = __builtin_amdgcn_exp2f(x * (LOG2E * d.by)), all = s.count + s.rest;
+        count = 0.f, rest = all * e, slope = e * fmaf(x, all, s.slope);
+    }
+#pragma unroll
+    for (int m = 32; m; m >>= 1) count += __shfl_xor(count, m), rest += __shfl_xor(rest, m), slope += __shfl_xor(slope, m);
+    const float log_sum = logf(count) + log1pf(rest / count);
+    const auto log_p = [&](float l) {
+        if (!(l > -INFINITY)) return -INFINITY;
+        return (l == M ? 0.f : (l - M) * d.by) - log_sum;
+    };
+    if (lane == 0) d.entropy[row] = count > 0.f ? log_sum - slope * d.by / (count + rest) : 0.f;
+    const int64_t base = (int64_t)row * d.stride;
+    for (int i = lane; i < d.tokens; i += 64) {
+        const int64_t at = (int64_t)row * d.tokens_stride + i;
+        const int64_t token = d.wide_tokens ? static_cast<const int64_t*>(d.token)[at] : static_cast<const int32_t*>(d.token)[at];
+        const bool there = token >= 0 && token < d.vocab;             // a token that is not in the vocabulary: probability 0
+        d.logprob[(int64_t)row * d.tokens + i] = there ? log_p(load_one(d.logits, d.type, base + token)) : -INFINITY;
+    }
+    if (!d.top) return;
+    // a chunk's places are in order, so that the next one is the largest of the chunks' heads
+    extern __shared__ uint64_t places[];
+    const uint64_t* from = static_cast<const uint64_t*>(d.places) + (int64_t)row * d.chunks * d.top;
+    for (int i = lane; i < d.chunks * d.top; i += 64) places[i] = from[i];
+    __syncthreads();
+    int* ids = d.top_ids + (int64_t)row * d.top;
+    float* logps = d.top_logprobs + (int64_t)row * d.top;
+    int next = lane * d.top + 1;
+    uint64_t head = lane < d.chunks ? places[lane * d.top] : 0;
+    int i = 0;
+    for (; i < d.top; ++i) {
+        const uint64_t best = max_over(64, head);
+        if (!best) break;
+        if (lane == 0) ids[i] = token_of(best), logps[i] = log_p(logit_of(best));
+        if (head == best) head = next < (lane + 1) * d.top ? places[next++] : 0;
+    }
+    // fewer logits than places are not masked: the masked tokens in order, enough of which are among the first 64
+    if (i < d.top) {
+        const bool masked = lane < d.vocab && !(load_one(d.logits, d.type, base + lane) > -INFINITY);
+        const int place = i + __popcll(__ballot(masked) & ((1ull << lane) - 1));
+        if (masked && place < d.top) ids[place] = lane, logps[place] = -INFINITY;
+    }
+}
+
+template <int TYPE, int V>
+hipError_t launch(hipStream_t s, const LogprobsJob& d) {
+    logprobs_chunk_kernel<TYPE, V><<<dim3((unsigned)(d.rows * (int64_t)d.chunks)), THREADS, 0, s>>>(d);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    logprobs_join_kernel<<<dim3((unsigned)d.rows), 64, (size_t)d.chunks * d.top * sizeof(uint64_t), s>>>(d);
+    return hipGetLastError();
+}
+template <int TYPE>
+hipError_t launch(hipStream_t s, const LogprobsJob& d, int groups) {
+    switch (groups) {
+        case 1: return launch<TYPE, 1>(s, d);
+        case 2: return launch<TYPE, 2>(s, d);
+        case 4: return launch<TYPE, 4>(s, d);
+        default: return launch<TYPE, 8>(s, d);
+    }
+}
+
+// Groups of eight logits a thread: as many as leave two workgroups a CU, and so many that a row has at most 64 chunks, one
+// a lane of the join.
+int chunks_of(int vocab, int groups) { return (int)(((int64_t)vocab + 8 * THREADS * groups - 1) / (8 * THREADS * groups)); }
+int groups_of(int rows, int vocab) {
+    int v = 8;
+    while (v > 1 && (int64_t)rows * chunks_of(vocab, v) < 512 && chunks_of(vocab, v / 2) <= 64) v /= 2;
+    return v;
+}
+
+}  // namespace
+
+int logprobs_chunks(int rows, int vocab) { return chunks_of(vocab, groups_of(rows, vocab)); }
+size_t logprobs_workspace(int rows, int vocab, int top) {
+    return (size_t)rows * logprobs_chunks(rows, vocab) * (sizeof(Share) + top * sizeof(uint64_t));
+}
+
+hipError_t launch_logprobs(hipStream_t s, LogprobsJob d, void* workspace) {
+    const int groups = groups_of(d.rows, d.vocab);
+    d.chunks = chunks_of(d.vocab, groups);
+    d.span = ((d.vocab + d.chunks - 1) / d.chunks + 7) / 8 * 8;
+    d.shares = workspace;
+    d.places = static_cast<char*>(workspace) + (size_t)d.rows * d.chunks * sizeof(Share);
+    if (d.type == TYPE_BF16) return launch<TYPE_BF16>(s, d, groups);
+    return d.type == TYPE_F16 ? launch<TYPE_F16>(s, d, groups) : launch<TYPE_F32>(s, d, groups);
+}
+
+}  // namespace gfr

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "lanes.hpp"
 #include "launch.hpp"
 #include "values.hpp"
 
@@ -16,8 +17,7 @@ namespace {
 // wave may still be reading from the sum before (two in turn are enough: each sum has a barrier).
 template <int L>
 __device__ __forceinline__ float total(float v, float* part) {
-#pragma unroll
-    for (int m = (L ? L : 64) / 2; m; m >>= 1) v += __shfl_xor(v, m);
+    v = sum_over(L ? L : 64, v);
     if constexpr (L == 0) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();

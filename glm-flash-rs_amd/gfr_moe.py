@@ -11,6 +11,7 @@ import ctypes
 import os
 import struct
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -110,6 +111,8 @@ def _load() -> ctypes.CDLL:
         "gfr_dense_run": ([P, P], I),
         "gfr_dense_form": ([P], I),
         "gfr_block_norm_run": ([P, P], I),
+        "gfr_logprobs_workspace": ([I, I, I], ctypes.c_int64),
+        "gfr_logprobs_run": ([P, P], I),
         "gfr_moe_reserve_bf16": ([VP], I),
         "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
@@ -406,10 +409,11 @@ class Norm:
 
 
 _NO_NORM = (0, 0, 0, 0.0, 0.0, 0, 0)
-# gfr_gate, gfr_dense and gfr_block_norm as bytes in the machine's layout: packed anew for every call, which a ctypes
+# gfr_gate, gfr_dense, gfr_block_norm and gfr_logprobs as bytes in the machine's layout: packed anew for every call, which a ctypes
 # structure of as many fields takes about three times as long for
 _GATE = struct.Struct("@5ifP")
 _DENSE = struct.Struct("@4iPqPq2ifiP2iPqPq")
+_LOGPROBS = struct.Struct("@6ifPqPq5Pq")
 _BLOCK_NORM = struct.Struct("@9i2fPqPqPqPqPq3i2f2P3i2f2P")
 
 
@@ -1125,6 +1129,55 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor = None, pre: Norm = None,
 def norm(x: torch.Tensor, norm: Norm, out: torch.Tensor = None, out_dtype: torch.dtype = None, stream=None):
     """The norm alone: rows [rows, n] (a token's, or its heads') to out (x's type by default; may be x itself)."""
     return _block_norm(x, None, norm, None, None, None, 1.0, 1.0, False, None, out, out_dtype, stream)[1]
+
+
+class LogProbs(NamedTuple):
+    """token_logprobs' results; top_ids and top_logprobs None for top = 0."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperature: float = 1.0,
+                   stream=None) -> LogProbs:
+    """gfr_logprobs_run: of the rows' distributions softmax(logits / temperature), logits [rows, vocab] (bf16, fp16 or fp32),
+    the log probabilities [rows, tokens] or [rows] of tokens of that shape (int32 or int64; -inf for one outside the
+    vocabulary), the entropies [rows], and the `top` (0 .. 32) most likely tokens [rows, top] int32 with their log
+    probabilities, equal logits by lower token. Masked logits (-inf, NaN) have probability 0. fp32 results, the workspace
+    from torch's allocator on the call's stream. No gradient is recorded. A stream other than the current one is the caller's
+    to order after the inputs' writes; they have to stay alive until it is done."""
+    rows, vocab = logits.shape
+    kind = _TYPE.get(logits.dtype)
+    if kind is None:
+        raise ValueError(f"logits {logits.dtype}: fp32, bf16 or fp16")
+    shape = tokens.shape
+    if len(shape) not in (1, 2) or shape[0] != rows or tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"tokens {tuple(shape)} {tokens.dtype}: want ({rows},) or ({rows}, any) int32 or int64")
+    here = _get_device()
+    if logits.get_device() != here or tokens.get_device() != here:
+        _elsewhere(logits, tokens)
+    each = tokens if len(shape) == 2 else tokens.unsqueeze(1)
+    L = _lib or lib()
+    need = L.gfr_logprobs_workspace(rows, vocab, top)
+    if need < 0:
+        _check(need)
+    workspace = _empty((need,), torch.uint8, logits, stream)
+    logprobs = _empty(shape, torch.float32, logits, stream)
+    entropy = _empty((rows,), torch.float32, logits, stream)
+    top_ids = top_logprobs = None
+    if top:
+        top_ids = _empty((rows, top), torch.int32, logits, stream)
+        top_logprobs = _empty((rows, top), torch.float32, logits, stream)
+    handle = _handle(stream, here)
+    rc = L.gfr_logprobs_run(
+        handle, _LOGPROBS.pack(rows, vocab, each.shape[1], top, kind, int(tokens.dtype is torch.int64), temperature,
+                               logits.data_ptr(), _row_stride(logits), each.data_ptr(), _row_stride(each),
+                               logprobs.data_ptr(), entropy.data_ptr(), _ptr(top_ids), _ptr(top_logprobs),
+                               workspace.data_ptr(), need))
+    if rc:
+        _check(rc)
+    return LogProbs(logprobs, entropy, top_ids, top_logprobs)
 
 
 def rotate(x: torch.Tensor, expert: torch.Tensor, suh: torch.Tensor, stream=None) -> torch.Tensor:

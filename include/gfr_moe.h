@@ -386,6 +386,40 @@ typedef struct gfr_block_norm {
 } gfr_block_norm;
 int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d);
 
+/* ---- Log probabilities of tokens --------------------------------------------------------------------------------
+ * Of each row's distribution p = softmax(logits / temperature) over the vocabulary:
+ *   logprobs [rows][tokens]    log p of the given tokens (token [rows][tokens_stride], int32 or, wide_tokens 1, int64); a
+ *                              token outside [0, vocab) has -inf, as one of probability 0
+ *   entropy [rows]             - sum of p log p
+ *   top_ids, top_logprobs [rows][top]   the most likely tokens in order (equal logits: the lower token) and their log p
+ * all fp32 but the ids. Masked logits (-inf, NaN) have probability 0 and log p -inf; they are among the top only where the
+ * row has fewer others, by lower token. Several logits of +inf share the probability. A row of masked logits only: -inf,
+ * entropy 0. logits in GFR_BF16, GFR_F16 or GFR_F32, rows of any stride and element-aligned address; sums in fp32, log p
+ * within a few units of 32 bits also where it is near 0. A row's results depend on no other row; its last bits may on the
+ * number of rows, which the order of its sums follows (the tokens' order does not). tokens or top may be 0; top <= 32 and
+ * vocab, vocab <= 2^21, temperature 1e-6 .. 1e6, at least one row.
+ * workspace: gfr_logprobs_workspace(rows, vocab, top) bytes of device memory (at most 2^31), 8-byte aligned, that are the
+ * call's until its work is done: two calls that may overlap, or two captured graphs that may, take two workspaces. Outputs
+ * and the workspace must not share memory with anything else. */
+typedef struct gfr_logprobs {
+    int rows, vocab, tokens, top;
+    int type;
+    int wide_tokens;
+    float temperature;
+    const void* logits;
+    int64_t stride;
+    const void* token;
+    int64_t tokens_stride;
+    float* logprobs;
+    float* entropy;
+    int32_t* top_ids;
+    float* top_logprobs;
+    void* workspace;
+    int64_t workspace_bytes;
+} gfr_logprobs;
+int64_t gfr_logprobs_workspace(int rows, int vocab, int top);   /* negative: GFR_EINVAL */
+int gfr_logprobs_run(hipStream_t stream, const gfr_logprobs* d);
+
 /* ---- Single EXL3 linear (benchmark config 1; the decode path's GEMV with rot_in / down-epilogue formulas) ----
  * y [n] fp32 = svh * had(W^T xh) / sqrt(128), xh = fp16(had(x * suh) / sqrt(128)), x [kin] fp16. */
 typedef struct gfr_linear gfr_linear;
