@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 SOURCES = ["grouping.hip", "exl3_decode.hip", "exl3_prefill.hip", "router.hip", "gfr_moe_api.hip", "prepared.hip", "prefetch.hip",
            "shared_fp8.hip", "gate.hip", "dense.hip", "norm.hip",
-           "logprobs.hip"]
+           "logprobs.hip", "experts16.hip"]
 LIB = os.path.join(PKG, "libgfr_moe.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -1,0 +1,376 @@
+// 16-bit routed experts for a few tokens: with e = picks[r][s] the expert of pair (r, s),
+//   g, u   = the halves of gu[e] x[r];  a = act(min(g, limit)) * clamp(u, -limit, limit)
+//   out[r] = residual[r] + sum over s of weights[r][s] * down[e] a       (slots in order; picks outside [0, experts): none)
+// x, gu and down in bf16 or fp16; sums, activations and weights in fp32, one rounding at the end. Between the two products
+// the activations are held as the sum of two 16-bit values, 16 bits of them or more, which costs the matrix core a second
+// pass over the same weights in registers.
+//
+// Bound: the weights of the experts that are picked, read once. A workgroup takes one expert's share of the columns and all
+// the rows that picked it, in passes of up to 16 RB, so that an expert's weights are read once however many rows pick it
+// (again, from the caches, for more than one pass). Weights are the matrix core's A operand (v_mfma_f32_16x16x32: D holds,
+// in lane l, columns 4 (l / 16) .. + 3 of the tile for row l % 16) and go through LDS stages of a wave's own as whole lines;
+// rows are the B operand, loaded as fragments, which the caches hold. A row's sums are taken in an order of the
+// sizes alone, so that they depend neither on the other rows nor on their number.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "launch.hpp"
+#include "mfma16.hpp"
+#include "values.hpp"
+
+namespace gfr {
+namespace {
+
+constexpr int PASS = 64;                                             // a pass's members at most
+
+// The members of an expert: the pairs (by number) whose pick it is, in order; first and their count over all, and those from
+// number `from` on, up to `room` of them, in LDS. Called by the whole workgroup (waves of it, at most 16).
+struct Members {
+    int pair[PASS];
+    int waves[16];
+};
+__device__ __forceinline__ int find_members(const Experts16Job& d, int expert, int from, int room, Members& m, int& first) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, pairs = d.rows * d.slots;
+    int seen = 0;
+    first = pairs;
+    for (int base = 0; base < pairs; base += blockDim.x) {
+        const int p = base + (int)threadIdx.x;
+        const bool mine = p < pairs && d.picks[p] == expert;
+        const uint64_t ballot = __ballot(mine);
+        __syncthreads();
+        if (lane == 0) m.waves[wave] = __popcll(ballot);
+        __syncthreads();
+        int before = seen + __popcll(ballot & ((1ull << lane) - 1));
+        for (int w = 0; w < waves; ++w) {
+            if (w < wave) before += m.waves[w];
+            seen += m.waves[w];
+        }
+        if (mine && before >= from && before < from + room) m.pair[before - from] = p;
+    }
+    __syncthreads();
+    if (seen && from == 0) first = m.pair[0];
+    return seen;
+}
+
+// This workgroup's expert: the experts in turn, or, where there are fewer pairs, the pairs' picks, each taken by the first
+// pair that has it. Negative: nothing to do. count: its members; the first `room` are in LDS.
+__device__ __forceinline__ int expert_of(const Experts16Job& d, int u, int room, Members& m, int& count) {
+    const bool by_pair = d.rows * d.slots < d.experts;
+    const int e = by_pair ? d.picks[u] : u;
+    if (e < 0 || e >= d.experts) return -1;
+    int first;
+    count = find_members(d, e, 0, room, m, first);
+    return count && (!by_pair || first == u) ? e : -1;
+}
+
+// A wave's stage of EB tiles of 16 weight rows by 64 k: rows of 128 bytes, 16-byte chunk c at position c ^ (row % 8), so
+// that the fragments' reads of neighbouring rows meet all banks.
+template <int TYPE, int EB>
+struct Weights {
+    const uint16_t* at[2 * EB];                                       // this lane's 16 bytes of every 8 rows
+    struct Chunk {
+        uint4 w[2 * EB];
+    };
+    __device__ __forceinline__ void load(Chunk& f, int k, int K) const {
+        const int lane = threadIdx.x & 63;
+        if (k + 64 <= K) {
+#pragma unroll
+            for (int i = 0; i < 2 * EB; ++i) __builtin_memcpy(&f.w[i], at[i] + k, 16);
+        } else {
+            const int left = K - k - (lane & 7) * 8;                  // from this lane's first on; nothing past the end
+#pragma unroll
+            for (int i = 0; i < 2 * EB; ++i) f.w[i] = load_chunk(at[i] + k, 0, left);
+        }
+    }
+    __device__ __forceinline__ void stage(const Chunk& f, char* stage) const {
+        const int lane = threadIdx.x & 63;
+        char* to = stage + (lane >> 3) * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 2 * EB; ++i) *reinterpret_cast<uint4*>(to + i * 1024) = f.w[i];
+        __builtin_amdgcn_wave_barrier();
+    }
+    // tile i's fragment of half s of the chunk: row l % 16, k 32 s + 8 (l / 16) ..
+    __device__ __forceinline__ uint4 fragment(const char* stage, int i, int s) const {
+        const int lane = threadIdx.x & 63, a = lane & 15, q = lane >> 4;
+        return *reinterpret_cast<const uint4*>(stage + i * 2048 + a * 128 + ((4 * s + q) ^ (a & 7)) * 16);
+    }
+};
+
+// ---- gate and up --------------------------------------------------------------------------------------------------
+constexpr int UP_WAVES = 8, UP_TILES = 2, UP_COLS = 8 * UP_TILES;
+
+// One pass: members [from, from + 16 RB) of the expert, columns c0 .. + UP_COLS. A tile of 16 weight rows is 8 gate rows
+// and the 8 up rows of the same columns; the waves share k by chunks of 64, and their sums are added in order.
+template <int TYPE, int RB>
+__device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYPE, UP_TILES>& w, const Members& m, int members,
+                                        int c0, char* lds) {
+    constexpr int EB = UP_TILES, U = 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = lane & 15, q = lane >> 4;
+    const uint16_t* xp[RB];
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+        const int pair = m.pair[min(16 * j + a, members - 1)];
+        xp[j] = d.x + (int64_t)(pair / d.slots) * d.x_stride + 8 * q;
+    }
+    struct Chunk {
+        typename Weights<TYPE, EB>::Chunk w;
+        uint4 x[RB][2];
+    };
+    f4_t acc[EB][RB];
+#pragma unroll
+    for (int i = 0; i < EB; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
+    const int chunks = (d.hidden + 63) / 64;
+    auto load = [&](Chunk& f, int c) {
+        w.load(f.w, c * 64, d.hidden);
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) f.x[j][s] = load_chunk(xp[j] + c * 64 + 32 * s, 0, d.hidden - c * 64 - 32 * s - 8 * q);
+    };
+    char* stage = lds + wave * EB * 2048;
+    auto multiply = [&](const Chunk& f) {
+        w.stage(f.w, stage);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < EB; ++i) {
+                const uint4 fw = w.fragment(stage, i, s);
+#pragma unroll
+                for (int j = 0; j < RB; ++j) acc[i][j] = mfma<TYPE>(fw, f.x[j][s], acc[i][j]);
+            }
+    };
+    Chunk f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (wave + u * UP_WAVES < chunks) load(f[u], wave + u * UP_WAVES);
+    for (int c = wave; c < chunks; c += U * UP_WAVES) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c + u * UP_WAVES < chunks) multiply(f[u]);
+            if (c + (u + U) * UP_WAVES < chunks) load(f[u], c + (u + U) * UP_WAVES);
+        }
+    }
+    __syncthreads();
+    f4_t* part = reinterpret_cast<f4_t*>(lds);                        // [UP_WAVES][EB * RB][64]
+#pragma unroll
+    for (int i = 0; i < EB; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) part[(wave * EB * RB + i * RB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    // a thread finishes four columns of a member: lanes 16 Q + member hold gate columns 4 Q .., lanes 32 on their up values
+    for (int t = threadIdx.x; t < EB * RB * 32; t += 64 * UP_WAVES) {
+        const int row = t & 15, Q = (t >> 4) & 1, tile = t >> 5, i = tile / RB, j = tile % RB;
+        if (16 * j + row >= members) continue;
+        f8_t v = {0, 0, 0, 0, 0, 0, 0, 0}, up = v;
+        for (int s = 0; s < UP_WAVES; ++s) {
+            const f4_t* p = part + (s * EB * RB + tile) * 64 + 16 * Q + row;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += p[0][e], up[e] += p[32][e];
+        }
+        v = shape<true>(v, up, d.act, d.limit);
+        const int col = c0 + 8 * i + 4 * Q;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = col + e < d.inter ? v[e] : 0.f;           // (columns up to a multiple of 64 are read)
+            hi[e] = f_to_16(x, TYPE);
+            // (up to twice fp16's range the second value holds what is above the first's)
+            if (TYPE == TYPE_F16 && fabsf(x) > 65504.f && fabsf(x) <= 131008.f) hi[e] = x > 0.f ? 0x7bff : 0xfbff;
+            const float h = TYPE == TYPE_BF16 ? bf16_to_f(hi[e]) : f16_to_f(hi[e]);
+            lo[e] = fabsf(h) < INFINITY ? f_to_16(x - h, TYPE) : 0;
+        }
+        uint16_t* to = d.acts + (int64_t)m.pair[16 * j + row] * 2 * d.inter_pad + col;
+        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
+        *reinterpret_cast<uint2*>(to + d.inter_pad) = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+    }
+    __syncthreads();
+}
+
+template <int TYPE, int RB>
+__global__ void __launch_bounds__(64 * UP_WAVES) experts16_up_kernel(Experts16Job d) {
+    __shared__ __align__(1024) char lds[UP_WAVES * UP_TILES * (RB > 2 ? RB * 1024 : 2048)];
+    __shared__ Members m;
+    const int lane = threadIdx.x & 63, tiles = d.inter_pad / UP_COLS;
+    const int u = blockIdx.x / tiles, c0 = (blockIdx.x % tiles) * UP_COLS;
+    int count;
+    const int e = expert_of(d, u, 16 * RB, m, count);
+    if (e < 0) return;
+    Weights<TYPE, UP_TILES> w;
+#pragma unroll
+    for (int i = 0; i < 2 * UP_TILES; ++i) {
+        const int row = min(c0 + (i >> 1) * 8 + (lane >> 3), d.inter - 1) + (i & 1) * d.inter;
+        w.at[i] = d.gu + (int64_t)e * d.gu_expert + (int64_t)row * d.gu_stride + (lane & 7) * 8;
+    }
+    for (int from = 0;;) {
+        const int members = min(count - from, 16 * RB);
+        if constexpr (RB == 1) {
+            up_pass<TYPE, 1>(d, w, m, members, c0, lds);
+        } else {
+            if (members <= 16) up_pass<TYPE, 1>(d, w, m, members, c0, lds);
+            else if (members <= 32) up_pass<TYPE, 2>(d, w, m, members, c0, lds);
+            else up_pass<TYPE, 4>(d, w, m, members, c0, lds);
+        }
+        if ((from += 16 * RB) >= count) break;
+        int first;
+        find_members(d, e, from, 16 * RB, m, first);
+    }
+}
+
+// ---- down ---------------------------------------------------------------------------------------------------------
+constexpr int DOWN_WAVES = 4, DOWN_TILES = 2, DOWN_COLS = 16 * DOWN_TILES * DOWN_WAVES;
+
+// One pass: a wave's 16 DOWN_TILES columns from c0 on, for members [from, from + 16 RB), over the whole of k.
+template <int TYPE, int RB>
+__device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<TYPE, DOWN_TILES>& w, const Members& m,
+                                          int members, int c0, char* stage) {
+    constexpr int EB = DOWN_TILES, U = 2;
+    const int lane = threadIdx.x & 63, a = lane & 15, q = lane >> 4;
+    const uint16_t* xp[RB];
+#pragma unroll
+    for (int j = 0; j < RB; ++j)
+        xp[j] = d.acts + (int64_t)m.pair[min(16 * j + a, members - 1)] * 2 * d.inter_pad + 8 * q;
+    struct Chunk {
+        typename Weights<TYPE, EB>::Chunk w;
+        uint4 x[RB][2][2];
+    };
+    f4_t acc[EB][RB];
+#pragma unroll
+    for (int i = 0; i < EB; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
+    const int chunks = d.inter_pad / 64;
+    auto load = [&](Chunk& f, int c) {
+        w.load(f.w, c * 64, d.inter);
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                f.x[j][s][0] = *reinterpret_cast<const uint4*>(xp[j] + c * 64 + 32 * s);
+                f.x[j][s][1] = *reinterpret_cast<const uint4*>(xp[j] + d.inter_pad + c * 64 + 32 * s);
+            }
+    };
+    auto multiply = [&](const Chunk& f) {
+        w.stage(f.w, stage);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < EB; ++i) {
+                const uint4 fw = w.fragment(stage, i, s);
+#pragma unroll
+                for (int j = 0; j < RB; ++j) {
+                    acc[i][j] = mfma<TYPE>(fw, f.x[j][s][0], acc[i][j]);
+                    acc[i][j] = mfma<TYPE>(fw, f.x[j][s][1], acc[i][j]);
+                }
+            }
+    };
+    Chunk f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (u < chunks) load(f[u], u);
+    for (int c = 0; c < chunks; c += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c + u < chunks) multiply(f[u]);
+            if (c + u + U < chunks) load(f[u], c + u + U);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+        if (16 * j + a >= members) continue;
+        float* y = d.y + (int64_t)m.pair[16 * j + a] * d.hidden_pad;
+#pragma unroll
+        for (int i = 0; i < EB; ++i) {
+            const int col = c0 + 16 * i + 4 * q;
+            if (col < d.hidden) *reinterpret_cast<f4_t*>(y + col) = acc[i][j];
+        }
+    }
+}
+
+template <int TYPE, int RB>
+__global__ void __launch_bounds__(64 * DOWN_WAVES) experts16_down_kernel(Experts16Job d) {
+    __shared__ __align__(1024) char lds[DOWN_WAVES * DOWN_TILES * 2048];
+    __shared__ Members m;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tiles = (d.hidden + DOWN_COLS - 1) / DOWN_COLS;
+    const int u = blockIdx.x / tiles, c0 = (blockIdx.x % tiles) * DOWN_COLS + wave * 16 * DOWN_TILES;
+    int count;
+    const int e = expert_of(d, u, 16 * RB, m, count);
+    if (e < 0) return;
+    Weights<TYPE, DOWN_TILES> w;
+#pragma unroll
+    for (int i = 0; i < 2 * DOWN_TILES; ++i)
+        w.at[i] = d.down + (int64_t)e * d.down_expert + (int64_t)min(c0 + i * 8 + (lane >> 3), d.hidden - 1) * d.down_stride +
+                  (lane & 7) * 8;
+    char* stage = lds + wave * DOWN_TILES * 2048;
+    for (int from = 0;;) {
+        const int members = min(count - from, 16 * RB);
+        if constexpr (RB == 1) {
+            down_pass<TYPE, 1>(d, w, m, members, c0, stage);
+        } else {
+            if (members <= 16) down_pass<TYPE, 1>(d, w, m, members, c0, stage);
+            else if (members <= 32) down_pass<TYPE, 2>(d, w, m, members, c0, stage);
+            else down_pass<TYPE, 4>(d, w, m, members, c0, stage);
+        }
+        if ((from += 16 * RB) >= count) break;
+        int first;
+        find_members(d, e, from, 16 * RB, m, first);
+    }
+}
+
+// ---- the rows' sums -----------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) experts16_combine_kernel(Experts16Job d) {
+    const int quads = d.hidden_pad / 4;
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= (int64_t)d.rows * quads) return;
+    const int row = (int)(t / quads), col = (int)(t % quads) * 4, count = min(4, d.hidden - col);
+    f4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < d.slots; ++s) {
+        const int pair = row * d.slots + s, e = d.picks[pair];
+        if (e < 0 || e >= d.experts) continue;
+        const f4_t y = *reinterpret_cast<const f4_t*>(d.y + (int64_t)pair * d.hidden_pad + col);
+        const float weight = d.weights[pair];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(weight, y[j], v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < count) {
+            if (d.residual) v[j] += load_one(d.residual, d.residual_type, (int64_t)row * d.residual_stride + col + j);
+            store_one(d.out, d.out_type, (int64_t)row * d.out_stride + col + j, v[j]);
+        }
+}
+
+template <int TYPE, int RB>
+hipError_t launch(hipStream_t s, const Experts16Job& d) {
+    const int64_t leaders = (int64_t)d.rows * d.slots < d.experts ? (int64_t)d.rows * d.slots : d.experts;
+    experts16_up_kernel<TYPE, RB><<<dim3((unsigned)(leaders * (d.inter_pad / UP_COLS))), 64 * UP_WAVES, 0, s>>>(d);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    experts16_down_kernel<TYPE, RB>
+        <<<dim3((unsigned)(leaders * ((d.hidden + DOWN_COLS - 1) / DOWN_COLS))), 64 * DOWN_WAVES, 0, s>>>(d);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    const int64_t threads = (int64_t)d.rows * (d.hidden_pad / 4);
+    experts16_combine_kernel<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, s>>>(d);
+    return hipGetLastError();
+}
+
+int padded(int n, int to) { return (n + to - 1) / to * to; }
+
+}  // namespace
+
+size_t experts16_workspace(int rows, int slots, int hidden, int inter) {
+    return (size_t)rows * slots * (4 * (size_t)padded(inter, 64) + 4 * (size_t)padded(hidden, 4));
+}
+
+hipError_t launch_experts16(hipStream_t s, Experts16Job d, void* workspace) {
+    d.inter_pad = padded(d.inter, 64), d.hidden_pad = padded(d.hidden, 4);
+    d.acts = static_cast<uint16_t*>(workspace);
+    d.y = reinterpret_cast<float*>(d.acts + (size_t)d.rows * d.slots * 2 * d.inter_pad);
+    const bool few = d.rows <= 16;                                    // (rows pick an expert once: one pass of 16)
+    if (d.type == TYPE_BF16) return few ? launch<TYPE_BF16, 1>(s, d) : launch<TYPE_BF16, 4>(s, d);
+    return few ? launch<TYPE_F16, 1>(s, d) : launch<TYPE_F16, 4>(s, d);
+}
+
+}  // namespace gfr

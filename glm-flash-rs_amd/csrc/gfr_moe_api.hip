@@ -514,6 +514,79 @@ int gfr_dense_form(const gfr_dense* d) {
     return rc ? rc : gfr::dense_form(job);
 }
 
+// ---- 16-bit routed experts ----------------------------------------------------------------------------------------
+int64_t gfr_experts16_workspace(int rows, int slots, int hidden, int inter) {
+    if (rows <= 0 || slots <= 0 || (int64_t)rows * slots > 65536)
+        return fail(GFR_EINVAL, "experts16: rows %d, slots %d: at least 1, and 65536 pairs at most", rows, slots);
+    if (hidden <= 0 || inter <= 0 || hidden > 1 << 20 || inter > 1 << 20)
+        return fail(GFR_EINVAL, "experts16: hidden %d, inter %d outside 1..%d", hidden, inter, 1 << 20);
+    return (int64_t)gfr::experts16_workspace(rows, slots, hidden, inter);
+}
+
+int gfr_experts16_run(hipStream_t stream, const gfr_experts16* d) {
+    if (!d) return fail(GFR_EINVAL, "experts16: null argument");
+    const int64_t need = gfr_experts16_workspace(d->rows, d->slots, d->hidden, d->inter);
+    if (need < 0) return GFR_EINVAL;
+    if (d->experts <= 0 || d->experts > 65536) return fail(GFR_EINVAL, "experts16: experts %d outside 1..65536", d->experts);
+    if (!d->x || !d->gu || !d->down || !d->picks || !d->weights || !d->out || !d->workspace)
+        return fail(GFR_EINVAL, "experts16: null argument");
+    if (d->type != GFR_BF16 && d->type != GFR_F16) return fail(GFR_EINVAL, "experts16: type %d is not bf16 or fp16", d->type);
+    const auto suits = [&](int t) { return t == d->type || t == GFR_F32; };
+    if (!suits(d->out_type) || (d->residual && !suits(d->residual_type)))
+        return fail(GFR_EINVAL, "experts16: out %d and residual %d must have x's type or fp32", d->out_type, d->residual_type);
+    if (d->act < GFR_ACT_NONE || d->act > GFR_ACT_SILU) return fail(GFR_EINVAL, "experts16: activation %d", d->act);
+    if (!(d->limit >= 0.f)) return fail(GFR_EINVAL, "experts16: limit %g must not be negative", (double)d->limit);
+    const int64_t rows = d->rows, H = d->hidden, I = d->inter, E = d->experts;
+    if (d->x_stride < H || d->gu_stride < H || d->down_stride < I || d->out_stride < H || (d->residual && d->residual_stride < H))
+        return fail(GFR_EINVAL, "experts16: a stride of x %lld, gu %lld, down %lld, residual %lld or out %lld below its columns",
+                    (long long)d->x_stride, (long long)d->gu_stride, (long long)d->down_stride,
+                    (long long)d->residual_stride, (long long)d->out_stride);
+    if (d->x_stride > FAR || d->gu_stride > FAR || d->down_stride > FAR || d->out_stride > FAR ||
+        (d->residual && d->residual_stride > FAR))
+        return fail(GFR_EINVAL, "experts16: a stride above 2^31");
+    const int64_t widest = (int64_t)1 << 40;
+    if (d->gu_expert < 0 || d->down_expert < 0 || d->gu_expert > widest || d->down_expert > widest)
+        return fail(GFR_EINVAL, "experts16: %lld and %lld elements between experts: outside 0..2^40", (long long)d->gu_expert,
+                    (long long)d->down_expert);
+    if (!aligned(d->x, 2) || !aligned(d->gu, 2) || !aligned(d->down, 2) || !aligned(d->picks, 4) || !aligned(d->weights, 4) ||
+        !aligned(d->out, type_bytes(d->out_type)) || (d->residual && !aligned(d->residual, type_bytes(d->residual_type))))
+        return fail(GFR_EINVAL, "experts16: tensors must be aligned to their elements");
+    if (!aligned(d->workspace, 16)) return fail(GFR_EINVAL, "experts16: the workspace must be 16-byte aligned");
+    if (d->workspace_bytes < need)
+        return fail(GFR_EINVAL, "experts16: workspace of %lld bytes, %lld needed", (long long)d->workspace_bytes, (long long)need);
+    const int64_t leaders = rows * d->slots < E ? rows * d->slots : E;   // a launch's threads: 2^32, 512 a workgroup
+    if (leaders * ((I + 63) / 64 * 4) >= 1 << 23 || leaders * ((H + 15) / 16) >= 1 << 23 || rows * ((H + 3) / 4) >= (int64_t)1 << 31)
+        return fail(GFR_EINVAL, "experts16: %d rows of %d slots are too many for a launch", d->rows, d->slots);
+    const auto whole = [](const void* p, int64_t elements, int64_t size) {
+        return RowBytes{reinterpret_cast<uintptr_t>(p), elements * size, elements * size, 1};
+    };
+    const RowBytes out = rows_of(d->out, d->out_type, rows, H, d->out_stride), space = whole(d->workspace, need, 1);
+    const RowBytes operands[] = {rows_of(d->x, d->type, rows, H, d->x_stride),
+                                 whole(d->gu, (E - 1) * d->gu_expert + (2 * I - 1) * d->gu_stride + H, 2),
+                                 whole(d->down, (E - 1) * d->down_expert + (H - 1) * d->down_stride + I, 2),
+                                 whole(d->picks, rows * d->slots, 4), whole(d->weights, rows * d->slots, 4)};
+    const char* const names[] = {"x", "gu", "down", "picks", "weights"};
+    for (int i = 0; i < 5; ++i) {
+        if (overlap(out, operands[i])) return fail(GFR_EINVAL, "experts16: out overlaps %s", names[i]);
+        if (overlap(space, operands[i])) return fail(GFR_EINVAL, "experts16: the workspace overlaps %s", names[i]);
+    }
+    if (overlap(out, space)) return fail(GFR_EINVAL, "experts16: out overlaps the workspace");
+    if (d->residual) {
+        const RowBytes residual = rows_of(d->residual, d->residual_type, rows, H, d->residual_stride);
+        const bool in_place = d->residual == d->out && d->residual_type == d->out_type &&
+                              (rows == 1 || d->residual_stride == d->out_stride);
+        if (!in_place && overlap(out, residual)) return fail(GFR_EINVAL, "experts16: out overlaps the residual, and is not the residual itself");
+        if (overlap(space, residual)) return fail(GFR_EINVAL, "experts16: the workspace overlaps the residual");
+    }
+    gfr::Experts16Job job = {d->x, d->gu, d->down, d->picks, d->weights, d->residual, d->out, d->x_stride, d->gu_stride,
+                             d->gu_expert, d->down_stride, d->down_expert, d->residual_stride, d->out_stride, d->rows,
+                             d->slots, d->hidden, d->inter, d->experts, d->type, d->residual_type, d->out_type, d->act,
+                             d->limit > 0.f ? d->limit : __builtin_inff(), 0, 0, nullptr, nullptr};
+    hipError_t e = gfr::launch_experts16(stream, job, d->workspace);
+    if (e != hipSuccess) return hip_fail(e, "experts16");
+    return 0;
+}
+
 // ---- norms around a block -----------------------------------------------------------------------------------------
 }  // extern "C"
 namespace {

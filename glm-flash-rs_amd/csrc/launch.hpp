@@ -166,6 +166,30 @@ hipError_t launch_dense(hipStream_t s, DenseJob d);
 // The form that launch_dense takes (gfr_dense_form's numbers); host only.
 int dense_form(const DenseJob& d);
 
+// experts16.hip
+// out[r] = residual[r] + sum over s of weights[r][s] * MLP of expert picks[r][s] of x[r] (picks outside [0, experts): none)
+struct Experts16Job {
+    const uint16_t* x;
+    const uint16_t* gu;             // [experts][2 inter][hidden]: gate rows, then up rows
+    const uint16_t* down;           // [experts][hidden][inter]
+    const int* picks;               // [rows][slots]
+    const float* weights;
+    const void* residual;
+    void* out;
+    int64_t x_stride, gu_stride, gu_expert, down_stride, down_expert, residual_stride, out_stride;
+    int rows, slots, hidden, inter, experts;
+    int type, residual_type, out_type;
+    int act;
+    float limit;                    // infinity: none
+    // set by launch_experts16: in the workspace the activations [rows slots][2][inter_pad] (the two 16-bit parts) and the
+    // pairs' outputs [rows slots][hidden_pad]
+    int inter_pad, hidden_pad;
+    uint16_t* acts;
+    float* y;
+};
+size_t experts16_workspace(int rows, int slots, int hidden, int inter);
+hipError_t launch_experts16(hipStream_t s, Experts16Job d, void* workspace);
+
 // norm.hip
 // A norm: (z - mean) / sqrt(mean of squares + eps) * (weight + offset) + bias; layer false: the mean is taken as 0.
 struct NormPart {

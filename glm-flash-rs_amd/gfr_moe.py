@@ -113,6 +113,8 @@ def _load() -> ctypes.CDLL:
         "gfr_block_norm_run": ([P, P], I),
         "gfr_logprobs_workspace": ([I, I, I], ctypes.c_int64),
         "gfr_logprobs_run": ([P, P], I),
+        "gfr_experts16_workspace": ([I, I, I, I], ctypes.c_int64),
+        "gfr_experts16_run": ([P, P], I),
         "gfr_moe_reserve_bf16": ([VP], I),
         "gfr_moe_run_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
         "gfr_moe_run_router_bf16": ([VP, P, ctypes.POINTER(_Exl3Struct), P, P, ctypes.POINTER(_Bf16Struct), I], I),
@@ -377,6 +379,16 @@ class Gate:
                           self.scale, 0 if bias is None else bias.data_ptr())
 
 
+@dataclass
+class Experts16:
+    """A layer's 16-bit routed experts: gu [experts, 2 inter, hidden] (gate rows, then up rows) and down [experts, hidden,
+    inter], bf16 or fp16 on the GPU, columns neighbours. A shared expert may be the last one: route_gate's picks have the id
+    `routed` in their last slot."""
+
+    gu: torch.Tensor
+    down: torch.Tensor
+
+
 _NORMS = {"rms": 1, "layer": 2}
 
 
@@ -409,10 +421,11 @@ class Norm:
 
 
 _NO_NORM = (0, 0, 0, 0.0, 0.0, 0, 0)
-# gfr_gate, gfr_dense, gfr_block_norm and gfr_logprobs as bytes in the machine's layout: packed anew for every call, which a ctypes
-# structure of as many fields takes about three times as long for
+# gfr_gate, gfr_dense, gfr_experts16, gfr_block_norm and gfr_logprobs as bytes in the machine's layout: packed anew for every
+# call, which a ctypes structure of as many fields takes about three times as long for
 _GATE = struct.Struct("@5ifP")
 _DENSE = struct.Struct("@4iPqPq2ifiP2iPqPq")
+_EXPERTS16 = struct.Struct("@7if2iPqPqqPqqPPPqPqPq")
 _LOGPROBS = struct.Struct("@6ifPqPq5Pq")
 _BLOCK_NORM = struct.Struct("@9i2fPqPqPqPqPq3i2f2P3i2f2P")
 
@@ -1057,6 +1070,62 @@ def _result(out, shape, dtype, like, stream, here, name="out"):
         raise ValueError(f"{name} {tuple(out.shape)} {out.dtype}: want {tuple(shape)} in bf16, fp16 or fp32")
     if out.get_device() != here:
         _elsewhere(out)
+    return out
+
+
+def experts16(x: torch.Tensor, experts: Experts16, picks: torch.Tensor, weights: torch.Tensor, activation: str = "silu",
+              limit: float = None, residual: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = None,
+              stream=None):
+    """gfr_experts16_run: out[r] = residual[r] + the sum over r's slots of weights[r, s] * (down[e] a), e = picks[r, s],
+    a = act(min(g, limit)) * clamp(u, -limit, limit), g and u the halves of gu[e] x[r] (limit None or 0: none), for x [rows,
+    hidden] of the experts' type and route_gate's picks (int32) and weights (fp32) [rows, slots]. A pick outside the experts
+    (-1) adds nothing. residual and out [rows, hidden] in x's type or fp32 (out: x's by default); residual may be out itself,
+    an out that shares memory with an operand in any other way is refused, as are zero rows. The workspace comes from torch's
+    allocator on the call's stream. No gradient is recorded. A stream other than the current one is the caller's to order
+    after the inputs' writes; they have to stay alive until it is done."""
+    gu, down, dtype, act, types = experts.gu, experts.down, x.dtype, _ACTIVATIONS.get(activation), _TYPE
+    rows, hidden = x.shape
+    E, both, wide = gu.shape
+    inter = both // 2
+    if gu.dtype is not dtype or down.dtype is not dtype or wide != hidden or both % 2 or down.shape != (E, hidden, inter):
+        raise ValueError(f"x {tuple(x.shape)} {dtype}, gu {tuple(gu.shape)} {gu.dtype}, down {tuple(down.shape)} {down.dtype}: "
+                         "want [rows, hidden], [experts, 2 inter, hidden] and [experts, hidden, inter] of one 16-bit type")
+    if act is None:
+        raise ValueError(f"activation {activation!r} of {[a for a in _ACTIVATIONS if a]}")
+    if picks.dim() != 2 or picks.shape[0] != rows or weights.shape != picks.shape or picks.dtype is not torch.int32 or \
+            weights.dtype is not torch.float32 or not picks.is_contiguous() or not weights.is_contiguous():
+        raise ValueError(f"picks {tuple(picks.shape)} {picks.dtype}, weights {tuple(weights.shape)} {weights.dtype}: want "
+                         f"({rows}, slots) int32 and float32, contiguous")
+    here = _get_device()
+    if not (x.get_device() == gu.get_device() == down.get_device() == picks.get_device() == weights.get_device() == here):
+        _elsewhere(x, gu, down, picks, weights)
+    gu_expert, gu_stride, gu_step = gu.stride()
+    down_expert, down_stride, down_step = down.stride()
+    if (gu_step != 1 and hidden > 1) or (down_step != 1 and inter > 1):
+        raise ValueError(f"gu strides {gu.stride()}, down strides {down.stride()}: columns must be neighbours")
+    residual_at = residual_type = residual_stride = 0
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual {tuple(residual.shape)}: want ({rows}, {hidden})")
+        if residual.get_device() != here:
+            _elsewhere(residual)
+        residual_at, residual_type, residual_stride = residual.data_ptr(), types.get(residual.dtype, -1), _row_stride(residual)
+    if out is not None and out_dtype is not None and out.dtype is not out_dtype:
+        raise ValueError(f"out {out.dtype}: want {out_dtype}")
+    L, slots = _lib or lib(), picks.shape[1]
+    need = L.gfr_experts16_workspace(rows, slots, hidden, inter)
+    if need < 0:
+        _check(need)
+    out = _result(out, x.shape, out_dtype or dtype, x, stream, here)
+    workspace = _empty((need,), torch.uint8, x, stream)
+    handle = _handle(stream, here)
+    rc = L.gfr_experts16_run(
+        handle, _EXPERTS16.pack(rows, slots, hidden, inter, E, types.get(dtype, -1), act, limit or 0.0, residual_type,
+                                types.get(out.dtype, -1), x.data_ptr(), _row_stride(x), gu.data_ptr(), gu_stride, gu_expert,
+                                down.data_ptr(), down_stride, down_expert, picks.data_ptr(), weights.data_ptr(), residual_at,
+                                residual_stride, out.data_ptr(), _row_stride(out), workspace.data_ptr(), need))
+    if rc:
+        _check(rc)
     return out
 
 

@@ -342,6 +342,46 @@ int gfr_dense_run(hipStream_t stream, const gfr_dense* d);
  * + 16 where x's or w's rows are off 16-byte alignment. Negative: refused. */
 int gfr_dense_form(const gfr_dense* d);
 
+/* ---- 16-bit routed experts for a few tokens ---------------------------------------------------------------------
+ *   out[r] = residual[r] + sum over s of weights[r][s] * (down[e] a),  e = picks[r][s],
+ *   a = act(min(g, limit)) * clamp(u, -limit, limit),  g and u the halves of gu[e] x[r]        (limit 0: none)
+ * x [rows][x_stride], gu [experts][2 inter][hidden] (gate rows, then up rows; gu_stride elements between rows, gu_expert
+ * between experts) and down [experts][hidden][inter] (likewise) in `type` (GFR_BF16 or GFR_F16); picks and weights
+ * [rows][slots] as gfr_route_gate gives them (a shared expert is the last of the stacks, its id `routed`); out and residual
+ * in `type` or GFR_F32, residual may be NULL. A pick outside [0, experts) adds nothing: a row padded with -1 gets its
+ * residual, or zeros. Picks of a row may repeat, each counts. Sums, activations and weights in fp32, the activations kept
+ * to 16 bits or more between the products (with fp16 weights, beyond 131008 they are infinite), one rounding to out's
+ * type. A row's result depends neither on the other rows nor on how many there are. The weights of the picked experts are
+ * read once for 64 rows of theirs (for 16 in windows of up to 16 rows): meant for windows in which an expert has few.
+ * Any size, stride and element-aligned address works, rows at 16-byte aligned addresses are the fast ones. residual may be
+ * out itself (address, type and stride); an out that shares memory with an operand in any other way is refused.
+ * workspace: gfr_experts16_workspace(rows, slots, hidden, inter) bytes of device memory, 16-byte aligned, that are the
+ * call's until its work is done: two calls that may overlap, or two captured graphs that may, take two workspaces.
+ * rows, slots >= 1 and rows * slots <= 65536; hidden and inter <= 2^20, experts <= 65536. */
+typedef struct gfr_experts16 {
+    int rows, slots, hidden, inter, experts;
+    int type;
+    int act;
+    float limit;
+    int residual_type, out_type;
+    const uint16_t* x;
+    int64_t x_stride;
+    const uint16_t* gu;
+    int64_t gu_stride, gu_expert;
+    const uint16_t* down;
+    int64_t down_stride, down_expert;
+    const int32_t* picks;
+    const float* weights;
+    const void* residual;
+    int64_t residual_stride;
+    void* out;
+    int64_t out_stride;
+    void* workspace;
+    int64_t workspace_bytes;
+} gfr_experts16;
+int64_t gfr_experts16_workspace(int rows, int slots, int hidden, int inter);   /* negative: GFR_EINVAL */
+int gfr_experts16_run(hipStream_t stream, const gfr_experts16* d);
+
 /* ---- The norms around a block, with its gate and residual -----------------------------------------------------
  *   v = post(x) * f(gate);  h = residual_scale * residual + scale * v;  y = pre(h)
  * a norm: (z - mean) / sqrt(mean of (z - mean)^2 + eps) * (weight + offset) + bias over a row's n columns, the mean 0 for

@@ -81,3 +81,45 @@ def test_logprobs_workspace():
         assert 1 <= chunks <= 64 and chunks * 32768 >= vocab
         assert L.gfr_logprobs_workspace(rows, vocab, 32) == rows * chunks * (16 + 32 * 8)
     assert L.gfr_logprobs_workspace(0, 10, 0) < 0 and L.gfr_logprobs_workspace(1, 10, 11) < 0
+
+
+EXPERTS = ("rows slots hidden inter experts type act limit residual_type out_type x x_stride gu gu_stride gu_expert down "
+           "down_stride down_expert picks weights residual residual_stride out out_stride workspace workspace_bytes").split()
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(rows=0), "rows 0"), (dict(slots=0), "slots 0"), (dict(rows=8193, slots=8), "65536 pairs"), (dict(hidden=0), "hidden 0"),
+    (dict(inter=-1), "inter -1"), (dict(hidden=(1 << 20) + 1), "outside"), (dict(experts=0), "experts 0"),
+    (dict(experts=65537), "experts 65537"), (dict(x=0), "null"), (dict(gu=0), "null"), (dict(down=0), "null"), (dict(picks=0), "null"),
+    (dict(weights=0), "null"), (dict(out=0), "null"), (dict(workspace=0), "null"), (dict(type=2), "type 2"),
+    (dict(out_type=1), "x's type or fp32"), (dict(residual=1 << 50, residual_type=1), "x's type or fp32"), (dict(act=5), "activation 5"),
+    (dict(limit=-1.0), "limit"), (dict(limit=float("nan")), "limit"), (dict(x_stride=63), "stride of x 63"),
+    (dict(gu_stride=63), "gu 63"), (dict(down_stride=31), "down 31"), (dict(out_stride=63), "out 63"),
+    (dict(residual=1 << 50, residual_stride=63), "residual 63"), (dict(x_stride=(1 << 31) + 1), "2^31"), (dict(gu_expert=-1), "between experts"),
+    (dict(down_expert=(1 << 40) + 1), "between experts"), (dict(x=(1 << 40) + 1), "aligned"), (dict(picks=(1 << 43) + 2), "aligned"),
+    (dict(out=(1 << 45) + 2, out_type=2), "aligned"), (dict(workspace=(1 << 46) + 8), "16-byte"), (dict(workspace_bytes=100), "workspace of 100"),
+    (dict(rows=65536, slots=1, hidden=1 << 20, experts=65536, x_stride=1 << 20, gu_stride=1 << 20, out_stride=1 << 20,
+          workspace_bytes=1 << 62), "too many"),
+    (dict(out=1 << 40), "overlaps x"), (dict(out=(1 << 41) + 1000), "overlaps gu"), (dict(out=1 << 42), "overlaps down"),
+    (dict(out=1 << 43), "overlaps picks"), (dict(out=1 << 44), "overlaps weights"), (dict(workspace=1 << 41), "workspace overlaps gu"),
+    (dict(workspace=(1 << 45) + 16), "out overlaps the workspace"), (dict(residual=1 << 45, residual_stride=65), "not the residual itself"),
+    (dict(residual=1 << 46), "workspace overlaps the residual"),
+])
+def test_experts16_refuses(kw, needle):
+    import gfr_moe
+    a = dict(rows=4, slots=2, hidden=64, inter=32, experts=5, type=0, act=4, limit=0.0, residual_type=0, out_type=0, x=1 << 40,
+             x_stride=64, gu=1 << 41, gu_stride=64, gu_expert=64 * 64, down=1 << 42, down_stride=32, down_expert=64 * 32,
+             picks=1 << 43, weights=1 << 44, residual=0, residual_stride=64, out=1 << 45, out_stride=64, workspace=1 << 46,
+             workspace_bytes=1 << 20)
+    a.update(kw)
+    L = gfr_moe.lib()
+    refused(L.gfr_experts16_run(None, gfr_moe._EXPERTS16.pack(*[a[n] for n in EXPERTS])), needle)
+    refused(L.gfr_experts16_run(None, None), "null")
+
+
+def test_experts16_workspace():
+    """Room for the activations' two parts, padded to whole chunks, and the pairs' outputs."""
+    import gfr_moe
+    L = gfr_moe.lib()
+    assert L.gfr_experts16_workspace(3, 2, 65, 65) >= 6 * (2 * 2 * 128 + 4 * 68)
+    assert L.gfr_experts16_workspace(8192, 8, 4096, 512) > 0 and L.gfr_experts16_workspace(8193, 8, 4096, 512) < 0
