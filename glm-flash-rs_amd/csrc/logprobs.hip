@@ -7,8 +7,8 @@
 // the sums against it, so that the row is read once and nothing is rescaled. S is held as C, the number of logits that equal
 // the maximum, and R, the sum over the others: where one token has nearly all of the probability, log S = log(1 + R) keeps
 // what 1 + R would round off. A second launch joins a row's chunks.
-// The most likely tokens of a chunk: with the lanes in G groups (G at least as many as are asked for) the least of the
-// groups' maxima is a threshold that G logits reach, and few more. These go to LDS, each counts those before it in the order
+// The most likely tokens of a chunk: maxima of sets of its logits give a threshold that as many logits reach as are asked
+// for, and few more. These go to LDS, each counts those before it in the order
 // (larger logits first, the lower token first among equal ones), and that is its place. Where more reach it than LDS has
 // room for (rows of one value, rows in order), the places are filled one by one.
 #include <hip/hip_runtime.h>
@@ -62,10 +62,46 @@ __device__ __forceinline__ Eight load_logits(const void* row, int64_t c, int64_t
     return e;
 }
 
+// The logits of a group, converted anew by instructions that the compiler takes for others each time: it would keep the
+// values of one use for the next, in twice the registers.
+template <int TYPE>
+__device__ __forceinline__ f8_t fresh(const Eight& e) {
+    if constexpr (TYPE == TYPE_F32) return values(e, TYPE);
+    const uint32_t h[4] = {e.a.x, e.a.y, e.a.z, e.a.w};
+    f8_t l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        if constexpr (TYPE == TYPE_BF16)
+            asm volatile("v_lshlrev_b32 %0, 16, %2\n\tv_and_b32 %1, 0xffff0000, %2" : "=&v"(lo), "=v"(hi) : "v"(h[j]));
+        else
+            asm volatile("v_cvt_f32_f16 %0, %2\n\tv_cvt_f32_f16_sdwa %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1"
+                         : "=&v"(lo), "=v"(hi) : "v"(h[j]));
+        l[2 * j] = lo, l[2 * j + 1] = hi;
+    }
+    return l;
+}
+
+// A logit that at least `top` of a chunk's logits reach, and few more: the lanes' maxima are those of 64 sets. For up to 8
+// places the least of eight sets' maxima (22 logits reach it on average), for more the place's largest of the 64 (44 reach
+// the 32nd).
+__device__ __forceinline__ float threshold(float set, int top) {
+    if (top <= 8) {
+        set = fmaxf(set, lane_xor_f<8>(set));
+        set = fmaxf(set, lane_xor_f<16>(set));
+        set = fmaxf(set, lane_xor_f<32>(set));
+        return -max_over(8, -set);
+    }
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) above += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, set), i)) > set;
+    return -max_over(64, above < top ? -set : -INFINITY);
+}
+
 // V groups of eight logits a thread: group g of thread i starts at the chunk's column 8 (g THREADS + i).
 template <int TYPE, int V>
 __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) {
-    __shared__ float maxima[32];
+    __shared__ float maxima[WAVES][64];
     __shared__ float sums[WAVES][3];
     __shared__ uint64_t places[ROOM];
     __shared__ int found;
@@ -77,88 +113,106 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
 #pragma unroll
     for (int g = 0; g < V; ++g) raw[g] = load_logits<TYPE>(logits, c0 + 8 * (g * THREADS + tid), end);
     if (tid == 0) found = 0;
-    float most = -INFINITY;                                           // fmaxf leaves NaN out
+    float each[V], most = -INFINITY;                                  // (fmaxf leaves NaN out)
 #pragma unroll
     for (int g = 0; g < V; ++g) {
-        const f8_t l = values(raw[g], TYPE);
+        const f8_t l = fresh<TYPE>(raw[g]);
+        each[g] = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, l[j]);
+        for (int j = 0; j < 8; ++j) each[g] = fmaxf(each[g], l[j]);
+        most = fmaxf(most, each[g]);
     }
-    // maxima of 16 neighbouring lanes, or of more where fewer places are asked for
-    const float near = max_over(d.top <= 8 ? 64 : d.top <= 16 ? 32 : 16, most);
-    if ((lane & 15) == 0) maxima[wave * 4 + lane / 16] = near;
+    maxima[wave][lane] = most;
     __syncthreads();
-    const float one = maxima[lane & 31], M = max_over(32, one), least = -max_over(32, -one);
+    // each lane's maximum over the waves: 64 sets of logits whose columns lie among each other
+    float set = maxima[0][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) set = fmaxf(set, maxima[w][lane]);
+    const float M = max_over(64, set);
+    const float least = d.top ? threshold(set, d.top) : 0.f;
 
+    // exp(z) = exp2(l k + c) with c = -M k: c's rounding is a factor of all terms, taken out of the sums afterwards. slope
+    // is summed in units of the exponent.
+    // Where M k is no finite number all others are too far below M to count (their distance is at least 2^-24 of M), or
+    // there are none.
+    const float by = LOG2E * d.by;
+    const bool finite = fabsf(M * by) < INFINITY;
+    const float k = finite ? by : 0.f, c = finite ? -M * k : -1e30f, off = finite ? fmaf(-M, k, -c) : 0.f;
+    const auto exponent = [&](float l) { return fmaxf(fmaf(l, k, c), -1e30f); };   // -1e30: masked, and exp2 of it is 0
     float rest = 0.f, slope = 0.f, count = 0.f;
-    const float k = LOG2E * d.by;
 #pragma unroll
     for (int g = 0; g < V; ++g) {
-        const f8_t l = values(raw[g], TYPE);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = fmaxf(l[j] - M, -1e30f);                  // -1e30: masked, and exp2 of it is 0
-            const float e = __builtin_amdgcn_exp2f(x * k);
-            rest += e, slope = fmaf(x, e, slope);
-        }
-    }
-    if (most == M) {                                                  // few threads: again without the largest
-        rest = 0.f;
-#pragma unroll
-        for (int g = 0; g < V; ++g) {
-            const f8_t l = values(raw[g], TYPE);
+        // (two loops and no third that serves both: the compiler would merge them, and do the work of both for every group)
+        if (__ballot(each[g] >= M)) {                                 // few: the maximum itself, and groups of masked ones
+            const f8_t l = fresh<TYPE>(raw[g]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float e = __builtin_amdgcn_exp2f(fmaxf(l[j] - M, -1e30f) * k);
+                const float x = exponent(l[j]), e = __builtin_amdgcn_exp2f(x);
                 if (l[j] == M) count += 1.f;
-                else rest += e;
+                else rest += e, slope = fmaf(x, e, slope);
             }
+            asm volatile("; the maximum's group" : "+v"(rest), "+v"(slope), "+v"(count));
+        } else {
+            const f8_t l = fresh<TYPE>(raw[g]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = exponent(l[j]), e = __builtin_amdgcn_exp2f(x);
+                rest += e, slope = fmaf(x, e, slope);
+            }
+            asm volatile("; another group" : "+v"(rest), "+v"(slope));
         }
-        if (M == -INFINITY) count = 0.f;
     }
+    if (M == -INFINITY) count = rest = slope = 0.f;
     rest = sum_over(64, rest), slope = sum_over(64, slope), count = sum_over(64, count);
     if (lane == 0) sums[wave][0] = rest, sums[wave][1] = slope, sums[wave][2] = count;
     if (d.top && most >= least) {
 #pragma unroll
-        for (int g = 0; g < V; ++g) {
-            const f8_t l = values(raw[g], TYPE);
+        for (int g = 0; g < V; ++g)
+            if (each[g] >= least && each[g] > -INFINITY) {
+                const f8_t l = fresh<TYPE>(raw[g]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (l[j] >= least && l[j] > -INFINITY) {
-                    const int at = atomicAdd(&found, 1);
-                    if (at < ROOM) places[at] = place_of(l[j], (int)(c0 + 8 * (g * THREADS + tid) + j));
-                }
-        }
+                for (int j = 0; j < 8; ++j)
+                    if (l[j] >= least && l[j] > -INFINITY) {
+                        const int at = atomicAdd(&found, 1);
+                        if (at < ROOM) places[at] = place_of(l[j], (int)(c0 + 8 * (g * THREADS + tid) + j));
+                    }
+            }
     }
     __syncthreads();
     const int64_t part = (int64_t)row * d.chunks + chunk;
-    if (tid == 0) {
-        Share s = {M, 0.f, 0.f, 0.f};
-        for (int w = 0; w < WAVES; ++w) s.rest += sums[w][0], s.slope += sums[w][1], s.count += sums[w][2];
-        static_cast<Share*>(d.shares)[part] = s;
+    if (tid < WAVES) {
+        Share s = {M, sum_over(WAVES, sums[tid][2]), sum_over(WAVES, sums[tid][0]), sum_over(WAVES, sums[tid][1])};
+        const float right = __builtin_amdgcn_exp2f(-off);
+        s.rest *= right, s.slope *= right / by;
+        if (tid == 0) static_cast<Share*>(d.shares)[part] = s;
     }
     if (!d.top) return;
     uint64_t* out = static_cast<uint64_t*>(d.places) + part * d.top;
     const int n = found;
     if (n <= ROOM) {
         if (tid >= n && tid < d.top) out[tid] = 0;
-        for (int i = tid; i < n; i += THREADS) {
+        // 2^by lanes count those before a place
+        int by = 6;
+        while (by && n << by > THREADS) --by;
+        for (int i = tid >> by; i < n; i += THREADS >> by) {
             const uint64_t p = places[i];
-            int place = 0;
-            for (int o = 0; o < n; ++o) place += places[o] > p;
-            if (place < d.top) out[place] = p;
+            int before = 0;
+            for (int o = tid & ((1 << by) - 1); o < n; o += 1 << by) before += places[o] > p;
+            before = sum_over(1 << by, before);
+            if (before < d.top) out[before] = p;
         }
         return;
     }
     uint64_t last = ~0ull;
     for (int i = 0; i < d.top; ++i) {                                 // (more than ROOM: none of them stays empty)
         uint64_t best = 0;
-#pragma unroll
-        for (int g = 0; g < V; ++g) {
-            const f8_t l = values(raw[g], TYPE);
+#pragma unroll 1
+        for (int g = 0; g < V; ++g) {                                 // (loaded again: registers hold no index)
+            const int64_t c = c0 + 8 * (g * THREADS + tid);
+            const f8_t l = values(load_logits<TYPE>(logits, c, end), TYPE);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint64_t p = place_of(l[j], (int)(c0 + 8 * (g * THREADS + tid) + j));
+                const uint64_t p = place_of(l[j], (int)c + j);
                 if (l[j] > -INFINITY && p < last && p > best) best = p;
             }
         }
@@ -172,28 +226,31 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
     }
 }
 
-// A wave a row: the chunks' shares against the row's largest logit, the tokens, the places.
-__global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsJob d) {
-    const int lane = threadIdx.x, row = blockIdx.x;
-    const Share* shares = static_cast<const Share*>(d.shares) + (int64_t)row * d.chunks;
+// A workgroup a row: the chunks' shares against the row's largest logit, in every wave; the tokens in all waves, the places
+// in the first.
+constexpr int JOIN = 256;
+__global__ void __launch_bounds__(JOIN) logprobs_join_kernel(LogprobsJob d) {
+    extern __shared__ uint64_t places[];
+    const int tid = threadIdx.x, lane = tid & 63, row = blockIdx.x;
+    const uint64_t* from = static_cast<const uint64_t*>(d.places) + (int64_t)row * d.chunks * d.top;
+    for (int i = tid; i < d.chunks * d.top; i += JOIN) places[i] = from[i];
     Share s = {-INFINITY, 0.f, 0.f, 0.f};
-    if (lane < d.chunks) s = shares[lane];
+    if (lane < d.chunks) s = static_cast<const Share*>(d.shares)[(int64_t)row * d.chunks + lane];
     const float M = max_over(64, s.most);
     float count = s.count, rest = s.rest, slope = s.slope;
     if (s.most < M) {
         const float x = fmaxf(s.most - M, -1e30f), e = __builtin_amdgcn_exp2f(x * (LOG2E * d.by)), all = s.count + s.rest;
         count = 0.f, rest = all * e, slope = e * fmaf(x, all, s.slope);
     }
-#pragma unroll
-    for (int m = 32; m; m >>= 1) count += __shfl_xor(count, m), rest += __shfl_xor(rest, m), slope += __shfl_xor(slope, m);
+    count = sum_over(64, count), rest = sum_over(64, rest), slope = sum_over(64, slope);
     const float log_sum = logf(count) + log1pf(rest / count);
     const auto log_p = [&](float l) {
         if (!(l > -INFINITY)) return -INFINITY;
         return (l == M ? 0.f : (l - M) * d.by) - log_sum;
     };
-    if (lane == 0) d.entropy[row] = count > 0.f ? log_sum - slope * d.by / (count + rest) : 0.f;
+    if (tid == 0) d.entropy[row] = count > 0.f ? log_sum - slope * d.by / (count + rest) : 0.f;
     const int64_t base = (int64_t)row * d.stride;
-    for (int i = lane; i < d.tokens; i += 64) {
+    for (int i = JOIN - 1 - tid; i < d.tokens; i += JOIN) {           // (from the last wave on: the first has the places)
         const int64_t at = (int64_t)row * d.tokens_stride + i;
         const int64_t token = d.wide_tokens ? static_cast<const int64_t*>(d.token)[at] : static_cast<const int32_t*>(d.token)[at];
         const bool there = token >= 0 && token < d.vocab;             // a token that is not in the vocabulary: probability 0
@@ -201,21 +258,22 @@ __global__ void __launch_bounds__(64) logprobs_join_kernel(LogprobsJob d) {
     }
     if (!d.top) return;
     // a chunk's places are in order, so that the next one is the largest of the chunks' heads
-    extern __shared__ uint64_t places[];
-    const uint64_t* from = static_cast<const uint64_t*>(d.places) + (int64_t)row * d.chunks * d.top;
-    for (int i = lane; i < d.chunks * d.top; i += 64) places[i] = from[i];
     __syncthreads();
+    if (tid >= 64) return;
     int* ids = d.top_ids + (int64_t)row * d.top;
     float* logps = d.top_logprobs + (int64_t)row * d.top;
-    int next = lane * d.top + 1;
-    uint64_t head = lane < d.chunks ? places[lane * d.top] : 0;
+    const int end = lane < d.chunks ? (lane + 1) * d.top : 0;
+    int next = lane * d.top;
+    const auto take = [&] { return next < end ? places[next++] : 0; };
+    uint64_t head = take(), after = take(), kept = 0;
     int i = 0;
     for (; i < d.top; ++i) {
         const uint64_t best = max_over(64, head);
         if (!best) break;
-        if (lane == 0) ids[i] = token_of(best), logps[i] = log_p(logit_of(best));
-        if (head == best) head = next < (lane + 1) * d.top ? places[next++] : 0;
+        if (lane == i) kept = best;
+        if (head == best) head = after, after = take();
     }
+    if (lane < i) ids[lane] = token_of(kept), logps[lane] = log_p(logit_of(kept));
     // fewer logits than places are not masked: the masked tokens in order, enough of which are among the first 64
     if (i < d.top) {
         const bool masked = lane < d.vocab && !(load_one(d.logits, d.type, base + lane) > -INFINITY);
@@ -229,7 +287,7 @@ hipError_t launch(hipStream_t s, const LogprobsJob& d) {
     logprobs_chunk_kernel<TYPE, V><<<dim3((unsigned)(d.rows * (int64_t)d.chunks)), THREADS, 0, s>>>(d);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    logprobs_join_kernel<<<dim3((unsigned)d.rows), 64, (size_t)d.chunks * d.top * sizeof(uint64_t), s>>>(d);
+    logprobs_join_kernel<<<dim3((unsigned)d.rows), JOIN, (size_t)d.chunks * d.top * sizeof(uint64_t), s>>>(d);
     return hipGetLastError();
 }
 template <int TYPE>
@@ -242,8 +300,8 @@ hipError_t launch(hipStream_t s, const LogprobsJob& d, int groups) {
     }
 }
 
-// Groups of eight logits a thread: as many as leave two workgroups a CU, and so many that a row has at most 64 chunks, one
-// a lane of the join.
+// Groups of eight logits a thread: 8, and fewer where that leaves CUs idle, as long as a row has no more chunks than the
+// join has lanes. (4096 rows of 160000 bf16, top 4, with 2, 4 and 8 groups: 440, 304 and 264 us.)
 int chunks_of(int vocab, int groups) { return (int)(((int64_t)vocab + 8 * THREADS * groups - 1) / (8 * THREADS * groups)); }
 int groups_of(int rows, int vocab) {
     int v = 8;
