@@ -33,6 +33,14 @@ __device__ __forceinline__ int find_members(const Experts16Job& d, int expert, i
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, pairs = d.rows * d.slots;
     int seen = 0;
     first = pairs;
+    if (pairs <= 64) {                                                // each wave by itself, all with the same values
+        const uint64_t ballot = __ballot(lane < pairs && d.picks[lane < pairs ? lane : 0] == expert);
+        const int at = __popcll(ballot & ((1ull << lane) - 1)) - from;
+        if ((ballot >> lane & 1) && at >= 0 && at < room) m.pair[at] = lane;
+        if (ballot) first = __builtin_ctzll(ballot);
+        __builtin_amdgcn_wave_barrier();
+        return __popcll(ballot);
+    }
     for (int base = 0; base < pairs; base += blockDim.x) {
         const int p = base + (int)threadIdx.x;
         const bool mine = p < pairs && d.picks[p] == expert;
@@ -67,20 +75,33 @@ __device__ __forceinline__ int expert_of(const Experts16Job& d, int u, int room,
 // that the fragments' reads of neighbouring rows meet all banks.
 template <int TYPE, int EB>
 struct Weights {
-    const uint16_t* at[2 * EB];                                       // this lane's 16 bytes of every 8 rows
+    const uint16_t* row[2 * EB];                                      // this lane's row of every eight
     struct Chunk {
         uint4 w[2 * EB];
     };
-    __device__ __forceinline__ void load(Chunk& f, int k, int K) const {
-        const int lane = threadIdx.x & 63;
-        if (k + 64 <= K) {
+    __device__ __forceinline__ void load(Chunk& f, int k) const {     // a whole chunk
+        k += (threadIdx.x & 7) * 8;
 #pragma unroll
-            for (int i = 0; i < 2 * EB; ++i) __builtin_memcpy(&f.w[i], at[i] + k, 16);
-        } else {
-            const int left = K - k - (lane & 7) * 8;                  // from this lane's first on; nothing past the end
+        for (int i = 0; i < 2 * EB; ++i) __builtin_memcpy(&f.w[i], row[i] + k, 16);
+    }
+    // any chunk of rows of at least eight, to be put in place where K ends in it
+    __device__ __forceinline__ void ask(Chunk& f, int k, int K) const {
+        k += (threadIdx.x & 7) * 8;
 #pragma unroll
-            for (int i = 0; i < 2 * EB; ++i) f.w[i] = load_chunk(at[i] + k, 0, left);
-        }
+        for (int i = 0; i < 2 * EB; ++i) f.w[i] = gfr::ask(row[i], k, K);
+    }
+    __device__ __forceinline__ void settle(Chunk& f, int k, int K) const {
+        k += (threadIdx.x & 7) * 8;
+#pragma unroll
+        for (int i = 0; i < 2 * EB; ++i) f.w[i] = gfr::settle(f.w[i], k, K);
+    }
+    // the one that K ends in, in place
+    __device__ __forceinline__ void load_last(Chunk& f, int k, int K) const {
+        k += (threadIdx.x & 7) * 8;
+#pragma unroll
+        for (int i = 0; i < 2 * EB; ++i) f.w[i] = ask_any(row[i], k, K);
+#pragma unroll
+        for (int i = 0; i < 2 * EB; ++i) f.w[i] = settle_any(f.w[i], row[i], k, K);
     }
     __device__ __forceinline__ void stage(const Chunk& f, char* stage) const {
         const int lane = threadIdx.x & 63;
@@ -97,6 +118,23 @@ struct Weights {
     }
 };
 
+// U chunks in flight: f[u] of the n that this wave takes is used and asked for again U further on. Past the end the last one
+// is asked for once more (the caches have it): a load under a condition would have the compiler wait for all loads wherever
+// it cannot tell how many there are.
+template <int U, typename Chunk, typename Load, typename Use>
+__device__ __forceinline__ void pipeline(Chunk (&f)[U], int n, Load load, Use use) {
+    if (n <= 0) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(f[u], min(u, n - 1));
+    for (int i = 0; i < n; i += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u < n) use(f[u]);
+            load(f[u], min(i + u + U, n - 1));
+        }
+    }
+}
+
 // ---- gate and up --------------------------------------------------------------------------------------------------
 constexpr int UP_WAVES = 8, UP_TILES = 2, UP_COLS = 8 * UP_TILES;
 
@@ -106,12 +144,12 @@ template <int TYPE, int RB>
 __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYPE, UP_TILES>& w, const Members& m, int members,
                                         int c0, char* lds) {
     constexpr int EB = UP_TILES, U = 2;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a = lane & 15, q = lane >> 4;
     const uint16_t* xp[RB];
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
         const int pair = m.pair[min(16 * j + a, members - 1)];
-        xp[j] = d.x + (int64_t)(pair / d.slots) * d.x_stride + 8 * q;
+        xp[j] = d.x + (int64_t)(pair / d.slots) * d.x_stride;
     }
     struct Chunk {
         typename Weights<TYPE, EB>::Chunk w;
@@ -122,13 +160,15 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
     for (int i = 0; i < EB; ++i)
 #pragma unroll
         for (int j = 0; j < RB; ++j) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
-    const int chunks = (d.hidden + 63) / 64;
-    auto load = [&](Chunk& f, int c) {
-        w.load(f.w, c * 64, d.hidden);
+    const int chunks = d.hidden / 64;                                 // whole ones
+    const bool last = d.hidden % 64 && wave == chunks % UP_WAVES;     // this wave has the one that hidden ends in
+    auto load = [&](Chunk& f, int i) {
+        const int c = wave + i * UP_WAVES;
+        w.load(f.w, c * 64);
 #pragma unroll
         for (int j = 0; j < RB; ++j)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) f.x[j][s] = load_chunk(xp[j] + c * 64 + 32 * s, 0, d.hidden - c * 64 - 32 * s - 8 * q);
+            for (int s = 0; s < 2; ++s) __builtin_memcpy(&f.x[j][s], xp[j] + c * 64 + 32 * s + 8 * q, 16);
     };
     char* stage = lds + wave * EB * 2048;
     auto multiply = [&](const Chunk& f) {
@@ -143,15 +183,19 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
             }
     };
     Chunk f[U];
+    pipeline(f, (chunks - wave + UP_WAVES - 1) / UP_WAVES, load, multiply);
+    if (last) {
+        const int k = chunks * 64, K = d.hidden;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (wave + u * UP_WAVES < chunks) load(f[u], wave + u * UP_WAVES);
-    for (int c = wave; c < chunks; c += U * UP_WAVES) {
+        for (int j = 0; j < RB; ++j)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (c + u * UP_WAVES < chunks) multiply(f[u]);
-            if (c + (u + U) * UP_WAVES < chunks) load(f[u], c + (u + U) * UP_WAVES);
-        }
+            for (int s = 0; s < 2; ++s) f[0].x[j][s] = ask_any(xp[j], k + 32 * s + 8 * q, K);
+        w.load_last(f[0].w, k, K);
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) f[0].x[j][s] = settle_any(f[0].x[j][s], xp[j], k + 32 * s + 8 * q, K);
+        multiply(f[0]);
     }
     __syncthreads();
     f4_t* part = reinterpret_cast<f4_t*>(lds);                        // [UP_WAVES][EB * RB][64]
@@ -190,7 +234,7 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
 }
 
 template <int TYPE, int RB>
-__global__ void __launch_bounds__(64 * UP_WAVES) experts16_up_kernel(Experts16Job d) {
+__global__ void __launch_bounds__(64 * UP_WAVES, RB == 1 ? 4 : 2) experts16_up_kernel(Experts16Job d) {
     __shared__ __align__(1024) char lds[UP_WAVES * UP_TILES * (RB > 2 ? RB * 1024 : 2048)];
     __shared__ Members m;
     const int lane = threadIdx.x & 63, tiles = d.inter_pad / UP_COLS;
@@ -202,7 +246,7 @@ __global__ void __launch_bounds__(64 * UP_WAVES) experts16_up_kernel(Experts16Jo
 #pragma unroll
     for (int i = 0; i < 2 * UP_TILES; ++i) {
         const int row = min(c0 + (i >> 1) * 8 + (lane >> 3), d.inter - 1) + (i & 1) * d.inter;
-        w.at[i] = d.gu + (int64_t)e * d.gu_expert + (int64_t)row * d.gu_stride + (lane & 7) * 8;
+        w.row[i] = d.gu + (int64_t)e * d.gu_expert + (int64_t)row * d.gu_stride;
     }
     for (int from = 0;;) {
         const int members = min(count - from, 16 * RB);
@@ -222,11 +266,20 @@ __global__ void __launch_bounds__(64 * UP_WAVES) experts16_up_kernel(Experts16Jo
 // ---- down ---------------------------------------------------------------------------------------------------------
 constexpr int DOWN_WAVES = 4, DOWN_TILES = 2, DOWN_COLS = 16 * DOWN_TILES * DOWN_WAVES;
 
+// A tile's sum over a chunk, in an order that both forms of the product share (each adds the chunks' sums in turn).
+template <int TYPE>
+__device__ __forceinline__ f4_t chunk_sum(uint4 w0, uint4 w1, const uint4 (&x)[2][2]) {
+    f4_t v = mfma<TYPE>(w0, x[0][0], (f4_t){0.f, 0.f, 0.f, 0.f});
+    v = mfma<TYPE>(w0, x[0][1], v);
+    v = mfma<TYPE>(w1, x[1][0], v);
+    return mfma<TYPE>(w1, x[1][1], v);
+}
+
 // One pass: a wave's 16 DOWN_TILES columns from c0 on, for members [from, from + 16 RB), over the whole of k.
 template <int TYPE, int RB>
 __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<TYPE, DOWN_TILES>& w, const Members& m,
                                           int members, int c0, char* stage) {
-    constexpr int EB = DOWN_TILES, U = 2;
+    constexpr int EB = DOWN_TILES, U = RB == 4 ? 1 : 2;
     const int lane = threadIdx.x & 63, a = lane & 15, q = lane >> 4;
     const uint16_t* xp[RB];
 #pragma unroll
@@ -241,9 +294,8 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
     for (int i = 0; i < EB; ++i)
 #pragma unroll
         for (int j = 0; j < RB; ++j) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
-    const int chunks = d.inter_pad / 64;
-    auto load = [&](Chunk& f, int c) {
-        w.load(f.w, c * 64, d.inter);
+    const int chunks = d.inter / 64;                                  // whole ones
+    auto load_rows = [&](Chunk& f, int c) {
 #pragma unroll
         for (int j = 0; j < RB; ++j)
 #pragma unroll
@@ -252,30 +304,25 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
                 f.x[j][s][1] = *reinterpret_cast<const uint4*>(xp[j] + d.inter_pad + c * 64 + 32 * s);
             }
     };
+    auto load = [&](Chunk& f, int c) {
+        w.load(f.w, c * 64);
+        load_rows(f, c);
+    };
     auto multiply = [&](const Chunk& f) {
         w.stage(f.w, stage);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < EB; ++i) {
+            const uint4 w0 = w.fragment(stage, i, 0), w1 = w.fragment(stage, i, 1);
 #pragma unroll
-            for (int i = 0; i < EB; ++i) {
-                const uint4 fw = w.fragment(stage, i, s);
-#pragma unroll
-                for (int j = 0; j < RB; ++j) {
-                    acc[i][j] = mfma<TYPE>(fw, f.x[j][s][0], acc[i][j]);
-                    acc[i][j] = mfma<TYPE>(fw, f.x[j][s][1], acc[i][j]);
-                }
-            }
+            for (int j = 0; j < RB; ++j) acc[i][j] += chunk_sum<TYPE>(w0, w1, f.x[j]);
+        }
     };
     Chunk f[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (u < chunks) load(f[u], u);
-    for (int c = 0; c < chunks; c += U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (c + u < chunks) multiply(f[u]);
-            if (c + u + U < chunks) load(f[u], c + u + U);
-        }
+    pipeline(f, chunks, load, multiply);
+    if (d.inter % 64) {
+        load_rows(f[0], chunks);
+        w.load_last(f[0].w, chunks * 64, d.inter);
+        multiply(f[0]);
     }
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
@@ -290,7 +337,7 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
 }
 
 template <int TYPE, int RB>
-__global__ void __launch_bounds__(64 * DOWN_WAVES) experts16_down_kernel(Experts16Job d) {
+__global__ void __launch_bounds__(64 * DOWN_WAVES, RB == 1 ? 4 : 2) experts16_down_kernel(Experts16Job d) {
     __shared__ __align__(1024) char lds[DOWN_WAVES * DOWN_TILES * 2048];
     __shared__ Members m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tiles = (d.hidden + DOWN_COLS - 1) / DOWN_COLS;
@@ -301,8 +348,7 @@ __global__ void __launch_bounds__(64 * DOWN_WAVES) experts16_down_kernel(Experts
     Weights<TYPE, DOWN_TILES> w;
 #pragma unroll
     for (int i = 0; i < 2 * DOWN_TILES; ++i)
-        w.at[i] = d.down + (int64_t)e * d.down_expert + (int64_t)min(c0 + i * 8 + (lane >> 3), d.hidden - 1) * d.down_stride +
-                  (lane & 7) * 8;
+        w.row[i] = d.down + (int64_t)e * d.down_expert + (int64_t)min(c0 + i * 8 + (lane >> 3), d.hidden - 1) * d.down_stride;
     char* stage = lds + wave * DOWN_TILES * 2048;
     for (int from = 0;;) {
         const int members = min(count - from, 16 * RB);
@@ -314,32 +360,161 @@ __global__ void __launch_bounds__(64 * DOWN_WAVES) experts16_down_kernel(Experts
             else down_pass<TYPE, 4>(d, w, m, members, c0, stage);
         }
         if ((from += 16 * RB) >= count) break;
+        __syncthreads();                                              // (the waves are done with the last pass's members)
         int first;
         find_members(d, e, from, 16 * RB, m, first);
     }
 }
 
 // ---- the rows' sums -----------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) experts16_combine_kernel(Experts16Job d) {
-    const int quads = d.hidden_pad / 4;
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= (int64_t)d.rows * quads) return;
-    const int row = (int)(t / quads), col = (int)(t % quads) * 4, count = min(4, d.hidden - col);
-    f4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < d.slots; ++s) {
-        const int pair = row * d.slots + s, e = d.picks[pair];
-        if (e < 0 || e >= d.experts) continue;
-        const f4_t y = *reinterpret_cast<const f4_t*>(d.y + (int64_t)pair * d.hidden_pad + col);
-        const float weight = d.weights[pair];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = fmaf(weight, y[j], v[j]);
-    }
+// Up to four columns of a row with their residual.
+__device__ __forceinline__ void finish(const Experts16Job& d, int row, int col, f4_t v) {
+    const int count = min(4, d.hidden - col);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (j < count) {
             if (d.residual) v[j] += load_one(d.residual, d.residual_type, (int64_t)row * d.residual_stride + col + j);
             store_one(d.out, d.out_type, (int64_t)row * d.out_stride + col + j, v[j]);
         }
+}
+__global__ void __launch_bounds__(256) experts16_combine_kernel(Experts16Job d) {
+    const int quads = d.hidden_pad / 4;
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= (int64_t)d.rows * quads) return;
+    const int row = (int)(t / quads), col = (int)(t % quads) * 4;
+    f4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < d.slots; s0 += 8) {                         // eight slots' loads at once
+        f4_t y[8];
+        float weight[8];
+        bool there[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const int pair = row * d.slots + min(s0 + s, d.slots - 1), e = d.picks[pair];
+            there[s] = s0 + s < d.slots && e >= 0 && e < d.experts;
+            weight[s] = d.weights[pair];
+            y[s] = *reinterpret_cast<const f4_t*>(d.y + (int64_t)pair * d.hidden_pad + col);
+        }
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = there[s] ? fmaf(weight[s], y[s][j], v[j]) : v[j];
+    }
+    finish(d, row, col, v);
+}
+
+// ---- down and the rows' sums at once, for few pairs ---------------------------------------------------------------
+// A workgroup takes 16 columns of all pairs (at most 64, inter at least 8): its waves share the picked experts' chunks of k in turn, a chunk's
+// sums of its members go to LDS, and are added there in the order of the other form: chunks, then slots.
+constexpr int FEW_WAVES = 8, FEW_PAIRS = 64, FEW_LDS = 65536;
+
+template <int TYPE>
+__global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Experts16Job d) {
+    extern __shared__ __align__(1024) char lds[];
+    __shared__ float weight[FEW_PAIRS];                               // of the pairs, and whether an expert is theirs
+    __shared__ bool there[FEW_PAIRS];
+    constexpr int U = 3;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a = lane & 15, q = lane >> 4;
+    const int c0 = blockIdx.x * 16, pairs = d.rows * d.slots, chunks = d.inter_pad / 64;
+    f4_t* parts = reinterpret_cast<f4_t*>(lds + FEW_WAVES * 2048);    // [pairs][chunks][4]
+    f4_t* sums = parts + pairs * chunks * 4;                          // [pairs][4]
+    char* stage = lds + wave * 2048;
+
+    // the picked experts, one a lane, with the pairs that picked them
+    const int pick = lane < pairs ? d.picks[lane] : -1;
+    if (threadIdx.x < pairs) weight[threadIdx.x] = d.weights[threadIdx.x], there[threadIdx.x] = pick >= 0 && pick < d.experts;
+    int expert = 0, count = 0;
+    uint32_t pairs_lo = 0, pairs_hi = 0;
+    for (int i = 0; i < pairs; ++i) {
+        const int e = __builtin_amdgcn_readlane(pick, i);
+        const uint64_t same = __ballot(pick == e && lane < pairs);
+        if (e < 0 || e >= d.experts || __builtin_ctzll(same) != i) continue;
+        if (lane == count) expert = e, pairs_lo = (uint32_t)same, pairs_hi = (uint32_t)(same >> 32);
+        ++count;
+    }
+    const int units = count * chunks;
+    const int64_t row0 = min(c0 + (lane >> 3), d.hidden - 1), row1 = min(c0 + 8 + (lane >> 3), d.hidden - 1);
+    struct Unit {
+        typename Weights<TYPE, 1>::Chunk w;
+        uint4 x[2][2];
+        int pair;                                                     // this lane's member; negative: none
+        int c;
+        int64_t at;                                                   // the expert's weights
+        uint64_t others;                                              // the members after the first 16
+    };
+    // the n-th pair of a set, n = this lane's a; negative: there are fewer
+    auto nth = [&](uint64_t set) {
+        if (!(set & (set - 1))) return a == 0 ? (int)__builtin_ctzll(set) : -1;
+        const int rank = __popcll(set & ((1ull << lane) - 1));
+        const bool in = set >> lane & 1;
+        const int list = __builtin_amdgcn_ds_permute((in && rank < 16 ? rank : 63) * 4, lane);
+        const int mine = __builtin_amdgcn_ds_bpermute(a * 4, list);
+        return a < __popcll(set) ? mine : -1;
+    };
+    auto load_rows = [&](uint4 (&x)[2][2], uint64_t set, int c) {     // this lane's member, or a negative number
+        const int pair = nth(set);
+        const uint16_t* xp = d.acts + (int64_t)(pair < 0 ? (int)__builtin_ctzll(set) : pair) * 2 * d.inter_pad + 8 * q + c * 64;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            x[s][0] = *reinterpret_cast<const uint4*>(xp + 32 * s);
+            x[s][1] = *reinterpret_cast<const uint4*>(xp + d.inter_pad + 32 * s);
+        }
+        return pair;
+    };
+    auto weights = [&](const Unit& f) {
+        return Weights<TYPE, 1>{{d.down + f.at + row0 * d.down_stride, d.down + f.at + row1 * d.down_stride}};
+    };
+    auto load = [&](Unit& f, int i) {
+        const int unit = wave + i * FEW_WAVES, n = unit / chunks;
+        f.c = unit - n * chunks;
+        f.at = (int64_t)__builtin_amdgcn_readlane(expert, n) * d.down_expert;
+        uint64_t set = (uint32_t)__builtin_amdgcn_readlane((int)pairs_lo, n) |
+                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)pairs_hi, n) << 32;
+        weights(f).ask(f.w, f.c * 64, d.inter);
+        f.pair = load_rows(f.x, set, f.c);
+        for (int i = 0; i < 16 && set; ++i) set &= set - 1;
+        f.others = set;
+    };
+    auto multiply = [&](Unit& f) {
+        const Weights<TYPE, 1> w = weights(f);
+        if (f.c * 64 + 64 > d.inter) w.settle(f.w, f.c * 64, d.inter);
+        w.stage(f.w, stage);
+        const uint4 w0 = w.fragment(stage, 0, 0), w1 = w.fragment(stage, 0, 1);
+        const f4_t v = chunk_sum<TYPE>(w0, w1, f.x);
+        if (f.pair >= 0) parts[(f.pair * chunks + f.c) * 4 + q] = v;
+        // (rows that pick an expert twice, or more than 16 rows; in registers of their own, that no wait of the others' differs)
+        for (uint64_t set = f.others; set;) {
+            uint4 x[2][2];
+            const int pair = load_rows(x, set, f.c);
+            const f4_t more = chunk_sum<TYPE>(w0, w1, x);
+            if (pair >= 0) parts[(pair * chunks + f.c) * 4 + q] = more;
+            for (int i = 0; i < 16 && set; ++i) set &= set - 1;
+        }
+    };
+    Unit f[U];
+    pipeline(f, (units - wave + FEW_WAVES - 1) / FEW_WAVES, load, multiply);
+    __syncthreads();
+    for (int t = threadIdx.x; t < pairs * 4; t += 64 * FEW_WAVES) {
+        f4_t v = {0.f, 0.f, 0.f, 0.f};
+        if (there[t >> 2])
+            for (int c = 0; c < chunks; ++c) v += parts[((t >> 2) * chunks + c) * 4 + (t & 3)];
+        sums[t] = v;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < d.rows * 4; t += 64 * FEW_WAVES) {
+        const int row = t >> 2, col = c0 + (t & 3) * 4;
+        if (col >= d.hidden) continue;
+        f4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < d.slots; ++s) {
+            const int pair = row * d.slots + s;
+            const f4_t y = sums[pair * 4 + (t & 3)];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = there[pair] ? fmaf(weight[pair], y[j], v[j]) : v[j];
+        }
+        finish(d, row, col, v);
+    }
+}
+size_t few_lds(const Experts16Job& d) {
+    return FEW_WAVES * 2048 + (size_t)d.rows * d.slots * (d.inter_pad / 64 + 1) * 64;
 }
 
 template <int TYPE, int RB>
@@ -348,6 +523,10 @@ hipError_t launch(hipStream_t s, const Experts16Job& d) {
     experts16_up_kernel<TYPE, RB><<<dim3((unsigned)(leaders * (d.inter_pad / UP_COLS))), 64 * UP_WAVES, 0, s>>>(d);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (d.rows * d.slots <= FEW_PAIRS && few_lds(d) <= FEW_LDS && d.inter >= 8) {
+        experts16_few_kernel<TYPE><<<dim3((unsigned)((d.hidden + 15) / 16)), 64 * FEW_WAVES, few_lds(d), s>>>(d);
+        return hipGetLastError();
+    }
     experts16_down_kernel<TYPE, RB>
         <<<dim3((unsigned)(leaders * ((d.hidden + DOWN_COLS - 1) / DOWN_COLS))), 64 * DOWN_WAVES, 0, s>>>(d);
     if ((e = hipGetLastError()) != hipSuccess) return e;
