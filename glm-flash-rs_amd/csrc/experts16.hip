@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "lanes.hpp"
 #include "launch.hpp"
 #include "mfma16.hpp"
 #include "values.hpp"
@@ -34,9 +35,10 @@ __device__ __forceinline__ int find_members(const Experts16Job& d, int expert, i
     int seen = 0;
     first = pairs;
     if (pairs <= 64) {                                                // each wave by itself, all with the same values
-        const uint64_t ballot = __ballot(lane < pairs && d.picks[lane < pairs ? lane : 0] == expert);
-        const int at = __popcll(ballot & ((1ull << lane) - 1)) - from;
-        if ((ballot >> lane & 1) && at >= 0 && at < room) m.pair[at] = lane;
+        const bool mine = lane < pairs && d.picks[lane] == expert;
+        const uint64_t ballot = __ballot(mine);
+        const int at = set_before(ballot) - from;
+        if (mine && at >= 0 && at < room) m.pair[at] = lane;
         if (ballot) first = __builtin_ctzll(ballot);
         __builtin_amdgcn_wave_barrier();
         return __popcll(ballot);
@@ -48,7 +50,7 @@ __device__ __forceinline__ int find_members(const Experts16Job& d, int expert, i
         __syncthreads();
         if (lane == 0) m.waves[wave] = __popcll(ballot);
         __syncthreads();
-        int before = seen + __popcll(ballot & ((1ull << lane) - 1));
+        int before = seen + set_before(ballot);
         for (int w = 0; w < waves; ++w) {
             if (w < wave) before += m.waves[w];
             seen += m.waves[w];
@@ -79,12 +81,7 @@ struct Weights {
     struct Chunk {
         uint4 w[2 * EB];
     };
-    __device__ __forceinline__ void load(Chunk& f, int k) const {     // a whole chunk
-        k += (threadIdx.x & 7) * 8;
-#pragma unroll
-        for (int i = 0; i < 2 * EB; ++i) __builtin_memcpy(&f.w[i], row[i] + k, 16);
-    }
-    // any chunk of rows of at least eight, to be put in place where K ends in it
+    // columns k .. + 63 of rows of K, at least eight: to be settled where K ends among them
     __device__ __forceinline__ void ask(Chunk& f, int k, int K) const {
         k += (threadIdx.x & 7) * 8;
 #pragma unroll
@@ -95,13 +92,10 @@ struct Weights {
 #pragma unroll
         for (int i = 0; i < 2 * EB; ++i) f.w[i] = gfr::settle(f.w[i], k, K);
     }
-    // the one that K ends in, in place
-    __device__ __forceinline__ void load_last(Chunk& f, int k, int K) const {
-        k += (threadIdx.x & 7) * 8;
+    // rows of less than eight
+    __device__ __forceinline__ void load_short(Chunk& f, int K) const {
 #pragma unroll
-        for (int i = 0; i < 2 * EB; ++i) f.w[i] = ask_any(row[i], k, K);
-#pragma unroll
-        for (int i = 0; i < 2 * EB; ++i) f.w[i] = settle_any(f.w[i], row[i], k, K);
+        for (int i = 0; i < 2 * EB; ++i) f.w[i] = gfr::load_short(row[i], (threadIdx.x & 7) * 8, K);
     }
     __device__ __forceinline__ void stage(const Chunk& f, char* stage) const {
         const int lane = threadIdx.x & 63;
@@ -129,21 +123,21 @@ __device__ __forceinline__ void pipeline(Chunk (&f)[U], int n, Load load, Use us
     for (int i = 0; i < n; i += U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (i + u < n) use(f[u]);
+            if (i + u < n) use(f[u], i + u);
             load(f[u], min(i + u + U, n - 1));
         }
     }
 }
 
 // ---- gate and up --------------------------------------------------------------------------------------------------
-constexpr int UP_WAVES = 8, UP_TILES = 2, UP_COLS = 8 * UP_TILES;
+constexpr int UP_WAVES = 8;
 
-// One pass: members [from, from + 16 RB) of the expert, columns c0 .. + UP_COLS. A tile of 16 weight rows is 8 gate rows
+// One pass: members [from, from + 16 RB) of the expert, columns c0 .. + 8 EB. A tile of 16 weight rows is 8 gate rows
 // and the 8 up rows of the same columns; the waves share k by chunks of 64, and their sums are added in order.
-template <int TYPE, int RB>
-__device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYPE, UP_TILES>& w, const Members& m, int members,
+template <int TYPE, int EB, int RB>
+__device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYPE, EB>& w, const Members& m, int members,
                                         int c0, char* lds) {
-    constexpr int EB = UP_TILES, U = 2;
+    constexpr int U = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a = lane & 15, q = lane >> 4;
     const uint16_t* xp[RB];
 #pragma unroll
@@ -160,18 +154,17 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
     for (int i = 0; i < EB; ++i)
 #pragma unroll
         for (int j = 0; j < RB; ++j) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
-    const int chunks = d.hidden / 64;                                 // whole ones
-    const bool last = d.hidden % 64 && wave == chunks % UP_WAVES;     // this wave has the one that hidden ends in
+    const int K = d.hidden, chunks = (K + 63) / 64;
     auto load = [&](Chunk& f, int i) {
-        const int c = wave + i * UP_WAVES;
-        w.load(f.w, c * 64);
+        const int k = (wave + i * UP_WAVES) * 64;
+        w.ask(f.w, k, K);
 #pragma unroll
         for (int j = 0; j < RB; ++j)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) __builtin_memcpy(&f.x[j][s], xp[j] + c * 64 + 32 * s + 8 * q, 16);
+            for (int s = 0; s < 2; ++s) f.x[j][s] = ask(xp[j], k + 32 * s + 8 * q, K);
     };
     char* stage = lds + wave * EB * 2048;
-    auto multiply = [&](const Chunk& f) {
+    auto product = [&](const Chunk& f) {
         w.stage(f.w, stage);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -182,20 +175,27 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
                 for (int j = 0; j < RB; ++j) acc[i][j] = mfma<TYPE>(fw, f.x[j][s], acc[i][j]);
             }
     };
+    auto multiply = [&](Chunk& f, int i) {
+        const int k = (wave + i * UP_WAVES) * 64;
+        if (k + 64 > K) {
+            w.settle(f.w, k, K);
+#pragma unroll
+            for (int j = 0; j < RB; ++j)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) f.x[j][s] = settle(f.x[j][s], k + 32 * s + 8 * q, K);
+        }
+        product(f);
+    };
     Chunk f[U];
-    pipeline(f, (chunks - wave + UP_WAVES - 1) / UP_WAVES, load, multiply);
-    if (last) {
-        const int k = chunks * 64, K = d.hidden;
+    if (K >= 8) {
+        pipeline(f, (chunks - wave + UP_WAVES - 1) / UP_WAVES, load, multiply);
+    } else if (wave == 0) {
+        w.load_short(f[0].w, K);
 #pragma unroll
         for (int j = 0; j < RB; ++j)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) f[0].x[j][s] = ask_any(xp[j], k + 32 * s + 8 * q, K);
-        w.load_last(f[0].w, k, K);
-#pragma unroll
-        for (int j = 0; j < RB; ++j)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) f[0].x[j][s] = settle_any(f[0].x[j][s], xp[j], k + 32 * s + 8 * q, K);
-        multiply(f[0]);
+            for (int s = 0; s < 2; ++s) f[0].x[j][s] = load_short(xp[j], 32 * s + 8 * q, K);
+        product(f[0]);
     }
     __syncthreads();
     f4_t* part = reinterpret_cast<f4_t*>(lds);                        // [UP_WAVES][EB * RB][64]
@@ -233,29 +233,29 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
     __syncthreads();
 }
 
-template <int TYPE, int RB>
+template <int TYPE, int EB, int RB>
 __global__ void __launch_bounds__(64 * UP_WAVES, RB == 1 ? 4 : 2) experts16_up_kernel(Experts16Job d) {
-    __shared__ __align__(1024) char lds[UP_WAVES * UP_TILES * (RB > 2 ? RB * 1024 : 2048)];
+    __shared__ __align__(1024) char lds[UP_WAVES * EB * (RB > 2 ? RB * 1024 : 2048)];
     __shared__ Members m;
-    const int lane = threadIdx.x & 63, tiles = d.inter_pad / UP_COLS;
-    const int u = blockIdx.x / tiles, c0 = (blockIdx.x % tiles) * UP_COLS;
+    const int lane = threadIdx.x & 63, tiles = d.inter_pad / (8 * EB);
+    const int u = blockIdx.x / tiles, c0 = (blockIdx.x % tiles) * 8 * EB;
     int count;
     const int e = expert_of(d, u, 16 * RB, m, count);
     if (e < 0) return;
-    Weights<TYPE, UP_TILES> w;
+    Weights<TYPE, EB> w;
 #pragma unroll
-    for (int i = 0; i < 2 * UP_TILES; ++i) {
+    for (int i = 0; i < 2 * EB; ++i) {
         const int row = min(c0 + (i >> 1) * 8 + (lane >> 3), d.inter - 1) + (i & 1) * d.inter;
         w.row[i] = d.gu + (int64_t)e * d.gu_expert + (int64_t)row * d.gu_stride;
     }
     for (int from = 0;;) {
         const int members = min(count - from, 16 * RB);
         if constexpr (RB == 1) {
-            up_pass<TYPE, 1>(d, w, m, members, c0, lds);
+            up_pass<TYPE, EB, 1>(d, w, m, members, c0, lds);
         } else {
-            if (members <= 16) up_pass<TYPE, 1>(d, w, m, members, c0, lds);
-            else if (members <= 32) up_pass<TYPE, 2>(d, w, m, members, c0, lds);
-            else up_pass<TYPE, 4>(d, w, m, members, c0, lds);
+            if (members <= 16) up_pass<TYPE, EB, 1>(d, w, m, members, c0, lds);
+            else if (members <= 32) up_pass<TYPE, EB, 2>(d, w, m, members, c0, lds);
+            else up_pass<TYPE, EB, 4>(d, w, m, members, c0, lds);
         }
         if ((from += 16 * RB) >= count) break;
         int first;
@@ -294,7 +294,7 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
     for (int i = 0; i < EB; ++i)
 #pragma unroll
         for (int j = 0; j < RB; ++j) acc[i][j] = (f4_t){0.f, 0.f, 0.f, 0.f};
-    const int chunks = d.inter / 64;                                  // whole ones
+    const int K = d.inter, chunks = d.inter_pad / 64;
     auto load_rows = [&](Chunk& f, int c) {
 #pragma unroll
         for (int j = 0; j < RB; ++j)
@@ -305,10 +305,10 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
             }
     };
     auto load = [&](Chunk& f, int c) {
-        w.load(f.w, c * 64);
+        w.ask(f.w, c * 64, K);
         load_rows(f, c);
     };
-    auto multiply = [&](const Chunk& f) {
+    auto product = [&](const Chunk& f) {
         w.stage(f.w, stage);
 #pragma unroll
         for (int i = 0; i < EB; ++i) {
@@ -317,12 +317,17 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
             for (int j = 0; j < RB; ++j) acc[i][j] += chunk_sum<TYPE>(w0, w1, f.x[j]);
         }
     };
+    auto multiply = [&](Chunk& f, int c) {
+        if (c * 64 + 64 > K) w.settle(f.w, c * 64, K);
+        product(f);
+    };
     Chunk f[U];
-    pipeline(f, chunks, load, multiply);
-    if (d.inter % 64) {
-        load_rows(f[0], chunks);
-        w.load_last(f[0].w, chunks * 64, d.inter);
-        multiply(f[0]);
+    if (K >= 8) {
+        pipeline(f, chunks, load, multiply);
+    } else {
+        w.load_short(f[0].w, K);
+        load_rows(f[0], 0);
+        product(f[0]);
     }
 #pragma unroll
     for (int j = 0; j < RB; ++j) {
@@ -337,7 +342,7 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
 }
 
 template <int TYPE, int RB>
-__global__ void __launch_bounds__(64 * DOWN_WAVES, RB == 1 ? 4 : 2) experts16_down_kernel(Experts16Job d) {
+__global__ void __launch_bounds__(64 * DOWN_WAVES, RB == 1 ? 3 : 2) experts16_down_kernel(Experts16Job d) {
     __shared__ __align__(1024) char lds[DOWN_WAVES * DOWN_TILES * 2048];
     __shared__ Members m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tiles = (d.hidden + DOWN_COLS - 1) / DOWN_COLS;
@@ -368,20 +373,25 @@ __global__ void __launch_bounds__(64 * DOWN_WAVES, RB == 1 ? 4 : 2) experts16_do
 
 // ---- the rows' sums -----------------------------------------------------------------------------------------------
 // Up to four columns of a row with their residual.
-__device__ __forceinline__ void finish(const Experts16Job& d, int row, int col, f4_t v) {
-    const int count = min(4, d.hidden - col);
+__device__ __forceinline__ f4_t residual_at(const Experts16Job& d, int row, int col) {
+    f4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (j < count) {
-            if (d.residual) v[j] += load_one(d.residual, d.residual_type, (int64_t)row * d.residual_stride + col + j);
-            store_one(d.out, d.out_type, (int64_t)row * d.out_stride + col + j, v[j]);
-        }
+        if (d.residual && col + j < d.hidden) v[j] = load_one(d.residual, d.residual_type, (int64_t)row * d.residual_stride + col + j);
+    return v;
+}
+__device__ __forceinline__ void finish(const Experts16Job& d, int row, int col, f4_t v, f4_t residual) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (col + j < d.hidden)
+            store_one(d.out, d.out_type, (int64_t)row * d.out_stride + col + j, d.residual ? v[j] + residual[j] : v[j]);
 }
 __global__ void __launch_bounds__(256) experts16_combine_kernel(Experts16Job d) {
     const int quads = d.hidden_pad / 4;
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= (int64_t)d.rows * quads) return;
     const int row = (int)(t / quads), col = (int)(t % quads) * 4;
+    const f4_t residual = residual_at(d, row, col);
     f4_t v = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < d.slots; s0 += 8) {                         // eight slots' loads at once
         f4_t y[8];
@@ -399,7 +409,7 @@ __global__ void __launch_bounds__(256) experts16_combine_kernel(Experts16Job d) 
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = there[s] ? fmaf(weight[s], y[s][j], v[j]) : v[j];
     }
-    finish(d, row, col, v);
+    finish(d, row, col, v, residual);
 }
 
 // ---- down and the rows' sums at once, for few pairs ---------------------------------------------------------------
@@ -431,21 +441,22 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Expert
         if (lane == count) expert = e, pairs_lo = (uint32_t)same, pairs_hi = (uint32_t)(same >> 32);
         ++count;
     }
-    const int units = count * chunks;
+    const int units = count * chunks, my_row = threadIdx.x >> 2, my_col = c0 + (threadIdx.x & 3) * 4;
+    f4_t residual = {0.f, 0.f, 0.f, 0.f};
+    if (my_row < d.rows) residual = residual_at(d, my_row, my_col);
     const int64_t row0 = min(c0 + (lane >> 3), d.hidden - 1), row1 = min(c0 + 8 + (lane >> 3), d.hidden - 1);
     struct Unit {
         typename Weights<TYPE, 1>::Chunk w;
         uint4 x[2][2];
         int pair;                                                     // this lane's member; negative: none
         int c;
-        int64_t at;                                                   // the expert's weights
         uint64_t others;                                              // the members after the first 16
     };
     // the n-th pair of a set, n = this lane's a; negative: there are fewer
     auto nth = [&](uint64_t set) {
         if (!(set & (set - 1))) return a == 0 ? (int)__builtin_ctzll(set) : -1;
-        const int rank = __popcll(set & ((1ull << lane) - 1));
-        const bool in = set >> lane & 1;
+        const int rank = set_before(set);
+        const bool in = (lane & 32 ? (uint32_t)(set >> 32) : (uint32_t)set) >> (lane & 31) & 1;
         const int list = __builtin_amdgcn_ds_permute((in && rank < 16 ? rank : 63) * 4, lane);
         const int mine = __builtin_amdgcn_ds_bpermute(a * 4, list);
         return a < __popcll(set) ? mine : -1;
@@ -460,22 +471,30 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Expert
         }
         return pair;
     };
-    auto weights = [&](const Unit& f) {
-        return Weights<TYPE, 1>{{d.down + f.at + row0 * d.down_stride, d.down + f.at + row1 * d.down_stride}};
+    // this wave's place among the units: expert n's chunk c, its weights and pairs; units are asked for in turn
+    int n = -1, c = chunks;
+    uint64_t set = 0;
+    Weights<TYPE, 1> w;
+    const auto move = [&](int by) {
+        for (c += by; c >= chunks; c -= chunks, ++n) {
+        }
+        const uint16_t* at = d.down + (int64_t)__builtin_amdgcn_readlane(expert, n) * d.down_expert;
+        set = (uint32_t)__builtin_amdgcn_readlane((int)pairs_lo, n) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)pairs_hi, n) << 32;
+        w = {{at + row0 * d.down_stride, at + row1 * d.down_stride}};
     };
+    const int mine = (units - wave + FEW_WAVES - 1) / FEW_WAVES;
+    int asked = 0;
     auto load = [&](Unit& f, int i) {
-        const int unit = wave + i * FEW_WAVES, n = unit / chunks;
-        f.c = unit - n * chunks;
-        f.at = (int64_t)__builtin_amdgcn_readlane(expert, n) * d.down_expert;
-        uint64_t set = (uint32_t)__builtin_amdgcn_readlane((int)pairs_lo, n) |
-                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)pairs_hi, n) << 32;
-        weights(f).ask(f.w, f.c * 64, d.inter);
-        f.pair = load_rows(f.x, set, f.c);
-        for (int i = 0; i < 16 && set; ++i) set &= set - 1;
+        if (i >= asked) move(asked++ ? FEW_WAVES : wave);             // (past the end: the last one again)
+        f.c = c;
+        w.ask(f.w, c * 64, d.inter);
+        f.pair = load_rows(f.x, set, c);
         f.others = set;
+        if (__popcll(set) <= 16) f.others = 0;
+        else
+            for (int i = 0; i < 16; ++i) f.others &= f.others - 1;
     };
-    auto multiply = [&](Unit& f) {
-        const Weights<TYPE, 1> w = weights(f);
+    auto multiply = [&](Unit& f, int) {
         if (f.c * 64 + 64 > d.inter) w.settle(f.w, f.c * 64, d.inter);
         w.stage(f.w, stage);
         const uint4 w0 = w.fragment(stage, 0, 0), w1 = w.fragment(stage, 0, 1);
@@ -491,7 +510,7 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Expert
         }
     };
     Unit f[U];
-    pipeline(f, (units - wave + FEW_WAVES - 1) / FEW_WAVES, load, multiply);
+    pipeline(f, mine, load, multiply);
     __syncthreads();
     for (int t = threadIdx.x; t < pairs * 4; t += 64 * FEW_WAVES) {
         f4_t v = {0.f, 0.f, 0.f, 0.f};
@@ -500,30 +519,38 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Expert
         sums[t] = v;
     }
     __syncthreads();
-    for (int t = threadIdx.x; t < d.rows * 4; t += 64 * FEW_WAVES) {
-        const int row = t >> 2, col = c0 + (t & 3) * 4;
-        if (col >= d.hidden) continue;
+    if (my_row < d.rows) {                                            // (at most 64 rows: every output has a thread)
         f4_t v = {0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < d.slots; ++s) {
-            const int pair = row * d.slots + s;
-            const f4_t y = sums[pair * 4 + (t & 3)];
+            const int pair = my_row * d.slots + s;
+            const f4_t y = sums[pair * 4 + (threadIdx.x & 3)];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = there[pair] ? fmaf(weight[pair], y[j], v[j]) : v[j];
         }
-        finish(d, row, col, v);
+        finish(d, my_row, my_col, v, residual);
     }
 }
+static_assert(FEW_PAIRS * 4 <= 64 * FEW_WAVES, "a thread an output");
 size_t few_lds(const Experts16Job& d) {
     return FEW_WAVES * 2048 + (size_t)d.rows * d.slots * (d.inter_pad / 64 + 1) * 64;
 }
 
+template <int TYPE, int EB, int RB>
+hipError_t launch_up(hipStream_t s, const Experts16Job& d, int64_t leaders) {
+    experts16_up_kernel<TYPE, EB, RB><<<dim3((unsigned)(leaders * (d.inter_pad / (8 * EB)))), 64 * UP_WAVES, 0, s>>>(d);
+    return hipGetLastError();
+}
 template <int TYPE, int RB>
 hipError_t launch(hipStream_t s, const Experts16Job& d) {
-    const int64_t leaders = (int64_t)d.rows * d.slots < d.experts ? (int64_t)d.rows * d.slots : d.experts;
-    experts16_up_kernel<TYPE, RB><<<dim3((unsigned)(leaders * (d.inter_pad / UP_COLS))), 64 * UP_WAVES, 0, s>>>(d);
-    hipError_t e = hipGetLastError();
+    const int64_t pairs = (int64_t)d.rows * d.slots, leaders = pairs < d.experts ? pairs : d.experts;
+    const bool few = pairs <= FEW_PAIRS && few_lds(d) <= FEW_LDS && d.inter >= 8;
+    hipError_t e;
+    if constexpr (RB == 1)
+        e = leaders * (d.inter_pad / 16) < 512 ? launch_up<TYPE, 1, 1>(s, d, leaders) : launch_up<TYPE, 2, 1>(s, d, leaders);
+    else
+        e = launch_up<TYPE, 2, RB>(s, d, leaders);
     if (e != hipSuccess) return e;
-    if (d.rows * d.slots <= FEW_PAIRS && few_lds(d) <= FEW_LDS && d.inter >= 8) {
+    if (few) {
         experts16_few_kernel<TYPE><<<dim3((unsigned)((d.hidden + 15) / 16)), 64 * FEW_WAVES, few_lds(d), s>>>(d);
         return hipGetLastError();
     }

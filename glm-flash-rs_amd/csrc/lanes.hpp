@@ -55,4 +55,9 @@ __device__ __forceinline__ T sum_over(int width, T v) {
     return v;
 }
 
+// How many lanes before this one have their bit set in a ballot.
+__device__ __forceinline__ int set_before(uint64_t ballot) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0));
+}
+
 }  // namespace gfr

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(LogprobsJob d) {
     // fewer logits than places are not masked: the masked tokens in order, enough of which are among the first 64
     if (i < d.top) {
         const bool masked = lane < d.vocab && !(load_one(d.logits, d.type, base + lane) > -INFINITY);
-        const int place = i + __popcll(__ballot(masked) & ((1ull << lane) - 1));
+        const int place = i + set_before(__ballot(masked));
         if (masked && place < d.top) ids[place] = lane, logps[place] = -INFINITY;
     }
 }

@@ -33,31 +33,32 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int k, int K) {
     return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
 }
 
-// The same in two steps, for loads that are used later: ask() loads the row's eight values from column k on, or its last
-// eight, settle() puts them in place. Only columns from K - 7 on need settle(); K is at least 8 (ask), or anything
-// (ask_any, settle_any).
+// The same in two steps, for loads that are used later, of rows of at least eight values: ask() loads the row's eight values
+// from column k on, or its last eight, settle() puts them in place where they are not (columns from K - 7 on).
 __device__ __forceinline__ uint4 ask(const uint16_t* row, int k, int K) {
     uint4 v;
     __builtin_memcpy(&v, row + min(k, K - 8), 16);
     return v;
 }
+// In 32-bit operations: a 64-bit shift that had its amount in the last register of the wave's allocation gave wrong values now
+// and then (the compiler may put it there).
 __device__ __forceinline__ uint4 settle(uint4 v, int k, int K) {
-    uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
-    const int bits = 16 * (k - min(k, K - 8));
-    if (bits >= 64) lo = hi, hi = 0;
-    if (bits >= 128) lo = 0;
-    if (bits & 63) lo = lo >> (bits & 63) | hi << (64 - (bits & 63)), hi >>= bits & 63;
-    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    const int n = k - min(k, K - 8);                                  // places to move down
+    if (n & 4) v.x = v.z, v.y = v.w, v.z = v.w = 0;
+    if (n & 2) v.x = v.y, v.y = v.z, v.z = v.w, v.w = 0;
+    if (n & 1)
+        v = make_uint4(__builtin_amdgcn_alignbit(v.y, v.x, 16), __builtin_amdgcn_alignbit(v.z, v.y, 16),
+                       __builtin_amdgcn_alignbit(v.w, v.z, 16), v.w >> 16);
+    return n < 8 ? v : make_uint4(0, 0, 0, 0);
 }
-__device__ __forceinline__ uint4 ask_any(const uint16_t* row, int k, int K) {
-    return K >= 8 ? ask(row, k, K) : make_uint4(0, 0, 0, 0);
-}
-__device__ __forceinline__ uint4 settle_any(uint4 v, const uint16_t* row, int k, int K) {
-    if (K >= 8) return settle(v, k, K);
-    uint64_t lo = 0, hi = 0;
+// Rows of less than eight, a value at a time.
+__device__ __forceinline__ uint4 load_short(const uint16_t* row, int k, int K) {
+    uint4 v = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
-    for (int j = K - 1; j >= k; --j) hi = hi << 16 | lo >> 48, lo = lo << 16 | row[j];
-    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    for (int j = K - 1; j >= k; --j)
+        v = make_uint4(v.x << 16 | row[j], __builtin_amdgcn_alignbit(v.y, v.x, 16), __builtin_amdgcn_alignbit(v.z, v.y, 16),
+                       __builtin_amdgcn_alignbit(v.w, v.z, 16));
+    return v;
 }
 
 }  // namespace gfr

@@ -253,3 +253,17 @@ def test_python_refusals(gfr):
                         (dict(out_dtype=torch.float16), "x's type or fp32")):
         with pytest.raises(gfr.GfrError, match=needle):
             gfr.experts16(**{**good, **bad})
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("hidden,inter", [(600, 1032), (1001, 333), (4096, 512), (2047, 1025)])
+def test_again(gfr, hidden, inter, dtype):
+    """The same bits from the same call, with the weights in the caches after the first."""
+    E, slots, dt = 40, 9, TYPES[dtype]
+    ex = stack(gfr, 2, E, hidden, inter, dt)
+    for rows in (1, 5, 40):
+        x, (picks, weights) = randn(rows, rows, hidden, dtype=dt), routing(3, rows, slots, E)
+        y = gfr.experts16(x, ex, picks, weights, out_dtype=torch.float32)
+        check(y, reference(x, ex, picks, weights), f"rows {rows}")
+        for _ in range(8):
+            assert torch.equal(gfr.experts16(x, ex, picks, weights, out_dtype=torch.float32), y)
