@@ -652,7 +652,7 @@ int norm_job(const gfr_block_norm* d, gfr::NormJob& job) {
         }
     job = {d->x, d->residual, d->gate, d->h, d->y, d->x_stride, d->residual_stride, d->gate_row, d->h_stride, d->y_stride,
            d->rows, d->n, d->x_type, d->residual_type, d->gate_type, d->h_type, d->y_type, d->gate_column, d->sigmoid != 0,
-           d->post.kind != GFR_NORM_NONE, d->scale, d->residual_scale, post, pre, 0.f};
+           d->post.kind != GFR_NORM_NONE, d->scale, d->residual_scale, post, pre, 0.f, 0};
     return 0;
 }
 }  // namespace

@@ -214,7 +214,9 @@ struct NormJob {
     bool sigmoid, has_post;
     float scale, residual_scale;
     NormPart post, pre;
-    float per_column;               // set by launch_norm: 1 / n
+    // set by launch_norm: 1 / n, the first row of a launch
+    float per_column;
+    int64_t first;
 };
 hipError_t launch_norm(hipStream_t s, NormJob d);
 

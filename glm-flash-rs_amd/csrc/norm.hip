@@ -27,13 +27,39 @@ __device__ __forceinline__ float total(float v, float* part) {
     return v;
 }
 
+// An operand's values where it is either fp32 or of the 16-bit type T (ANY: of any). The branches stay branches: the
+// compiler would convert both ways and select, for every operand.
+constexpr int ANY = -1;
+template <int T>
+__device__ __forceinline__ f8_t converted(const Eight& e, int type) {
+    if constexpr (T == ANY) return values(e, type);
+    f8_t v;
+    if (type == TYPE_F32) {
+        asm volatile("; fp32");
+        v = values(e, TYPE_F32);
+    } else {
+        asm volatile("; 16 bits");
+        v = values(e, T);
+    }
+    return v;
+}
+template <int T>
+__device__ __forceinline__ void store(void* p, int type, int64_t i, f8_t v, int count) {
+    if (T == ANY || type == TYPE_F32) store_some(p, T == ANY ? type : TYPE_F32, i, v, count);
+    else store_some(p, T, i, v, count);
+}
+
 // V groups of eight columns a lane: group g of lane i starts at column 8 (g lanes + i).
-template <int L, int V>
+template <int T, int L, int V>
 __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
+    constexpr bool LATE = V > 2;                                      // operands at their use: registers hold one row
     __shared__ float part[2][16];
     const int lanes = L ? L : (int)blockDim.x, lane = L ? threadIdx.x % L : threadIdx.x, per = L ? 256 / L : 1;
+    const bool ragged = d.n % 8;
     int side = 0;
-    for (int64_t row = (int64_t)blockIdx.x * per + (L ? threadIdx.x / L : 0); row < d.rows; row += (int64_t)gridDim.x * per) {
+    const int64_t row = d.first + (int64_t)blockIdx.x * per + (L ? threadIdx.x / L : 0);
+    if (row >= d.rows) return;
+    {
         int c[V], count[V];
         Eight ex[V], er[V], eg[V];
         float gate = 1.f;
@@ -44,21 +70,35 @@ __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
             ex[g].a = ex[g].b = er[g].a = er[g].b = eg[g].a = eg[g].b = make_uint4(0, 0, 0, 0);
             if (count[g] > 0) {
                 ex[g] = load_some(d.x, d.x_type, row * d.x_stride + c[g], count[g]);
-                if (d.residual) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
-                if (d.gate && d.gate_col) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
+                if (!LATE && d.residual) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
+                if (!LATE && d.gate && d.gate_col) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
             }
         }
         f8_t v[V];
 #pragma unroll
-        for (int g = 0; g < V; ++g) v[g] = values(ex[g], d.x_type);
-        // v's columns past n are kept at zero up to a norm's weights
+        for (int g = 0; g < V; ++g) v[g] = converted<T>(ex[g], d.x_type);
+        // columns past n hold zeros; a norm leaves what it adds to them out again
+        const auto clear = [&] {
+#pragma unroll
+            for (int g = 0; g < V; ++g) {
+                if (ragged) {
+                    asm volatile("; by column");
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[g][j] = j < count[g] ? v[g][j] : 0.f;
+                } else {
+                    asm volatile("; by group");
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[g][j] = count[g] > 0 ? v[g][j] : 0.f;
+                }
+            }
+        };
         const auto norm = [&](const NormPart& p) {
             Eight ew[V], eb[V];
 #pragma unroll
             for (int g = 0; g < V; ++g) {
                 ew[g].a = ew[g].b = eb[g].a = eb[g].b = make_uint4(0, 0, 0, 0);
-                if (count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
-                if (count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
+                if (!LATE && count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
+                if (!LATE && count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
             }
             if (p.layer) {
                 float s = 0.f;
@@ -70,72 +110,105 @@ __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
 #pragma unroll
                 for (int g = 0; g < V; ++g)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] = j < count[g] ? v[g][j] - mean : 0.f;
+                    for (int j = 0; j < 8; ++j) v[g][j] -= mean;
+                clear();
             }
             float s = 0.f;
 #pragma unroll
             for (int g = 0; g < V; ++g)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s = fmaf(v[g][j], v[g][j], s);
-            const float r = 1.f / sqrtf(total<L>(s, part[side ^= 1]) * d.per_column + p.eps);
+            const float r = __builtin_amdgcn_rsqf(total<L>(s, part[side ^= 1]) * d.per_column + p.eps);
 #pragma unroll
             for (int g = 0; g < V; ++g) {
-                const f8_t w = values(ew[g], p.weight_type), b = values(eb[g], p.bias_type);
+                if (LATE && count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
+                if (LATE && count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
+                if (p.weight) {
+                    const f8_t w = converted<T>(ew[g], p.weight_type);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[g][j] = p.weight ? v[g][j] * r * (w[j] + p.offset) : v[g][j] * r;
-                if (p.bias) {
+                    for (int j = 0; j < 8; ++j) v[g][j] = v[g][j] * r * (w[j] + p.offset);
+                } else {
+                    asm volatile("; no weight");
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] += j < count[g] ? b[j] : 0.f;
+                    for (int j = 0; j < 8; ++j) v[g][j] *= r;
                 }
+                if (p.bias) v[g] += converted<T>(eb[g], p.bias_type);  // (zeros past n)
             }
         };
         if (d.has_post) norm(d.post);
-        if (d.gate && !d.gate_col && d.sigmoid) gate = times_logistic(1.f, gate);
+        if (d.gate) {
+            if (!d.gate_col && d.sigmoid) gate = times_logistic(1.f, gate);
 #pragma unroll
-        for (int g = 0; g < V; ++g) {
-            if (d.gate && d.gate_col) {
-                const f8_t b = values(eg[g], d.gate_type);
+            for (int g = 0; g < V; ++g) {
+                if (!d.gate_col) {
+                    asm volatile("; a gate a row");
+                    v[g] *= gate;
+                    continue;
+                }
+                if (LATE && count[g] > 0) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
+                f8_t b = converted<T>(eg[g], d.gate_type);
+                if (d.sigmoid) {
+                    asm volatile("; sigmoid");
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[g][j] *= d.sigmoid ? times_logistic(1.f, b[j]) : b[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[g][j] *= gate;
+                    for (int j = 0; j < 8; ++j) b[j] = times_logistic(1.f, b[j]);
+                }
+                v[g] *= b;
             }
+        }
+        if (d.h) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[g][j] *= d.scale;
-            if (d.residual) {
-                const f8_t r = values(er[g], d.residual_type);
+            for (int g = 0; g < V; ++g) {
+                v[g] *= d.scale;
+                if (d.residual) {
+                    if (LATE && count[g] > 0) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
+                    const f8_t r = converted<T>(er[g], d.residual_type);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[g][j] = fmaf(d.residual_scale, r[j], v[g][j]);
+                    for (int j = 0; j < 8; ++j) v[g][j] = fmaf(d.residual_scale, r[j], v[g][j]);
+                }
+                if (count[g] > 0) store<T>(d.h, d.h_type, row * d.h_stride + c[g], v[g], count[g]);
             }
-            if (d.h && count[g] > 0) store_some(d.h, d.h_type, row * d.h_stride + c[g], v[g], count[g]);
         }
         if (d.y) {
             norm(d.pre);
 #pragma unroll
             for (int g = 0; g < V; ++g)
-                if (count[g] > 0) store_some(d.y, d.y_type, row * d.y_stride + c[g], v[g], count[g]);
+                if (count[g] > 0) store<T>(d.y, d.y_type, row * d.y_stride + c[g], v[g], count[g]);
         }
     }
 }
 
-template <int L, int V>
-hipError_t launch(hipStream_t s, const NormJob& d) {
+template <int T, int L, int V>
+hipError_t launch(hipStream_t s, NormJob d) {
     const int lanes = (d.n + 8 * V - 1) / (8 * V), threads = L ? 256 : (lanes + 63) / 64 * 64, per = L ? 256 / L : 1;
-    const int64_t groups = ((int64_t)d.rows + per - 1) / per;
-    norm_kernel<L, V><<<dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20)), threads, 0, s>>>(d);
-    return hipGetLastError();
+    for (; d.first < d.rows; d.first += (int64_t)per << 21) {         // (a launch holds 2^32 threads)
+        const int64_t groups = (d.rows - d.first + per - 1) / per;
+        norm_kernel<T, L, V><<<dim3((unsigned)(groups < 1 << 21 ? groups : 1 << 21)), threads, 0, s>>>(d);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+template <int T>
+hipError_t launch(hipStream_t s, const NormJob& d) {
+    if (d.n <= 128) return launch<T, 16, 1>(s, d);
+    if (d.n <= 512) return launch<T, 64, 1>(s, d);
+    if (d.n <= 8192) return launch<T, 0, 1>(s, d);
+    if (d.n <= 16384) return launch<T, 0, 2>(s, d);
+    return launch<T, 0, 4>(s, d);
 }
 
 }  // namespace
 
 hipError_t launch_norm(hipStream_t s, NormJob d) {
     d.per_column = 1.f / (float)d.n;
-    if (d.n <= 128) return launch<16, 1>(s, d);
-    if (d.n <= 512) return launch<64, 1>(s, d);
-    if (d.n <= 8192) return launch<0, 1>(s, d);
-    if (d.n <= 16384) return launch<0, 2>(s, d);
-    return launch<0, 4>(s, d);
+    // the 16-bit type of the operands that are there, if they share one
+    const void* const at[] = {d.x, d.residual, d.gate, d.h, d.y, d.post.weight, d.post.bias, d.pre.weight, d.pre.bias};
+    const int types[] = {d.x_type, d.residual_type, d.gate_type, d.h_type, d.y_type,
+                         d.post.weight_type, d.post.bias_type, d.pre.weight_type, d.pre.bias_type};
+    bool bf16 = true, fp16 = true;
+    for (int i = 0; i < 9; ++i)
+        if (at[i]) bf16 = bf16 && types[i] != TYPE_F16, fp16 = fp16 && types[i] != TYPE_BF16;
+    return bf16 ? launch<TYPE_BF16>(s, d) : fp16 ? launch<TYPE_F16>(s, d) : launch<ANY>(s, d);
 }
 
 }  // namespace gfr

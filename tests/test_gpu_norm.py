@@ -221,3 +221,13 @@ def test_python_refusals(gfr):
             gfr.block_norm(wide[:, :64] if "pre" not in bad else x, **bad)
     with pytest.raises(gfr.GfrError, match="rows 0"):
         gfr.block_norm(x[:0], pre=p)
+
+
+def test_more_rows_than_a_launch_holds(gfr):
+    """2^21 + 3 rows of a workgroup each: the rows on both sides of the second launch's start."""
+    rows, n = (1 << 21) + 3, 520
+    x = torch.randn((rows, n), dtype=torch.bfloat16, device="cuda")
+    p = made(gfr, 1, n, "rms", torch.bfloat16)
+    y = gfr.norm(x, p)
+    for part in (slice(0, 5), slice(rows - 7, rows)):
+        assert torch.equal(y[part], gfr.norm(x[part].contiguous(), p))
