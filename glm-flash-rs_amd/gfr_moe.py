@@ -409,15 +409,21 @@ class Norm:
         kind, w, b = _NORMS.get(self.kind), self.weight, self.bias
         if kind is None:
             raise ValueError(f"norm kind {self.kind!r} of {list(_NORMS)}")
-        for t in (w, b):
-            if t is None:
-                continue
-            if t.shape != (n,) or t.dtype not in _TYPE or not t.is_contiguous():
-                raise ValueError(f"norm weight or bias {tuple(t.shape)} {t.dtype}: want ({n},) bf16, fp16 or fp32, contiguous")
-            if t.get_device() != here:
-                _elsewhere(t)
-        return (kind, 0 if w is None else _TYPE[w.dtype], 0 if b is None else _TYPE[b.dtype], self.eps, self.offset,
-                0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr())
+        w_type = w_at = b_type = b_at = 0
+        if w is not None:
+            w_type, w_at = self._vector(w, n, here)
+        if b is not None:
+            b_type, b_at = self._vector(b, n, here)
+        return kind, w_type, b_type, self.eps, self.offset, w_at, b_at
+
+    @staticmethod
+    def _vector(t, n, here):
+        kind = _TYPE.get(t.dtype)
+        if kind is None or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"norm weight or bias {tuple(t.shape)} {t.dtype}: want ({n},) bf16, fp16 or fp32, contiguous")
+        if t.get_device() != here:
+            _elsewhere(t)
+        return kind, t.data_ptr()
 
 
 _NO_NORM = (0, 0, 0, 0.0, 0.0, 0, 0)
@@ -1063,14 +1069,16 @@ def dense_gated(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor = None, act
 
 
 def _result(out, shape, dtype, like, stream, here, name="out"):
-    """A new output, or the caller's own after its checks."""
+    """A new output [rows, columns], or the caller's own after its checks, and its row stride."""
     if out is None:
-        return _empty(shape, dtype, like, stream)
+        if stream is None:
+            return like.new_empty(shape, dtype=dtype), shape[1]
+        return _empty(shape, dtype, like, stream), shape[1]
     if out.shape != shape or out.dtype not in _TYPE:
         raise ValueError(f"{name} {tuple(out.shape)} {out.dtype}: want {tuple(shape)} in bf16, fp16 or fp32")
     if out.get_device() != here:
         _elsewhere(out)
-    return out
+    return out, _row_stride(out)
 
 
 def experts16(x: torch.Tensor, experts: Experts16, picks: torch.Tensor, weights: torch.Tensor, activation: str = "silu",
@@ -1116,17 +1124,20 @@ def experts16(x: torch.Tensor, experts: Experts16, picks: torch.Tensor, weights:
     need = L.gfr_experts16_workspace(rows, slots, hidden, inter)
     if need < 0:
         _check(need)
-    out = _result(out, x.shape, out_dtype or dtype, x, stream, here)
+    out, out_stride = _result(out, x.shape, out_dtype or dtype, x, stream, here)
     workspace = _empty((need,), torch.uint8, x, stream)
     handle = _handle(stream, here)
     rc = L.gfr_experts16_run(
         handle, _EXPERTS16.pack(rows, slots, hidden, inter, E, types.get(dtype, -1), act, limit or 0.0, residual_type,
                                 types.get(out.dtype, -1), x.data_ptr(), _row_stride(x), gu.data_ptr(), gu_stride, gu_expert,
                                 down.data_ptr(), down_stride, down_expert, picks.data_ptr(), weights.data_ptr(), residual_at,
-                                residual_stride, out.data_ptr(), _row_stride(out), workspace.data_ptr(), need))
+                                residual_stride, out.data_ptr(), out_stride, workspace.data_ptr(), need))
     if rc:
         _check(rc)
     return out
+
+
+_GATE_ACTIVATIONS = {None: 0, "none": 0, "sigmoid": 1}
 
 
 def _block_norm(x, residual, pre, post, gate, gate_activation, scale, residual_scale, keep, h, out, out_dtype, stream):
@@ -1155,28 +1166,31 @@ def _block_norm(x, residual, pre, post, gate, gate_activation, scale, residual_s
             raise ValueError(f"gate {tuple(gate.shape)}: [n], [rows, 1], [1, n] or [rows, n] of ({rows}, {n})")
         gate_at, gate_type, gate_column = gate.data_ptr(), types[gate.dtype], int(g.shape[1] == n and n > 1)
         gate_row = _row_stride(g) if g.shape[0] > 1 else 0
-    if gate_activation not in (None, "none", "sigmoid"):
+    sigmoid = _GATE_ACTIVATIONS.get(gate_activation)
+    if sigmoid is None:
         raise ValueError(f"gate activation {gate_activation!r} of ['none', 'sigmoid']")
     h_at = h_type = h_stride = y_at = y_type = y_stride = 0
+    post_fields = pre_fields = _NO_NORM
+    if post is not None:
+        post_fields = post.fields(n, here)
     if keep:
-        h = _result(h, shape, x.dtype if residual is None else residual.dtype, x, stream, here, "h")
-        h_at, h_type, h_stride = h.data_ptr(), types[h.dtype], _row_stride(h)
+        h, h_stride = _result(h, shape, x.dtype if residual is None else residual.dtype, x, stream, here, "h")
+        h_at, h_type = h.data_ptr(), types[h.dtype]
     if pre is not None:
-        if out is not None and out_dtype is not None and out.dtype is not out_dtype:
-            raise ValueError(f"out {out.dtype}: want {out_dtype}")
-        if out_dtype is not None and out_dtype not in types:
-            raise ValueError(f"out {out_dtype}: bf16, fp16 or fp32")
-        out = _result(out, shape, out_dtype or x.dtype, x, stream, here)
-        y_at, y_type, y_stride = out.data_ptr(), types[out.dtype], _row_stride(out)
+        pre_fields = pre.fields(n, here)
+        if out_dtype is None:
+            out_dtype = x.dtype if out is None else out.dtype
+        elif out_dtype not in types or (out is not None and out.dtype is not out_dtype):
+            raise ValueError(f"out {out_dtype if out is None else out.dtype}: want {out_dtype}, one of bf16, fp16 and fp32")
+        out, y_stride = _result(out, shape, out_dtype, x, stream, here)
+        y_at, y_type = out.data_ptr(), types[out_dtype]
     elif out is not None or out_dtype is not None:
         raise ValueError("out is the pre norm's: want pre")
     handle = _handle(stream, here)
     rc = (_lib or lib()).gfr_block_norm_run(
-        handle, _BLOCK_NORM.pack(rows, n, x_type, residual_type, gate_type, h_type, y_type, gate_column,
-                                 int(gate_activation == "sigmoid"), scale, residual_scale, x.data_ptr(), _row_stride(x),
-                                 residual_at, residual_stride, gate_at, gate_row, h_at, h_stride, y_at, y_stride,
-                                 *(_NO_NORM if post is None else post.fields(n, here)),
-                                 *(_NO_NORM if pre is None else pre.fields(n, here))))
+        handle, _BLOCK_NORM.pack(rows, n, x_type, residual_type, gate_type, h_type, y_type, gate_column, sigmoid, scale,
+                                 residual_scale, x.data_ptr(), _row_stride(x), residual_at, residual_stride, gate_at,
+                                 gate_row, h_at, h_stride, y_at, y_stride, *post_fields, *pre_fields))
     if rc:
         _check(rc)
     return h, out
@@ -1226,24 +1240,29 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     here = _get_device()
     if logits.get_device() != here or tokens.get_device() != here:
         _elsewhere(logits, tokens)
-    each = tokens if len(shape) == 2 else tokens.unsqueeze(1)
+    count = 1
+    if len(shape) == 2:
+        count, token_stride = shape[1], _row_stride(tokens)
+    else:
+        token_stride = max(tokens.stride(0), 1) if rows == 1 else tokens.stride(0)
     L = _lib or lib()
     need = L.gfr_logprobs_workspace(rows, vocab, top)
     if need < 0:
         _check(need)
-    workspace = _empty((need,), torch.uint8, logits, stream)
-    logprobs = _empty(shape, torch.float32, logits, stream)
-    entropy = _empty((rows,), torch.float32, logits, stream)
+    new = logits.new_empty if stream is None else lambda shape, dtype: _empty(shape, dtype, logits, stream)
+    f32 = torch.float32
+    workspace = new((need,), dtype=torch.uint8)
+    logprobs, entropy = new(shape, dtype=f32), new((rows,), dtype=f32)
     top_ids = top_logprobs = None
+    ids_at = top_at = 0
     if top:
-        top_ids = _empty((rows, top), torch.int32, logits, stream)
-        top_logprobs = _empty((rows, top), torch.float32, logits, stream)
+        top_ids, top_logprobs = new((rows, top), dtype=torch.int32), new((rows, top), dtype=f32)
+        ids_at, top_at = top_ids.data_ptr(), top_logprobs.data_ptr()
     handle = _handle(stream, here)
     rc = L.gfr_logprobs_run(
-        handle, _LOGPROBS.pack(rows, vocab, each.shape[1], top, kind, int(tokens.dtype is torch.int64), temperature,
-                               logits.data_ptr(), _row_stride(logits), each.data_ptr(), _row_stride(each),
-                               logprobs.data_ptr(), entropy.data_ptr(), _ptr(top_ids), _ptr(top_logprobs),
-                               workspace.data_ptr(), need))
+        handle, _LOGPROBS.pack(rows, vocab, count, top, kind, tokens.dtype is torch.int64, temperature, logits.data_ptr(),
+                               _row_stride(logits), tokens.data_ptr(), token_stride,
+                               logprobs.data_ptr(), entropy.data_ptr(), ids_at, top_at, workspace.data_ptr(), need))
     if rc:
         _check(rc)
     return LogProbs(logprobs, entropy, top_ids, top_logprobs)
