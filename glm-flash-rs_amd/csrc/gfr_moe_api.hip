@@ -682,7 +682,7 @@ int gfr_logprobs_run(hipStream_t stream, const gfr_logprobs* d) {
     const int64_t need = gfr_logprobs_workspace(d->rows, d->vocab, d->top);
     if (need < 0) return GFR_EINVAL;
     if (d->tokens < 0 || d->tokens > 1 << 24) return fail(GFR_EINVAL, "logprobs: tokens %d outside 0..%d", d->tokens, 1 << 24);
-    if (!d->logits || !d->entropy || !d->workspace || (d->tokens && (!d->token || !d->logprobs)) ||
+    if (!d->logits || !d->entropy || (need && !d->workspace) || (d->tokens && (!d->token || !d->logprobs)) ||
         (d->top && (!d->top_ids || !d->top_logprobs)))
         return fail(GFR_EINVAL, "logprobs: null argument");
     if (!known_type(d->type)) return fail(GFR_EINVAL, "logprobs: logits type %d", d->type);

@@ -21,7 +21,6 @@
 namespace gfr {
 namespace {
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, ROOM = 1024;
 constexpr float LOG2E = 1.44269504088896341f;
 
 // A chunk's share of its row: the largest logit, how many equal it, the sums of the others' exponentials and of
@@ -98,15 +97,54 @@ __device__ __forceinline__ float threshold(float set, int top) {
     return -max_over(64, above < top ? -set : -INFINITY);
 }
 
+// A row's results from its sums: the entropy, the tokens' log probabilities (thread `from` of `threads` on), a place's.
+struct Row {
+    float most, log_sum;
+    __device__ __forceinline__ float log_p(const LogprobsJob& d, float l) const {
+        if (!(l > -INFINITY)) return -INFINITY;
+        return (l == most ? 0.f : (l - most) * d.by) - log_sum;
+    }
+    __device__ __forceinline__ void tokens(const LogprobsJob& d, int row, int from, int threads) const {
+        for (int i = from; i < d.tokens; i += threads) {
+            const int64_t at = (int64_t)row * d.tokens_stride + i;
+            const int64_t token = d.wide_tokens ? static_cast<const int64_t*>(d.token)[at] : static_cast<const int32_t*>(d.token)[at];
+            const bool there = token >= 0 && token < d.vocab;         // a token that is not in the vocabulary: probability 0
+            d.logprob[(int64_t)row * d.tokens + i] =
+                there ? log_p(d, load_one(d.logits, d.type, (int64_t)row * d.stride + token)) : -INFINITY;
+        }
+    }
+    __device__ __forceinline__ void place(const LogprobsJob& d, int row, int i, uint64_t p) const {
+        d.top_ids[(int64_t)row * d.top + i] = token_of(p);
+        d.top_logprobs[(int64_t)row * d.top + i] = log_p(d, logit_of(p));
+    }
+    // Fewer logits than places are not masked: from place i on the masked tokens in order, enough of which are among the first
+    // 64. One wave.
+    __device__ __forceinline__ void masked(const LogprobsJob& d, int row, int i) const {
+        const int lane = threadIdx.x & 63;
+        const bool masked = lane < d.vocab && !(load_one(d.logits, d.type, (int64_t)row * d.stride + lane) > -INFINITY);
+        const int at = i + set_before(__ballot(masked));
+        if (!masked || at >= d.top) return;
+        d.top_ids[(int64_t)row * d.top + at] = lane;
+        d.top_logprobs[(int64_t)row * d.top + at] = -INFINITY;
+    }
+};
+__device__ __forceinline__ Row row_of(const LogprobsJob& d, int row, const Share& s, bool writes) {
+    const Row r = {s.most, logf(s.count) + log1pf(s.rest / s.count)};
+    if (writes) d.entropy[row] = s.count > 0.f ? r.log_sum - s.slope * d.by / (s.count + s.rest) : 0.f;
+    return r;
+}
+
 // V groups of eight logits a thread: group g of thread i starts at the chunk's column 8 (g THREADS + i).
-template <int TYPE, int V>
+// ONE: the chunk is its row, and there is no second launch.
+template <int TYPE, int THREADS, int V, bool ONE>
 __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) {
+    constexpr int WAVES = THREADS / 64, ROOM = 2 * THREADS;
     __shared__ float maxima[WAVES][64];
     __shared__ float sums[WAVES][3];
     __shared__ uint64_t places[ROOM];
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x / d.chunks, chunk = blockIdx.x % d.chunks;
+    const int row = ONE ? (int)blockIdx.x : blockIdx.x / d.chunks, chunk = ONE ? 0 : blockIdx.x % d.chunks;
     const int64_t c0 = (int64_t)chunk * d.span, end = c0 + d.span < d.vocab ? c0 + d.span : d.vocab;
     const char* logits = static_cast<const char*>(d.logits) + (int64_t)row * d.stride * (TYPE == TYPE_F32 ? 4 : 2);
     Eight raw[V];
@@ -179,18 +217,36 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
             }
     }
     __syncthreads();
-    const int64_t part = (int64_t)row * d.chunks + chunk;
-    if (tid < WAVES) {
-        Share s = {M, sum_over(WAVES, sums[tid][2]), sum_over(WAVES, sums[tid][0]), sum_over(WAVES, sums[tid][1])};
+    // the sums in the first lanes of every wave of a row's only chunk, or of the first one
+    Share s = {M, 0.f, 0.f, 0.f};
+    if (ONE || tid < WAVES) {
+        const int w = lane & (WAVES - 1);
+        s.count = sum_over(WAVES, sums[w][2]), s.rest = sum_over(WAVES, sums[w][0]), s.slope = sum_over(WAVES, sums[w][1]);
         const float right = __builtin_amdgcn_exp2f(-off);
         s.rest *= right, s.slope *= right / by;
+    }
+    Row r;
+    uint64_t* out = nullptr;
+    if constexpr (ONE) {
+        r = row_of(d, row, s, tid == 0);
+        r.tokens(d, row, THREADS - 1 - tid, THREADS);
+    } else {
+        const int64_t part = (int64_t)row * d.chunks + chunk;
         if (tid == 0) static_cast<Share*>(d.shares)[part] = s;
+        out = static_cast<uint64_t*>(d.places) + part * d.top;
     }
     if (!d.top) return;
-    uint64_t* out = static_cast<uint64_t*>(d.places) + part * d.top;
+    const auto put = [&](int i, uint64_t p) {
+        if constexpr (ONE) r.place(d, row, i, p);
+        else out[i] = p;
+    };
     const int n = found;
     if (n <= ROOM) {
-        if (tid >= n && tid < d.top) out[tid] = 0;
+        if constexpr (ONE) {
+            if (wave == 0 && n < d.top) r.masked(d, row, n);
+        } else {
+            if (tid >= n && tid < d.top) out[tid] = 0;
+        }
         // 2^by lanes count those before a place
         int by = 6;
         while (by && n << by > THREADS) --by;
@@ -199,7 +255,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
             int before = 0;
             for (int o = tid & ((1 << by) - 1); o < n; o += 1 << by) before += places[o] > p;
             before = sum_over(1 << by, before);
-            if (before < d.top) out[before] = p;
+            if (before < d.top && (tid & ((1 << by) - 1)) == 0) put(before, p);
         }
         return;
     }
@@ -222,7 +278,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
         __syncthreads();
         last = places[0];
         for (int w = 1; w < WAVES; ++w) last = larger(last, places[w]);
-        if (tid == 0) out[i] = last;
+        if (tid == 0) put(i, last);
     }
 }
 
@@ -243,25 +299,12 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(LogprobsJob d) {
         count = 0.f, rest = all * e, slope = e * fmaf(x, all, s.slope);
     }
     count = sum_over(64, count), rest = sum_over(64, rest), slope = sum_over(64, slope);
-    const float log_sum = logf(count) + log1pf(rest / count);
-    const auto log_p = [&](float l) {
-        if (!(l > -INFINITY)) return -INFINITY;
-        return (l == M ? 0.f : (l - M) * d.by) - log_sum;
-    };
-    if (tid == 0) d.entropy[row] = count > 0.f ? log_sum - slope * d.by / (count + rest) : 0.f;
-    const int64_t base = (int64_t)row * d.stride;
-    for (int i = JOIN - 1 - tid; i < d.tokens; i += JOIN) {           // (from the last wave on: the first has the places)
-        const int64_t at = (int64_t)row * d.tokens_stride + i;
-        const int64_t token = d.wide_tokens ? static_cast<const int64_t*>(d.token)[at] : static_cast<const int32_t*>(d.token)[at];
-        const bool there = token >= 0 && token < d.vocab;             // a token that is not in the vocabulary: probability 0
-        d.logprob[(int64_t)row * d.tokens + i] = there ? log_p(load_one(d.logits, d.type, base + token)) : -INFINITY;
-    }
+    const Row r = row_of(d, row, {M, count, rest, slope}, tid == 0);
+    r.tokens(d, row, JOIN - 1 - tid, JOIN);                           // (from the last wave on: the first has the places)
     if (!d.top) return;
     // a chunk's places are in order, so that the next one is the largest of the chunks' heads
     __syncthreads();
     if (tid >= 64) return;
-    int* ids = d.top_ids + (int64_t)row * d.top;
-    float* logps = d.top_logprobs + (int64_t)row * d.top;
     const int end = lane < d.chunks ? (lane + 1) * d.top : 0;
     int next = lane * d.top;
     const auto take = [&] { return next < end ? places[next++] : 0; };
@@ -273,18 +316,23 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(LogprobsJob d) {
         if (lane == i) kept = best;
         if (head == best) head = after, after = take();
     }
-    if (lane < i) ids[lane] = token_of(kept), logps[lane] = log_p(logit_of(kept));
-    // fewer logits than places are not masked: the masked tokens in order, enough of which are among the first 64
-    if (i < d.top) {
-        const bool masked = lane < d.vocab && !(load_one(d.logits, d.type, base + lane) > -INFINITY);
-        const int place = i + set_before(__ballot(masked));
-        if (masked && place < d.top) ids[place] = lane, logps[place] = -INFINITY;
-    }
+    if (lane < i) r.place(d, row, lane, kept);
+    if (i < d.top) r.masked(d, row, i);
 }
 
+// A row of at most 8 * 8 * 512 logits is one chunk, of the fewest groups that hold it: of 512 threads, or of 128 where there
+// are rows for every CU and they are short (us with 512 threads in two launches, in one, with 128: 8192 rows of 1000 118, 47,
+// 19; 8192 of 4000 without places -, 37, 18; 2000 of 8000 -, 18.3, 19.3; one of 4000 11.6, 5.2, 7.0).
+constexpr int WIDE = 512, NARROW = 128, MOST = 8 * 8 * WIDE;
+
+template <int TYPE, int THREADS, int V>
+hipError_t launch_rows(hipStream_t s, const LogprobsJob& d) {
+    logprobs_chunk_kernel<TYPE, THREADS, V, true><<<dim3((unsigned)d.rows), THREADS, 0, s>>>(d);
+    return hipGetLastError();
+}
 template <int TYPE, int V>
-hipError_t launch(hipStream_t s, const LogprobsJob& d) {
-    logprobs_chunk_kernel<TYPE, V><<<dim3((unsigned)(d.rows * (int64_t)d.chunks)), THREADS, 0, s>>>(d);
+hipError_t launch_chunks(hipStream_t s, const LogprobsJob& d) {
+    logprobs_chunk_kernel<TYPE, WIDE, V, false><<<dim3((unsigned)(d.rows * (int64_t)d.chunks)), WIDE, 0, s>>>(d);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     logprobs_join_kernel<<<dim3((unsigned)d.rows), JOIN, (size_t)d.chunks * d.top * sizeof(uint64_t), s>>>(d);
@@ -292,19 +340,29 @@ hipError_t launch(hipStream_t s, const LogprobsJob& d) {
 }
 template <int TYPE>
 hipError_t launch(hipStream_t s, const LogprobsJob& d, int groups) {
+    if (d.chunks == 1) {
+        if (d.rows >= 1024 && d.vocab <= 32 * NARROW) {
+            if (d.vocab <= 8 * NARROW) return launch_rows<TYPE, NARROW, 1>(s, d);
+            return d.vocab <= 16 * NARROW ? launch_rows<TYPE, NARROW, 2>(s, d) : launch_rows<TYPE, NARROW, 4>(s, d);
+        }
+        if (d.vocab <= 8 * WIDE) return launch_rows<TYPE, WIDE, 1>(s, d);
+        if (d.vocab <= 16 * WIDE) return launch_rows<TYPE, WIDE, 2>(s, d);
+        return d.vocab <= 32 * WIDE ? launch_rows<TYPE, WIDE, 4>(s, d) : launch_rows<TYPE, WIDE, 8>(s, d);
+    }
     switch (groups) {
-        case 1: return launch<TYPE, 1>(s, d);
-        case 2: return launch<TYPE, 2>(s, d);
-        case 4: return launch<TYPE, 4>(s, d);
-        default: return launch<TYPE, 8>(s, d);
+        case 1: return launch_chunks<TYPE, 1>(s, d);
+        case 2: return launch_chunks<TYPE, 2>(s, d);
+        case 4: return launch_chunks<TYPE, 4>(s, d);
+        default: return launch_chunks<TYPE, 8>(s, d);
     }
 }
 
-// Groups of eight logits a thread: 8, and fewer where that leaves CUs idle, as long as a row has no more chunks than the
-// join has lanes. (4096 rows of 160000 bf16, top 4, with 2, 4 and 8 groups: 440, 304 and 264 us.)
-int chunks_of(int vocab, int groups) { return (int)(((int64_t)vocab + 8 * THREADS * groups - 1) / (8 * THREADS * groups)); }
+// Groups of eight logits a thread of longer rows: 8, and fewer where that leaves CUs idle, as long as a row has no more
+// chunks than the join has lanes. (4096 rows of 160000 bf16, top 4, with 2, 4 and 8 groups: 440, 304 and 264 us.)
+int chunks_of(int vocab, int groups) { return (int)(((int64_t)vocab + 8 * WIDE * groups - 1) / (8 * WIDE * groups)); }
 int groups_of(int rows, int vocab) {
     int v = 8;
+    if (vocab <= MOST) return v;
     while (v > 1 && (int64_t)rows * chunks_of(vocab, v) < 512 && chunks_of(vocab, v / 2) <= 64) v /= 2;
     return v;
 }
@@ -313,7 +371,8 @@ int groups_of(int rows, int vocab) {
 
 int logprobs_chunks(int rows, int vocab) { return chunks_of(vocab, groups_of(rows, vocab)); }
 size_t logprobs_workspace(int rows, int vocab, int top) {
-    return (size_t)rows * logprobs_chunks(rows, vocab) * (sizeof(Share) + top * sizeof(uint64_t));
+    const int chunks = logprobs_chunks(rows, vocab);
+    return chunks == 1 ? 0 : (size_t)rows * chunks * (sizeof(Share) + top * sizeof(uint64_t));
 }
 
 hipError_t launch_logprobs(hipStream_t s, LogprobsJob d, void* workspace) {

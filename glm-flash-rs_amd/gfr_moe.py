@@ -1251,7 +1251,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
         _check(need)
     new = logits.new_empty if stream is None else lambda shape, dtype: _empty(shape, dtype, logits, stream)
     f32 = torch.float32
-    workspace = new((need,), dtype=torch.uint8)
+    workspace = new((need,), dtype=torch.uint8) if need else None
     logprobs, entropy = new(shape, dtype=f32), new((rows,), dtype=f32)
     top_ids = top_logprobs = None
     ids_at = top_at = 0
@@ -1262,7 +1262,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     rc = L.gfr_logprobs_run(
         handle, _LOGPROBS.pack(rows, vocab, count, top, kind, tokens.dtype is torch.int64, temperature, logits.data_ptr(),
                                _row_stride(logits), tokens.data_ptr(), token_stride,
-                               logprobs.data_ptr(), entropy.data_ptr(), ids_at, top_at, workspace.data_ptr(), need))
+                               logprobs.data_ptr(), entropy.data_ptr(), ids_at, top_at, _ptr(workspace), need))
     if rc:
         _check(rc)
     return LogProbs(logprobs, entropy, top_ids, top_logprobs)

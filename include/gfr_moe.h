@@ -438,8 +438,8 @@ int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d);
  * within a few units of 32 bits also where it is near 0. A row's results depend on no other row; its last bits may on the
  * number of rows, which the order of its sums follows (the tokens' order does not). tokens or top may be 0; top <= 32 and
  * vocab, vocab <= 2^21, temperature 1e-6 .. 1e6, at least one row.
- * workspace: gfr_logprobs_workspace(rows, vocab, top) bytes of device memory (at most 2^31), 8-byte aligned, that are the
- * call's until its work is done: two calls that may overlap, or two captured graphs that may, take two workspaces. Outputs
+ * workspace: gfr_logprobs_workspace(rows, vocab, top) bytes of device memory (0 for vocab <= 32768; NULL then), 8-byte
+ * aligned, that are the call's until its work is done: two calls that may overlap, or two captured graphs that may, take two workspaces. Outputs
  * and the workspace must not share memory with anything else. */
 typedef struct gfr_logprobs {
     int rows, vocab, tokens, top;

@@ -101,6 +101,17 @@ def test_logprobs(gfr, vocab):
         check(gfr, l, tokens, top, rng.choice([1.0, 0.7, 1.3]), f"rows {rows} vocab {vocab} top {top} {dtype}")
 
 
+@pytest.mark.parametrize("vocab", [5, 1000, 1024, 1025, 2048, 2049, 4095, 4096, 4097, 9000])
+def test_many_rows(gfr, vocab):
+    """Windows of more rows than CUs hold, in every form that they take."""
+    for dtype in TYPES.values():
+        l = randn(vocab, 1100, vocab, dtype)
+        l[7] = -torch.inf
+        l[9, 1:] = torch.nan
+        l[11] = 2.0
+        check(gfr, l, torch.randint(0, vocab, (1100, 2), device="cuda"), min(vocab, 32), 0.7, f"vocab {vocab} {dtype}")
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("rows,vocab", [(1, 5), (3, 40), (2, 5000), (300, 33000), (2, 100001)])
 def test_orders(gfr, rows, vocab, dtype):

@@ -53,7 +53,7 @@ LOGPROBS = ("rows vocab tokens top type wide_tokens temperature logits stride to
     (dict(token=0), "null"), (dict(logprobs=0), "null"), (dict(top_ids=0), "null"), (dict(top_logprobs=0), "null"),
     (dict(type=3), "type 3"), (dict(wide_tokens=2), "wide tokens 2"), (dict(temperature=0.0), "temperature"),
     (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
-    (dict(temperature=float("inf")), "temperature"), (dict(stride=99), "stride 99"), (dict(tokens_stride=1), "tokens' 1"),
+    (dict(temperature=float("inf")), "temperature"), (dict(stride=39999), "stride 39999"), (dict(tokens_stride=1), "tokens' 1"),
     (dict(stride=(1 << 31) + 1), "stride"), (dict(workspace_bytes=100), "workspace of 100 bytes"), (dict(logits=(1 << 40) + 1), "aligned"),
     (dict(token=(1 << 41) + 4), "aligned"), (dict(entropy=(1 << 43) + 2), "aligned"), (dict(workspace=(1 << 46) + 4), "aligned"),
     (dict(entropy=1 << 40), "overlaps"), (dict(workspace=1 << 41), "overlaps"), (dict(top_ids=(1 << 42) + 24), "overlaps"),
@@ -61,7 +61,7 @@ LOGPROBS = ("rows vocab tokens top type wide_tokens temperature logits stride to
 ])
 def test_logprobs_refuses(kw, needle):
     import gfr_moe
-    a = dict(rows=4, vocab=100, tokens=2, top=5, type=0, wide_tokens=1, temperature=1.0, logits=1 << 40, stride=100,
+    a = dict(rows=4, vocab=40000, tokens=2, top=5, type=0, wide_tokens=1, temperature=1.0, logits=1 << 40, stride=40000,
              token=1 << 41, tokens_stride=2, logprobs=1 << 42, entropy=1 << 43, top_ids=1 << 44, top_logprobs=1 << 45,
              workspace=1 << 46, workspace_bytes=1 << 20)
     a.update(kw)
@@ -74,11 +74,12 @@ def test_logprobs_workspace():
     """Enough for every chunk's sums and places, and refused for what a run refuses."""
     import gfr_moe
     L = gfr_moe.lib()
-    assert L.gfr_logprobs_workspace(1, 1, 0) == 16
+    for rows, vocab, top in ((1, 1, 0), (5, 32768, 32), (70000, 1000, 5)):
+        assert L.gfr_logprobs_workspace(rows, vocab, top) == 0          # a row is one chunk
     assert L.gfr_logprobs_workspace(1, 160000, 20) >= 40 * (16 + 20 * 8)
-    for rows, vocab in ((1, 1 << 21), (3, 32003), (4096, 160000)):
+    for rows, vocab in ((1, 1 << 21), (3, 32769), (4096, 160000)):
         chunks = L.gfr_logprobs_workspace(rows, vocab, 0) // (16 * rows)
-        assert 1 <= chunks <= 64 and chunks * 32768 >= vocab
+        assert 2 <= chunks <= 64 and chunks * 32768 >= vocab
         assert L.gfr_logprobs_workspace(rows, vocab, 32) == rows * chunks * (16 + 32 * 8)
     assert L.gfr_logprobs_workspace(0, 10, 0) < 0 and L.gfr_logprobs_workspace(1, 10, 11) < 0
 
