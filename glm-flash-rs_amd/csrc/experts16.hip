@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Expert
     extern __shared__ __align__(1024) char lds[];
     __shared__ float weight[FEW_PAIRS];                               // of the pairs, and whether an expert is theirs
     __shared__ bool there[FEW_PAIRS];
-    constexpr int U = 3;
+    constexpr int U = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a = lane & 15, q = lane >> 4;
     const int c0 = blockIdx.x * 16, pairs = d.rows * d.slots, chunks = d.inter_pad / 64;
     f4_t* parts = reinterpret_cast<f4_t*>(lds + FEW_WAVES * 2048);    // [pairs][chunks][4]

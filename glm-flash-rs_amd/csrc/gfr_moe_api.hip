@@ -713,7 +713,7 @@ int gfr_logprobs_run(hipStream_t stream, const gfr_logprobs* d) {
                 return fail(GFR_EINVAL, "logprobs: an output or the workspace overlaps another tensor");
     gfr::LogprobsJob job = {d->logits, d->token, d->logprobs, d->entropy, d->top_ids, d->top_logprobs, d->stride,
                             d->tokens_stride, d->type, d->rows, d->vocab, d->tokens, d->top, d->wide_tokens != 0,
-                            1.f / d->temperature, 0, 0, nullptr, nullptr};
+                            d->temperature, (float)(1.4426950408889634 / d->temperature), 0, 0, nullptr, nullptr};
     hipError_t e = gfr::launch_logprobs(stream, job, d->workspace);
     if (e != hipSuccess) return hip_fail(e, "logprobs");
     return 0;

@@ -234,7 +234,7 @@ struct LogprobsJob {
     int64_t stride, tokens_stride;
     int type, rows, vocab, tokens, top;
     bool wide_tokens;
-    float by;                       // 1 / temperature
+    float temperature, by;          // by: log2(e) / temperature
     // set by launch_logprobs: chunks a row, logits a chunk, the chunks' sums and places in the workspace
     int chunks;
     int64_t span;

@@ -21,7 +21,6 @@
 namespace gfr {
 namespace {
 
-constexpr float LOG2E = 1.44269504088896341f;
 
 // A chunk's share of its row: the largest logit, how many equal it, the sums of the others' exponentials and of
 // (l - largest) times these (logits before they are divided by the temperature).
@@ -102,7 +101,7 @@ struct Row {
     float most, log_sum;
     __device__ __forceinline__ float log_p(const LogprobsJob& d, float l) const {
         if (!(l > -INFINITY)) return -INFINITY;
-        return (l == most ? 0.f : (l - most) * d.by) - log_sum;
+        return (l == most ? 0.f : (l - most) / d.temperature) - log_sum;
     }
     __device__ __forceinline__ void tokens(const LogprobsJob& d, int row, int from, int threads) const {
         for (int i = from; i < d.tokens; i += threads) {
@@ -130,7 +129,7 @@ struct Row {
 };
 __device__ __forceinline__ Row row_of(const LogprobsJob& d, int row, const Share& s, bool writes) {
     const Row r = {s.most, logf(s.count) + log1pf(s.rest / s.count)};
-    if (writes) d.entropy[row] = s.count > 0.f ? r.log_sum - s.slope * d.by / (s.count + s.rest) : 0.f;
+    if (writes) d.entropy[row] = s.count > 0.f ? r.log_sum - s.slope / d.temperature / (s.count + s.rest) : 0.f;
     return r;
 }
 
@@ -173,9 +172,8 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
     // is summed in units of the exponent.
     // Where M k is no finite number all others are too far below M to count (their distance is at least 2^-24 of M), or
     // there are none.
-    const float by = LOG2E * d.by;
-    const bool finite = fabsf(M * by) < INFINITY;
-    const float k = finite ? by : 0.f, c = finite ? -M * k : -1e30f, off = finite ? fmaf(-M, k, -c) : 0.f;
+    const bool finite = fabsf(M * d.by) < INFINITY;
+    const float k = finite ? d.by : 0.f, c = finite ? -M * k : -1e30f, off = finite ? fmaf(-M, k, -c) : 0.f;
     const auto exponent = [&](float l) { return fmaxf(fmaf(l, k, c), -1e30f); };   // -1e30: masked, and exp2 of it is 0
     float rest = 0.f, slope = 0.f, count = 0.f;
 #pragma unroll
@@ -223,7 +221,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
         const int w = lane & (WAVES - 1);
         s.count = sum_over(WAVES, sums[w][2]), s.rest = sum_over(WAVES, sums[w][0]), s.slope = sum_over(WAVES, sums[w][1]);
         const float right = __builtin_amdgcn_exp2f(-off);
-        s.rest *= right, s.slope *= right / by;
+        s.rest *= right, s.slope *= right / d.by;
     }
     Row r;
     uint64_t* out = nullptr;
@@ -295,7 +293,7 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(LogprobsJob d) {
     const float M = max_over(64, s.most);
     float count = s.count, rest = s.rest, slope = s.slope;
     if (s.most < M) {
-        const float x = fmaxf(s.most - M, -1e30f), e = __builtin_amdgcn_exp2f(x * (LOG2E * d.by)), all = s.count + s.rest;
+        const float x = fmaxf(s.most - M, -1e30f), e = __builtin_amdgcn_exp2f(x * d.by), all = s.count + s.rest;
         count = 0.f, rest = all * e, slope = e * fmaf(x, all, s.slope);
     }
     count = sum_over(64, count), rest = sum_over(64, rest), slope = sum_over(64, slope);
