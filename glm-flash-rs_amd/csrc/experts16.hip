@@ -5,12 +5,16 @@
 // the activations are held as the sum of two 16-bit values, 16 bits of them or more, which costs the matrix core a second
 // pass over the same weights in registers.
 //
-// Bound: the weights of the experts that are picked, read once. A workgroup takes one expert's share of the columns and all
-// the rows that picked it, in passes of up to 16 RB, so that an expert's weights are read once however many rows pick it
+// Bound: HBM, the weights of the experts that are picked, read once. A workgroup takes one expert's share of the columns and
+// all the rows that picked it, in passes of up to 16 RB, so that an expert's weights are read once however many rows pick it
 // (again, from the caches, for more than one pass). Weights are the matrix core's A operand (v_mfma_f32_16x16x32: D holds,
 // in lane l, columns 4 (l / 16) .. + 3 of the tile for row l % 16) and go through LDS stages of a wave's own as whole lines;
 // rows are the B operand, loaded as fragments, which the caches hold. A row's sums are taken in an order of the
 // sizes alone, so that they depend neither on the other rows nor on their number.
+// Graph replays, us (GB/s of weights): 64 rows top-8 of 160, 5120 -> 1408 bf16 1110 (5880); 12 rows top-8 of 288, 4096 ->
+// 512 148 (6020); 4 rows top-8 of 64, 4096 -> 1024 115 (5800); one row of 9 slots, 4096 -> 512 28.8 (3930), where two launches'
+// starts and ends are a quarter; 5 rows top-3 of 20, 1001 -> 333 fp16 19.6, all of it latency. Asking for the down matrices
+// from the first launch's end made the one row slower (34 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -130,6 +134,9 @@ __device__ __forceinline__ void pipeline(Chunk (&f)[U], int n, Load load, Use us
 }
 
 // ---- gate and up --------------------------------------------------------------------------------------------------
+// Eight waves (16 took 37.7 us and not 31.9 at one row, 1806 and not 1107 at 64), two chunks in flight (four: 34.1 and 1171; no
+// registers for them). Two tiles a wave, and one where the workgroups would be fewer than 1.25 a CU: one row of 9 slots, 4096
+// -> 512 29.3 us and not 31.5, 4 rows of 2, 1024 -> 256 9.3 and 9.6; beyond that 2 rows of 8 43.0 and 41.8, 64 rows 1238 and 1110.
 constexpr int UP_WAVES = 8;
 
 // One pass: members [from, from + 16 RB) of the expert, columns c0 .. + 8 EB. A tile of 16 weight rows is 8 gate rows
@@ -264,6 +271,7 @@ __global__ void __launch_bounds__(64 * UP_WAVES, RB == 1 ? 4 : 2) experts16_up_k
 }
 
 // ---- down ---------------------------------------------------------------------------------------------------------
+// (146 registers, three waves a SIMD; held to four, with registers spilled, 12 rows took 161 us and not 148)
 constexpr int DOWN_WAVES = 4, DOWN_TILES = 2, DOWN_COLS = 16 * DOWN_TILES * DOWN_WAVES;
 
 // A tile's sum over a chunk, in an order that both forms of the product share (each adds the chunks' sums in turn).
@@ -413,113 +421,96 @@ __global__ void __launch_bounds__(256) experts16_combine_kernel(Experts16Job d) 
 }
 
 // ---- down and the rows' sums at once, for few pairs ---------------------------------------------------------------
-// A workgroup takes 16 columns of all pairs (at most 64, inter at least 8): its waves share the picked experts' chunks of k in turn, a chunk's
-// sums of its members go to LDS, and are added there in the order of the other form: chunks, then slots.
-constexpr int FEW_WAVES = 8, FEW_PAIRS = 64, FEW_LDS = 65536;
+// A workgroup takes 16 columns of all pairs (inter at least 8): its waves share the picked experts' chunks of k in turn, a
+// chunk's sums of its members go to LDS, and are added there in the order of the other form: chunks, then slots. Every wave lists the
+// picks for itself, and few workgroups hold long chains of chunks, so that this is for up to 10 pairs and 96 chunks of them.
+// us with it, and with the down launch and the rows' sums in another: 1 row of 9 slots, 4096 -> 512 28.8, 33.1; 1 of 4, 2048 ->
+// 768 13.7, 16.4; 4 of 2, 1024 -> 256 8.7, 10.3; 1 of 8, 4097 -> 511 34.1, 34.7; and beyond: 1 of 8, 2048 -> 1024 29.6, 28.9; 5 of
+// 3, 1024 -> 384 17.3, 15.4; 1 of 8, 7168 -> 2048 132, 127. (16 or 4 waves at the first: 34.2, 30.0; three chunks in flight 29.4.)
+constexpr int FEW_WAVES = 8, FEW_PAIRS = 10, FEW_UNITS = 96;
 
 template <int TYPE>
-__global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Experts16Job d) {
-    extern __shared__ __align__(1024) char lds[];
+__global__ void __launch_bounds__(64 * FEW_WAVES) experts16_few_kernel(Experts16Job d) {
+    constexpr int U = 2;
+    __shared__ __align__(1024) char stages[FEW_WAVES * 2048];
+    __shared__ f4_t parts[FEW_UNITS * 4], sums[FEW_PAIRS * 4];        // [pairs][chunks][4], [pairs][4]
     __shared__ float weight[FEW_PAIRS];                               // of the pairs, and whether an expert is theirs
     __shared__ bool there[FEW_PAIRS];
-    constexpr int U = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), a = lane & 15, q = lane >> 4;
     const int c0 = blockIdx.x * 16, pairs = d.rows * d.slots, chunks = d.inter_pad / 64;
-    f4_t* parts = reinterpret_cast<f4_t*>(lds + FEW_WAVES * 2048);    // [pairs][chunks][4]
-    f4_t* sums = parts + pairs * chunks * 4;                          // [pairs][4]
-    char* stage = lds + wave * 2048;
+    char* stage = stages + wave * 2048;
 
     // the picked experts, one a lane, with the pairs that picked them
     const int pick = lane < pairs ? d.picks[lane] : -1;
     if (threadIdx.x < pairs) weight[threadIdx.x] = d.weights[threadIdx.x], there[threadIdx.x] = pick >= 0 && pick < d.experts;
     int expert = 0, count = 0;
-    uint32_t pairs_lo = 0, pairs_hi = 0;
+    uint32_t members = 0;
     for (int i = 0; i < pairs; ++i) {
         const int e = __builtin_amdgcn_readlane(pick, i);
-        const uint64_t same = __ballot(pick == e && lane < pairs);
-        if (e < 0 || e >= d.experts || __builtin_ctzll(same) != i) continue;
-        if (lane == count) expert = e, pairs_lo = (uint32_t)same, pairs_hi = (uint32_t)(same >> 32);
+        const uint32_t same = (uint32_t)__ballot(pick == e && lane < pairs);
+        if (e < 0 || e >= d.experts || __builtin_ctz(same) != i) continue;
+        if (lane == count) expert = e, members = same;
         ++count;
     }
     const int units = count * chunks, my_row = threadIdx.x >> 2, my_col = c0 + (threadIdx.x & 3) * 4;
     f4_t residual = {0.f, 0.f, 0.f, 0.f};
-    if (my_row < d.rows) residual = residual_at(d, my_row, my_col);
+    if (my_row < d.rows) residual = residual_at(d, my_row, my_col);   // (asked for ahead of its use)
     const int64_t row0 = min(c0 + (lane >> 3), d.hidden - 1), row1 = min(c0 + 8 + (lane >> 3), d.hidden - 1);
     struct Unit {
         typename Weights<TYPE, 1>::Chunk w;
         uint4 x[2][2];
         int pair;                                                     // this lane's member; negative: none
         int c;
-        uint64_t others;                                              // the members after the first 16
     };
     // the n-th pair of a set, n = this lane's a; negative: there are fewer
-    auto nth = [&](uint64_t set) {
-        if (!(set & (set - 1))) return a == 0 ? (int)__builtin_ctzll(set) : -1;
-        const int rank = set_before(set);
-        const bool in = (lane & 32 ? (uint32_t)(set >> 32) : (uint32_t)set) >> (lane & 31) & 1;
-        const int list = __builtin_amdgcn_ds_permute((in && rank < 16 ? rank : 63) * 4, lane);
+    const auto nth = [&](uint32_t set) {
+        if (!(set & (set - 1))) return a == 0 ? (int)__builtin_ctz(set) : -1;
+        const bool in = lane < 32 && (set >> (lane & 31) & 1);
+        const int list = __builtin_amdgcn_ds_permute((in ? set_before(set) : 63) * 4, lane);
         const int mine = __builtin_amdgcn_ds_bpermute(a * 4, list);
-        return a < __popcll(set) ? mine : -1;
-    };
-    auto load_rows = [&](uint4 (&x)[2][2], uint64_t set, int c) {     // this lane's member, or a negative number
-        const int pair = nth(set);
-        const uint16_t* xp = d.acts + (int64_t)(pair < 0 ? (int)__builtin_ctzll(set) : pair) * 2 * d.inter_pad + 8 * q + c * 64;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            x[s][0] = *reinterpret_cast<const uint4*>(xp + 32 * s);
-            x[s][1] = *reinterpret_cast<const uint4*>(xp + d.inter_pad + 32 * s);
-        }
-        return pair;
+        return a < __popc(set) ? mine : -1;
     };
     // this wave's place among the units: expert n's chunk c, its weights and pairs; units are asked for in turn
     int n = -1, c = chunks;
-    uint64_t set = 0;
+    uint32_t set = 0;
     Weights<TYPE, 1> w;
     const auto move = [&](int by) {
         for (c += by; c >= chunks; c -= chunks, ++n) {
         }
         const uint16_t* at = d.down + (int64_t)__builtin_amdgcn_readlane(expert, n) * d.down_expert;
-        set = (uint32_t)__builtin_amdgcn_readlane((int)pairs_lo, n) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)pairs_hi, n) << 32;
+        set = (uint32_t)__builtin_amdgcn_readlane((int)members, n);
         w = {{at + row0 * d.down_stride, at + row1 * d.down_stride}};
     };
     const int mine = (units - wave + FEW_WAVES - 1) / FEW_WAVES;
     int asked = 0;
     auto load = [&](Unit& f, int i) {
         if (i >= asked) move(asked++ ? FEW_WAVES : wave);             // (past the end: the last one again)
-        f.c = c;
+        f.c = c, f.pair = nth(set);
         w.ask(f.w, c * 64, d.inter);
-        f.pair = load_rows(f.x, set, c);
-        f.others = set;
-        if (__popcll(set) <= 16) f.others = 0;
-        else
-            for (int i = 0; i < 16; ++i) f.others &= f.others - 1;
+        const uint16_t* xp = d.acts + (int64_t)(f.pair < 0 ? (int)__builtin_ctz(set) : f.pair) * 2 * d.inter_pad + 8 * q + c * 64;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            f.x[s][0] = *reinterpret_cast<const uint4*>(xp + 32 * s);
+            f.x[s][1] = *reinterpret_cast<const uint4*>(xp + d.inter_pad + 32 * s);
+        }
     };
     auto multiply = [&](Unit& f, int) {
         if (f.c * 64 + 64 > d.inter) w.settle(f.w, f.c * 64, d.inter);
         w.stage(f.w, stage);
-        const uint4 w0 = w.fragment(stage, 0, 0), w1 = w.fragment(stage, 0, 1);
-        const f4_t v = chunk_sum<TYPE>(w0, w1, f.x);
+        const f4_t v = chunk_sum<TYPE>(w.fragment(stage, 0, 0), w.fragment(stage, 0, 1), f.x);
         if (f.pair >= 0) parts[(f.pair * chunks + f.c) * 4 + q] = v;
-        // (rows that pick an expert twice, or more than 16 rows; in registers of their own, that no wait of the others' differs)
-        for (uint64_t set = f.others; set;) {
-            uint4 x[2][2];
-            const int pair = load_rows(x, set, f.c);
-            const f4_t more = chunk_sum<TYPE>(w0, w1, x);
-            if (pair >= 0) parts[(pair * chunks + f.c) * 4 + q] = more;
-            for (int i = 0; i < 16 && set; ++i) set &= set - 1;
-        }
     };
     Unit f[U];
     pipeline(f, mine, load, multiply);
     __syncthreads();
-    for (int t = threadIdx.x; t < pairs * 4; t += 64 * FEW_WAVES) {
+    if (threadIdx.x < pairs * 4) {
         f4_t v = {0.f, 0.f, 0.f, 0.f};
-        if (there[t >> 2])
-            for (int c = 0; c < chunks; ++c) v += parts[((t >> 2) * chunks + c) * 4 + (t & 3)];
-        sums[t] = v;
+        if (there[threadIdx.x >> 2])
+            for (int i = 0; i < chunks; ++i) v += parts[((threadIdx.x >> 2) * chunks + i) * 4 + (threadIdx.x & 3)];
+        sums[threadIdx.x] = v;
     }
     __syncthreads();
-    if (my_row < d.rows) {                                            // (at most 64 rows: every output has a thread)
+    if (my_row < d.rows) {
         f4_t v = {0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < d.slots; ++s) {
             const int pair = my_row * d.slots + s;
@@ -530,10 +521,7 @@ __global__ void __launch_bounds__(64 * FEW_WAVES, 4) experts16_few_kernel(Expert
         finish(d, my_row, my_col, v, residual);
     }
 }
-static_assert(FEW_PAIRS * 4 <= 64 * FEW_WAVES, "a thread an output");
-size_t few_lds(const Experts16Job& d) {
-    return FEW_WAVES * 2048 + (size_t)d.rows * d.slots * (d.inter_pad / 64 + 1) * 64;
-}
+static_assert(FEW_PAIRS <= 16 && FEW_PAIRS * 4 <= 64 * FEW_WAVES, "one tile of members, a thread an output");
 
 template <int TYPE, int EB, int RB>
 hipError_t launch_up(hipStream_t s, const Experts16Job& d, int64_t leaders) {
@@ -543,15 +531,15 @@ hipError_t launch_up(hipStream_t s, const Experts16Job& d, int64_t leaders) {
 template <int TYPE, int RB>
 hipError_t launch(hipStream_t s, const Experts16Job& d) {
     const int64_t pairs = (int64_t)d.rows * d.slots, leaders = pairs < d.experts ? pairs : d.experts;
-    const bool few = pairs <= FEW_PAIRS && few_lds(d) <= FEW_LDS && d.inter >= 8;
+    const bool few = pairs <= FEW_PAIRS && pairs * (d.inter_pad / 64) <= FEW_UNITS && d.inter >= 8;
     hipError_t e;
     if constexpr (RB == 1)
-        e = leaders * (d.inter_pad / 16) < 512 ? launch_up<TYPE, 1, 1>(s, d, leaders) : launch_up<TYPE, 2, 1>(s, d, leaders);
+        e = leaders * (d.inter_pad / 16) < 320 ? launch_up<TYPE, 1, 1>(s, d, leaders) : launch_up<TYPE, 2, 1>(s, d, leaders);
     else
         e = launch_up<TYPE, 2, RB>(s, d, leaders);
     if (e != hipSuccess) return e;
     if (few) {
-        experts16_few_kernel<TYPE><<<dim3((unsigned)((d.hidden + 15) / 16)), 64 * FEW_WAVES, few_lds(d), s>>>(d);
+        experts16_few_kernel<TYPE><<<dim3((unsigned)((d.hidden + 15) / 16)), 64 * FEW_WAVES, 0, s>>>(d);
         return hipGetLastError();
     }
     experts16_down_kernel<TYPE, RB>

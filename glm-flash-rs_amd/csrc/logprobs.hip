@@ -3,14 +3,19 @@
 //   log p(t) = z_t - m - log S,   H = log S - (sum of (z - m) exp(z - m)) / S
 // Masked logits (-inf, NaN) have probability 0; several of +inf share it equally.
 //
-// A row is cut into chunks of a workgroup each, whose logits stay in registers as they were loaded: their maximum first, then
-// the sums against it, so that the row is read once and nothing is rescaled. S is held as C, the number of logits that equal
-// the maximum, and R, the sum over the others: where one token has nearly all of the probability, log S = log(1 + R) keeps
-// what 1 + R would round off. A second launch joins a row's chunks.
+// A row of up to 32768 logits is a workgroup's, a longer one is cut into chunks of one each, which a second launch joins. A
+// chunk's logits stay in registers as they were loaded: their maximum first, then the sums against it, so that the row is read
+// once and nothing is rescaled. S is held as C, the number of logits that equal the maximum, and R, the sum over the others:
+// where one token has nearly all of the probability, log S = log(1 + R) keeps what 1 + R would round off.
 // The most likely tokens of a chunk: maxima of sets of its logits give a threshold that as many logits reach as are asked
-// for, and few more. These go to LDS, each counts those before it in the order
-// (larger logits first, the lower token first among equal ones), and that is its place. Where more reach it than LDS has
-// room for (rows of one value, rows in order), the places are filled one by one.
+// for, and few more. These go to LDS, each counts those before it in the order (larger logits first, the lower token first
+// among equal ones), and that is its place. Where more reach it than LDS has room for (rows of one value, a set far below the
+// others), the places are filled one by one.
+//
+// Bound: HBM, the logits read once; next to it VALU issue, six instructions and an exponential a logit (4096 rows of 160000
+// bf16 with 4 places 262 us, 5000 GB/s; without places 226, 5800; fp32 2048 rows 215, 6100). The threshold and the places are
+// what the difference is: a chain of two barriers and LDS for each of three workgroups a CU. Short calls are latency: 1 x 160000
+// with 20 places 13 us (two launches), 16 x 131072 10.3, 77 x 32003 10.1, 1 x 4000 5.2.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

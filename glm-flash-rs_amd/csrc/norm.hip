@@ -3,6 +3,13 @@
 // where a norm is  (z - mean) * 1 / sqrt(mean of squares + eps) * (weight + offset) + bias,  the mean 0 for the RMS kind.
 // post, the gate, the residual and pre may each be absent. Statistics and values in fp32, each output rounded once: pre
 // takes h as it is before its rounding. Variances are sums of squared differences from the mean, so that they don't cancel.
+//
+// Bound: HBM, each operand read and each output written once, the row in registers between. 16384 rows of 5120 (bf16 x and
+// gate, fp32 stream, both norms) 237 us, 4950 GB/s; 4096 of 4096 (bf16) 23.2, 5790; 65536 of 128 7.9, 4240, of which launch
+// and drain are about 3; one of 4096 2.9, two trips to memory. Which lanes hold a row follows its width alone, so that a
+// row's results do not depend on the window: 16 lanes up to 128 columns, a wave up to 512, else a workgroup with eight columns
+// a lane (with sixteen, half the threads, 16384 x 5120 took 384 us and not 265, one row 4.4 and not 3.4: fewer rows in flight
+// for the registers), sixteen over 8192, where eight would need more than 1024 threads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -57,123 +64,122 @@ __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
     const int lanes = L ? L : (int)blockDim.x, lane = L ? threadIdx.x % L : threadIdx.x, per = L ? 256 / L : 1;
     const bool ragged = d.n % 8;
     int side = 0;
+    // (a loop over rows kept every argument in scalar registers, 62 of which were spilled: 265 us and not 237)
     const int64_t row = d.first + (int64_t)blockIdx.x * per + (L ? threadIdx.x / L : 0);
     if (row >= d.rows) return;
-    {
-        int c[V], count[V];
-        Eight ex[V], er[V], eg[V];
-        float gate = 1.f;
-        if (d.gate && !d.gate_col) gate = load_one(d.gate, d.gate_type, row * d.gate_row);
+    int c[V], count[V];
+    Eight ex[V], er[V], eg[V];
+    float gate = 1.f;
+    if (d.gate && !d.gate_col) gate = load_one(d.gate, d.gate_type, row * d.gate_row);
+#pragma unroll
+    for (int g = 0; g < V; ++g) {
+        c[g] = 8 * (g * lanes + lane), count[g] = d.n - c[g];
+        ex[g].a = ex[g].b = er[g].a = er[g].b = eg[g].a = eg[g].b = make_uint4(0, 0, 0, 0);
+        if (count[g] > 0) {
+            ex[g] = load_some(d.x, d.x_type, row * d.x_stride + c[g], count[g]);
+            if (!LATE && d.residual) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
+            if (!LATE && d.gate && d.gate_col) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
+        }
+    }
+    f8_t v[V];
+#pragma unroll
+    for (int g = 0; g < V; ++g) v[g] = converted<T>(ex[g], d.x_type);
+    // columns past n hold zeros; a norm leaves what it adds to them out again
+    const auto clear = [&] {
 #pragma unroll
         for (int g = 0; g < V; ++g) {
-            c[g] = 8 * (g * lanes + lane), count[g] = d.n - c[g];
-            ex[g].a = ex[g].b = er[g].a = er[g].b = eg[g].a = eg[g].b = make_uint4(0, 0, 0, 0);
-            if (count[g] > 0) {
-                ex[g] = load_some(d.x, d.x_type, row * d.x_stride + c[g], count[g]);
-                if (!LATE && d.residual) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
-                if (!LATE && d.gate && d.gate_col) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
+            if (ragged) {
+                asm volatile("; by column");
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[g][j] = j < count[g] ? v[g][j] : 0.f;
+            } else {
+                asm volatile("; by group");
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[g][j] = count[g] > 0 ? v[g][j] : 0.f;
             }
         }
-        f8_t v[V];
+    };
+    const auto norm = [&](const NormPart& p) {
+        Eight ew[V], eb[V];
 #pragma unroll
-        for (int g = 0; g < V; ++g) v[g] = converted<T>(ex[g], d.x_type);
-        // columns past n hold zeros; a norm leaves what it adds to them out again
-        const auto clear = [&] {
-#pragma unroll
-            for (int g = 0; g < V; ++g) {
-                if (ragged) {
-                    asm volatile("; by column");
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] = j < count[g] ? v[g][j] : 0.f;
-                } else {
-                    asm volatile("; by group");
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] = count[g] > 0 ? v[g][j] : 0.f;
-                }
-            }
-        };
-        const auto norm = [&](const NormPart& p) {
-            Eight ew[V], eb[V];
-#pragma unroll
-            for (int g = 0; g < V; ++g) {
-                ew[g].a = ew[g].b = eb[g].a = eb[g].b = make_uint4(0, 0, 0, 0);
-                if (!LATE && count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
-                if (!LATE && count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
-            }
-            if (p.layer) {
-                float s = 0.f;
-#pragma unroll
-                for (int g = 0; g < V; ++g)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) s += v[g][j];
-                const float mean = total<L>(s, part[side ^= 1]) * d.per_column;
-#pragma unroll
-                for (int g = 0; g < V; ++g)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] -= mean;
-                clear();
-            }
+        for (int g = 0; g < V; ++g) {
+            ew[g].a = ew[g].b = eb[g].a = eb[g].b = make_uint4(0, 0, 0, 0);
+            if (!LATE && count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
+            if (!LATE && count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
+        }
+        if (p.layer) {
             float s = 0.f;
 #pragma unroll
             for (int g = 0; g < V; ++g)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s = fmaf(v[g][j], v[g][j], s);
-            const float r = __builtin_amdgcn_rsqf(total<L>(s, part[side ^= 1]) * d.per_column + p.eps);
-#pragma unroll
-            for (int g = 0; g < V; ++g) {
-                if (LATE && count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
-                if (LATE && count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
-                if (p.weight) {
-                    const f8_t w = converted<T>(ew[g], p.weight_type);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] = v[g][j] * r * (w[j] + p.offset);
-                } else {
-                    asm volatile("; no weight");
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] *= r;
-                }
-                if (p.bias) v[g] += converted<T>(eb[g], p.bias_type);  // (zeros past n)
-            }
-        };
-        if (d.has_post) norm(d.post);
-        if (d.gate) {
-            if (!d.gate_col && d.sigmoid) gate = times_logistic(1.f, gate);
-#pragma unroll
-            for (int g = 0; g < V; ++g) {
-                if (!d.gate_col) {
-                    asm volatile("; a gate a row");
-                    v[g] *= gate;
-                    continue;
-                }
-                if (LATE && count[g] > 0) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
-                f8_t b = converted<T>(eg[g], d.gate_type);
-                if (d.sigmoid) {
-                    asm volatile("; sigmoid");
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[j] = times_logistic(1.f, b[j]);
-                }
-                v[g] *= b;
-            }
-        }
-        if (d.h) {
-#pragma unroll
-            for (int g = 0; g < V; ++g) {
-                v[g] *= d.scale;
-                if (d.residual) {
-                    if (LATE && count[g] > 0) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
-                    const f8_t r = converted<T>(er[g], d.residual_type);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[g][j] = fmaf(d.residual_scale, r[j], v[g][j]);
-                }
-                if (count[g] > 0) store<T>(d.h, d.h_type, row * d.h_stride + c[g], v[g], count[g]);
-            }
-        }
-        if (d.y) {
-            norm(d.pre);
+                for (int j = 0; j < 8; ++j) s += v[g][j];
+            const float mean = total<L>(s, part[side ^= 1]) * d.per_column;
 #pragma unroll
             for (int g = 0; g < V; ++g)
-                if (count[g] > 0) store<T>(d.y, d.y_type, row * d.y_stride + c[g], v[g], count[g]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[g][j] -= mean;
+            clear();
         }
+        float s = 0.f;
+#pragma unroll
+        for (int g = 0; g < V; ++g)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf(v[g][j], v[g][j], s);
+        const float r = __builtin_amdgcn_rsqf(total<L>(s, part[side ^= 1]) * d.per_column + p.eps);
+#pragma unroll
+        for (int g = 0; g < V; ++g) {
+            if (LATE && count[g] > 0 && p.weight) ew[g] = load_some(p.weight, p.weight_type, c[g], count[g]);
+            if (LATE && count[g] > 0 && p.bias) eb[g] = load_some(p.bias, p.bias_type, c[g], count[g]);
+            if (p.weight) {
+                const f8_t w = converted<T>(ew[g], p.weight_type);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[g][j] = v[g][j] * r * (w[j] + p.offset);
+            } else {
+                asm volatile("; no weight");
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[g][j] *= r;
+            }
+            if (p.bias) v[g] += converted<T>(eb[g], p.bias_type);  // (zeros past n)
+        }
+    };
+    if (d.has_post) norm(d.post);
+    if (d.gate) {
+        if (!d.gate_col && d.sigmoid) gate = times_logistic(1.f, gate);
+#pragma unroll
+        for (int g = 0; g < V; ++g) {
+            if (!d.gate_col) {
+                asm volatile("; a gate a row");
+                v[g] *= gate;
+                continue;
+            }
+            if (LATE && count[g] > 0) eg[g] = load_some(d.gate, d.gate_type, row * d.gate_row + c[g], count[g]);
+            f8_t b = converted<T>(eg[g], d.gate_type);
+            if (d.sigmoid) {
+                asm volatile("; sigmoid");
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[j] = times_logistic(1.f, b[j]);
+            }
+            v[g] *= b;
+        }
+    }
+    if (d.h) {
+#pragma unroll
+        for (int g = 0; g < V; ++g) {
+            v[g] *= d.scale;
+            if (d.residual) {
+                if (LATE && count[g] > 0) er[g] = load_some(d.residual, d.residual_type, row * d.residual_stride + c[g], count[g]);
+                const f8_t r = converted<T>(er[g], d.residual_type);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[g][j] = fmaf(d.residual_scale, r[j], v[g][j]);
+            }
+            if (count[g] > 0) store<T>(d.h, d.h_type, row * d.h_stride + c[g], v[g], count[g]);
+        }
+    }
+    if (d.y) {
+        norm(d.pre);
+#pragma unroll
+        for (int g = 0; g < V; ++g)
+            if (count[g] > 0) store<T>(d.y, d.y_type, row * d.y_stride + c[g], v[g], count[g]);
     }
 }
 

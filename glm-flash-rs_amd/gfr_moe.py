@@ -395,8 +395,8 @@ _NORMS = {"rms": 1, "layer": 2}
 @dataclass
 class Norm:
     """A norm over a row's columns (gfr_norm): kind "rms" or "layer" (which takes the mean off first), then times
-    weight + offset and plus bias; weight and bias [n], bf16, fp16 or fp32 (None: 1 and 0). offset 1 is for weights that are
-    stored less one."""
+    weight + offset and plus bias; weight and bias [n], bf16, fp16 or fp32 (None: neither weight nor offset, no bias). offset
+    1 is for weights that are stored less one."""
 
     kind: str = "rms"
     weight: torch.Tensor = None
@@ -1165,7 +1165,9 @@ def _block_norm(x, residual, pre, post, gate, gate_activation, scale, residual_s
         if g.shape[0] not in (1, rows) or g.shape[1] not in (1, n):
             raise ValueError(f"gate {tuple(gate.shape)}: [n], [rows, 1], [1, n] or [rows, n] of ({rows}, {n})")
         gate_at, gate_type, gate_column = gate.data_ptr(), types[gate.dtype], int(g.shape[1] == n and n > 1)
-        gate_row = _row_stride(g) if g.shape[0] > 1 else 0
+        gate_row = _row_stride(g)              # (and that its columns are neighbours)
+        if g.shape[0] == 1:
+            gate_row = 0
     sigmoid = _GATE_ACTIVATIONS.get(gate_activation)
     if sigmoid is None:
         raise ValueError(f"gate activation {gate_activation!r} of ['none', 'sigmoid']")

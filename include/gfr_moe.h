@@ -387,7 +387,7 @@ int gfr_experts16_run(hipStream_t stream, const gfr_experts16* d);
  * a norm: (z - mean) / sqrt(mean of (z - mean)^2 + eps) * (weight + offset) + bias over a row's n columns, the mean 0 for
  * GFR_NORM_RMS; f the identity, or the logistic function. x, residual, gate, h, y, the weights and biases each in any of
  * GFR_BF16, GFR_F16, GFR_F32. post.kind GFR_NORM_NONE, gate, residual, weights and biases NULL: not there (a residual that
- * is not there is 0, a weight that is not there 1). h or y may be NULL, and y is exactly where pre.kind is not
+ * is not there is 0, a weight that is not there 1, whatever the offset). h or y may be NULL, and y is exactly where pre.kind is not
  * GFR_NORM_NONE. The gate's element of row r and column c is gate[r * gate_row + c * gate_column], gate_column 0 or 1,
  * gate_row 0 or any (at least n, or 1 where gate_column is 0). Values and statistics in fp32 (pre takes h before its rounding), one rounding an
  * output. Strides count elements; any size, stride and element-aligned address works. h and y may each be x or the residual

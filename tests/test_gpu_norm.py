@@ -162,6 +162,15 @@ def test_rows_by_themselves(gfr, n):
     assert torch.isnan(h2[7]).all() and torch.isnan(y2[7]).all()
 
 
+def test_gates_of_one_row(gfr):
+    """A gate that torch expands to all rows or columns is the row or column itself."""
+    n, rows = 300, 7
+    x, column, row = randn(1, rows, n), randn(2, n), randn(3, rows, 1)
+    for gate, same in ((column.expand(rows, n), column), (column.view(1, n), column), (row[:1].expand(rows, 1), row[:1]),
+                       (row[0, 0], row[:1]), (row, row.expand(rows, n).contiguous())):
+        assert torch.equal(gfr.block_norm(x, gate=gate)[0], gfr.block_norm(x, gate=same)[0])
+
+
 def test_rows_of_one_value(gfr):
     """No variance: the layer norm's bias alone; rows of zeros: zeros."""
     for n in (1, 5, 128, 1000, 9000):
@@ -212,6 +221,7 @@ def test_python_refusals(gfr):
     for bad in (dict(residual=x[:, :32]), dict(residual=x.double()), dict(gate=x[:3]), dict(gate=x.double()),
                 dict(gate=x, gate_activation="tanh"), dict(pre=gfr.Norm("l2")), dict(pre=gfr.Norm("rms", weight=x[0, :32])),
                 dict(pre=p, out=x[:, :32]), dict(pre=p, out_dtype=torch.float64), dict(out=x.clone()),
+                dict(gate=randn(4, 128)[::2]), dict(gate=randn(4, 1, 128)[:, ::2]),
                 dict(residual=x.cpu()), dict(pre=p, out=torch.empty_like(x), out_dtype=torch.float32), dict(gate=x.t())):
         with pytest.raises(ValueError):
             gfr.block_norm(x, **bad)
