@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
             v[g] *= b;
         }
     }
-    if (d.h) {
+    if (d.h || d.residual || d.scale != 1.f) {
 #pragma unroll
         for (int g = 0; g < V; ++g) {
             v[g] *= d.scale;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[g][j] = fmaf(d.residual_scale, r[j], v[g][j]);
             }
-            if (count[g] > 0) store<T>(d.h, d.h_type, row * d.h_stride + c[g], v[g], count[g]);
+            if (d.h && count[g] > 0) store<T>(d.h, d.h_type, row * d.h_stride + c[g], v[g], count[g]);
         }
     }
     if (d.y) {

@@ -162,6 +162,22 @@ def test_rows_by_themselves(gfr, n):
     assert torch.isnan(h2[7]).all() and torch.isnan(y2[7]).all()
 
 
+@pytest.mark.parametrize("n", [64, 300, 3000, 20000])
+def test_rows_without_the_stream(gfr, n):
+    """The C interface with h NULL: the same y, of the residual and the scales all the same."""
+    rows = 5
+    x, r, p = randn(1, rows, n), randn(2, rows, n), made(gfr, 3, n, "rms", torch.bfloat16)
+    for residual, scale, residual_scale in ((r, 0.5, 0.9), (None, 0.5, 1.0), (r, 1.0, 1.0), (None, 1.0, 1.0)):
+        want = gfr.block_norm(x, residual, pre=p, scale=scale, residual_scale=residual_scale)[1]
+        y = torch.empty_like(x)
+        call = gfr._BLOCK_NORM.pack(rows, n, 0, 0, 0, 0, 0, 0, 0, scale, residual_scale, x.data_ptr(), n,
+                                    0 if residual is None else residual.data_ptr(), n, 0, 0, 0, 0, y.data_ptr(), n,
+                                    *gfr._NO_NORM, *p.fields(n, torch.cuda.current_device()))
+        gfr._check(gfr.lib().gfr_block_norm_run(gfr._stream(), call))
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
 def test_gates_of_one_row(gfr):
     """A gate that torch expands to all rows or columns is the row or column itself."""
     n, rows = 300, 7
