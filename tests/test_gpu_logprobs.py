@@ -56,7 +56,7 @@ def reference(logits, tokens, top, temperature):
 def near(out, want, what):
     y, e = want
     assert out.dtype is torch.float32 and out.shape == y.shape, what
-    same = out.double() == y                                             # infinities
+    same = out == y.float()     # infinities, and what rounds to them: the lowest bf16 less the largest is -6.8e38, fp32's end 3.4e38
     off = torch.where(same, torch.zeros_like(y), (out.double() - y).abs())
     assert (off <= e).all(), f"{what}: off by {off.max().item():.3g}"
 
@@ -152,6 +152,26 @@ def test_masked(gfr, vocab, dtype):
         assert torch.allclose(alone.logprobs, got.logprobs[8:], rtol=1e-5, atol=1e-6)
     assert torch.isneginf(got.logprobs[0]).all() and got.entropy[0] == 0
     assert got.entropy[6] == 0 and got.logprobs[7, 0].item() == pytest.approx(-torch.log(torch.tensor(3.0)).item(), rel=1e-6)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(6, 4096), (1100, 3000), (6, 32768), (6, 70000)])
+def test_magnitudes(gfr, rows, vocab, dtype):
+    """Places where the logits' magnitudes lie far apart: whole columns of a few hundred at the lowest value or at -1e4, all
+    of one value but some, values near the largest and the lowest finite one, and next to +inf."""
+    dt = TYPES[dtype]
+    l = randn(vocab, rows, vocab, dt)
+    column = torch.arange(vocab, device="cuda")
+    l[0, column // 8 % 64 >= 40] = torch.finfo(dt).min
+    l[1, column // 8 % 64 >= 10] = -1e4
+    l[2] = 1.0
+    l[2, column % 701 == 3] = 2.0
+    l[3] = torch.where(column % 2 == 0, torch.finfo(dt).max, torch.finfo(dt).min)
+    l[4, column % 1009 == 5] = torch.inf
+    l[5] = l[5] * 1e-3
+    tokens = column[:40].repeat(rows, 1)
+    for top in (1, 4, 9, 20, 32):
+        check(gfr, l, tokens, top, 1.0, f"top {top}")
 
 
 def test_near_certain(gfr):
