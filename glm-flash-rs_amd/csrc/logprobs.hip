@@ -332,9 +332,11 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(LogprobsJob d) {
     if (i < d.top) r.masked(d, row, i);
 }
 
-// A row of at most 8 * 8 * 512 logits is one chunk, of the fewest groups that hold it: of 512 threads, or of 128 where there
-// are rows for every CU and they are short (us with 512 threads in two launches, in one, with 128: 8192 rows of 1000 118, 47,
-// 19; 8192 of 4000 without places -, 37, 18; 2000 of 8000 -, 18.3, 19.3; one of 4000 11.6, 5.2, 7.0).
+// A row of at most 8 * 8 * 512 logits is one chunk, of the fewest groups that hold it: of 512 threads, or of 128 or 256 where
+// there are rows for every CU, as long as 8 groups of a thread hold a row: more rows are under way at once, and barriers join
+// fewer waves (us with 512 threads in two launches, in one, with fewer: 8192 rows of 1000 118, 47, 19; 8192 of 4000 without
+// places -, 37, 18; 8192 of 8000 with 4 -, 57, 35; 4096 of 16000 with 32 -, 47, 41; 2000 of 8000 without -, 13.9, 11.2; one of
+// 4000 11.6, 5.2, 7.0. 16 groups of 256 threads for longer rows: 8192 of 32000 97 -> 90, but 1200 of them with 20 25.0 -> 25.8).
 constexpr int WIDE = 512, NARROW = 128, MOST = 8 * 8 * WIDE;
 
 template <int TYPE, int THREADS, int V>
@@ -353,9 +355,11 @@ hipError_t launch_chunks(hipStream_t s, const LogprobsJob& d) {
 template <int TYPE>
 hipError_t launch(hipStream_t s, const LogprobsJob& d, int groups) {
     if (d.chunks == 1) {
-        if (d.rows >= 1024 && d.vocab <= 32 * NARROW) {
+        if (d.rows >= 1024 && d.vocab <= 128 * NARROW) {
             if (d.vocab <= 8 * NARROW) return launch_rows<TYPE, NARROW, 1>(s, d);
-            return d.vocab <= 16 * NARROW ? launch_rows<TYPE, NARROW, 2>(s, d) : launch_rows<TYPE, NARROW, 4>(s, d);
+            if (d.vocab <= 16 * NARROW) return launch_rows<TYPE, NARROW, 2>(s, d);
+            if (d.vocab <= 32 * NARROW) return launch_rows<TYPE, NARROW, 4>(s, d);
+            return d.vocab <= 64 * NARROW ? launch_rows<TYPE, NARROW, 8>(s, d) : launch_rows<TYPE, 2 * NARROW, 8>(s, d);
         }
         if (d.vocab <= 8 * WIDE) return launch_rows<TYPE, WIDE, 1>(s, d);
         if (d.vocab <= 16 * WIDE) return launch_rows<TYPE, WIDE, 2>(s, d);

@@ -101,7 +101,7 @@ def test_logprobs(gfr, vocab):
         check(gfr, l, tokens, top, rng.choice([1.0, 0.7, 1.3]), f"rows {rows} vocab {vocab} top {top} {dtype}")
 
 
-@pytest.mark.parametrize("vocab", [5, 1000, 1024, 1025, 2048, 2049, 4095, 4096, 4097, 9000])
+@pytest.mark.parametrize("vocab", [5, 1000, 1024, 1025, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 9000, 16384, 16385])
 def test_many_rows(gfr, vocab):
     """Windows of more rows than CUs hold, in every form that they take."""
     for dtype in TYPES.values():
@@ -155,7 +155,7 @@ def test_masked(gfr, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("rows,vocab", [(6, 4096), (1100, 3000), (6, 32768), (6, 70000)])
+@pytest.mark.parametrize("rows,vocab", [(6, 4096), (1100, 3000), (1030, 8000), (1030, 16000), (6, 32768), (6, 70000)])
 def test_magnitudes(gfr, rows, vocab, dtype):
     """Places where the logits' magnitudes lie far apart: whole columns of a few hundred at the lowest value or at -1e4, all
     of one value but some, values near the largest and the lowest finite one, and next to +inf."""
