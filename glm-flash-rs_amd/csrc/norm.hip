@@ -5,7 +5,7 @@
 // takes h as it is before its rounding. Variances are sums of squared differences from the mean, so that they don't cancel.
 //
 // Bound: HBM, each operand read and each output written once, the row in registers between. 16384 rows of 5120 (bf16 x and
-// gate, fp32 stream, both norms) 237 us, 4950 GB/s; 4096 of 4096 (bf16) 23.2, 5790; 65536 of 128 7.9, 4240, of which launch
+// gate, fp32 stream, both norms) 237 us, 4950 GB/s; 4096 of 4096 (bf16) 23.2, 5790; 65536 of 128 7.1, 4730, of which launch
 // and drain are about 3; one of 4096 2.9, two trips to memory. Which lanes hold a row follows its width alone, so that a
 // row's results do not depend on the window: 16 lanes up to 128 columns, a wave up to 512, else a workgroup with eight columns
 // a lane (with sixteen, half the threads, 16384 x 5120 took 384 us and not 265, one row 4.4 and not 3.4: fewer rows in flight
@@ -16,6 +16,9 @@
 #include "lanes.hpp"
 #include "launch.hpp"
 #include "values.hpp"
+
+// products and sums are rounded as they are written, so that a row has the same bits from either kernel
+#pragma clang fp contract(off)
 
 namespace gfr {
 namespace {
@@ -183,6 +186,66 @@ __global__ void __launch_bounds__(L ? 256 : 1024) norm_kernel(NormJob d) {
     }
 }
 
+// The norm alone, y = pre(x), of many rows: a workgroup keeps the weight and the bias in registers, takes rows in turn and asks
+// for the next while it works on one; the kernel above has one load a lane under way and waits for its sums. Columns lie as
+// above, and sums are in the same order. (us, above -> here: 16384 x 4096 bf16 60.3 -> 43.6, 6150 GB/s; its layer norm 74.6 ->
+// 49; 15935 x 4264 fp16 with an fp32 weight 85 -> 51; 16384 x 8192 165 -> 98; 65536 x 128 8.0 -> 7.1; 1200 x 4096 7.1 -> 6.4. With
+// scale, residual and h in it, registers spill: 16384 x 4096 94 -> 102, 5120 with an fp32 stream 182 -> 241.)
+template <int T, int L>
+__global__ void __launch_bounds__(L ? 256 : 1024, 8) norm_rows_kernel(NormJob d) {
+    __shared__ float part[2][16];
+    const int lanes = L ? L : (int)blockDim.x, lane = L ? threadIdx.x % L : threadIdx.x, per = L ? 256 / L : 1;
+    const NormPart& p = d.pre;
+    const int c = 8 * lane, count = d.n - c;
+    const int64_t step = (int64_t)gridDim.x * per;
+    int side = 0;
+    int64_t row = (int64_t)blockIdx.x * per + (L ? threadIdx.x / L : 0);
+    if (row >= d.rows) return;
+    Eight ex;
+    ex.a = ex.b = make_uint4(0, 0, 0, 0);
+    const auto ask = [&](int64_t at) {
+        if (count > 0) ex = load_some(d.x, d.x_type, at * d.x_stride + c, count);
+    };
+    ask(row);
+    f8_t w = 1.f, b = -0.f;                                           // (-0 leaves a -0 as it is)
+    if (count > 0 && p.weight) w = converted<T>(load_some(p.weight, p.weight_type, c, count), p.weight_type) + p.offset;
+    if (count > 0 && p.bias) b = converted<T>(load_some(p.bias, p.bias_type, c, count), p.bias_type);
+    while (true) {
+        f8_t v = converted<T>(ex, d.x_type);
+        const int64_t next = row + step < d.rows ? row + step : row;
+        ask(next);
+        if (p.layer) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+            const float mean = total<L>(s, part[side ^= 1]) * d.per_column;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < count ? v[j] - mean : 0.f;
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(v[j], v[j], s);
+        const float root = __builtin_amdgcn_rsqf(total<L>(s, part[side ^= 1]) * d.per_column + p.eps);
+        if (count > 0) store<T>(d.y, d.y_type, row * d.y_stride + c, v * root * w + b, count);
+        if (next == row) return;
+        row = next;
+    }
+}
+
+// The rows of more threads than the card holds at once.
+constexpr int RESIDENT = 256 * 2048;
+bool alone(const NormJob& d) {
+    return d.n <= 8192 && (int64_t)d.rows * d.n >= (int64_t)8 * RESIDENT && d.y && !d.has_post && !d.gate && !d.residual && !d.h &&
+           d.scale == 1.f;
+}
+template <int T, int L>
+hipError_t launch_rows(hipStream_t s, const NormJob& d) {
+    const int threads = L ? 256 : (d.n + 511) / 512 * 64, per = L ? 256 / L : 1;
+    const int64_t groups = ((int64_t)d.rows + per - 1) / per, most = 256 * (2048 / threads);
+    norm_rows_kernel<T, L><<<dim3((unsigned)(groups < most ? groups : most)), threads, 0, s>>>(d);
+    return hipGetLastError();
+}
+
 template <int T, int L, int V>
 hipError_t launch(hipStream_t s, NormJob d) {
     const int lanes = (d.n + 8 * V - 1) / (8 * V), threads = L ? 256 : (lanes + 63) / 64 * 64, per = L ? 256 / L : 1;
@@ -196,6 +259,11 @@ hipError_t launch(hipStream_t s, NormJob d) {
 }
 template <int T>
 hipError_t launch(hipStream_t s, const NormJob& d) {
+    if constexpr (T != ANY)
+        if (alone(d)) {
+            if (d.n <= 128) return launch_rows<T, 16>(s, d);
+            return d.n <= 512 ? launch_rows<T, 64>(s, d) : launch_rows<T, 0>(s, d);
+        }
     if (d.n <= 128) return launch<T, 16, 1>(s, d);
     if (d.n <= 512) return launch<T, 64, 1>(s, d);
     if (d.n <= 8192) return launch<T, 0, 1>(s, d);

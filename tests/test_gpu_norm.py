@@ -257,3 +257,41 @@ def test_more_rows_than_a_launch_holds(gfr):
     y = gfr.norm(x, p)
     for part in (slice(0, 5), slice(rows - 7, rows)):
         assert torch.equal(y[part], gfr.norm(x[part].contiguous(), p))
+
+
+def test_more_rows_with_the_stream(gfr):
+    """The same with a residual, whose rows are a launch's by themselves."""
+    rows, n = (1 << 21) + 3, 520
+    x, r = [torch.randn((rows, n), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    p = made(gfr, 1, n, "rms", torch.bfloat16)
+    h, y = gfr.block_norm(x, r, pre=p)
+    for part in (slice(0, 5), slice(rows - 7, rows)):
+        h1, y1 = gfr.block_norm(x[part].contiguous(), r[part].contiguous(), pre=p)
+        assert torch.equal(h[part], h1) and torch.equal(y[part], y1)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("n", [9, 120, 127, 128, 129, 500, 512, 513, 1001, 4100, 5120, 8191, 8192])
+def test_many_rows(gfr, n, kind):
+    """The norm of more rows than the card holds at once: the bits of windows of few, which the reference judges, from slices
+    between NaN, in place, with and without a weight and a bias, and rows with NaN or infinities by themselves."""
+    least = -(-8 * 256 * 2048 // n)
+    for rows, dtype, weight, out in ((least, torch.bfloat16, torch.float32, torch.bfloat16),
+                                     (least + 77, torch.float16, torch.float16, torch.float32),
+                                     (3 * least + 1, torch.float32, torch.bfloat16, torch.bfloat16),
+                                     (least, torch.float16, None, torch.float16)):
+        p = made(gfr, n, n, kind, weight, 1.0)
+        wide = torch.full((rows, n + 5), float("nan"), dtype=dtype, device="cuda")
+        x = wide[:, 3:3 + n]
+        x.copy_(torch.randn((rows, n), dtype=torch.float32, device="cuda"))
+        x[least // 2, n // 2], x[least // 3, 0] = float("nan"), float("inf")
+        y = gfr.norm(x, p, out_dtype=out)
+        few = torch.cat([gfr.norm(part, p, out_dtype=out) for part in x.split(min(8 * 256 * 2048 // n, least // 3 + 1))])
+        keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+        keep[[least // 2, least // 3]] = False
+        assert torch.equal(y[keep], few[keep]) and torch.isnan(y[least // 2]).all() and not torch.isfinite(y[least // 3]).all()
+        some = x[rows - 200:].double()
+        check(y[rows - 200:], norm64(some, torch.zeros_like(some), p), f"rows {rows} n {n}")
+        if out is dtype:
+            assert gfr.norm(x, p, out=x) is x and torch.equal(x[keep], y[keep])
+            assert torch.isnan(wide[:, :3]).all() and torch.isnan(wide[:, 3 + n:]).all()
