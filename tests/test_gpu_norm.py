@@ -273,7 +273,7 @@ def test_more_rows_with_the_stream(gfr):
 @pytest.mark.parametrize("kind", ["rms", "layer"])
 @pytest.mark.parametrize("n", [9, 120, 127, 128, 129, 500, 512, 513, 1001, 4100, 5120, 8191, 8192])
 def test_many_rows(gfr, n, kind):
-    """The norm of more rows than the card holds at once: the bits of windows of few, which the reference judges, from slices
+    """The norm of more rows than the card holds at once: the bits of windows of few, and the formula's values, from slices
     between NaN, in place, with and without a weight and a bias, and rows with NaN or infinities by themselves."""
     least = -(-8 * 256 * 2048 // n)
     for rows, dtype, weight, out in ((least, torch.bfloat16, torch.float32, torch.bfloat16),
