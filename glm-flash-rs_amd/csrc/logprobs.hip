@@ -12,8 +12,8 @@
 // among equal ones), and that is its place. Where more reach it than LDS has room for (rows of one value, a set far below the
 // others), the places are filled one by one.
 //
-// Bound: HBM, the logits read once; next to it VALU issue, 15 instructions a logit, half of them a chunk's fixed part (4096 rows
-// of 160000 bf16 with 4 places 247 us, 5300 GB/s; without places 226, 5800; fp32 2048 rows 215, 6100). The threshold and the
+// Bound: HBM, the logits read once; next to it VALU issue, 16 instructions a logit, half of them a chunk's fixed part (4096 rows
+// of 160000 bf16 with 4 places 264 us, 4960 GB/s; without places 232, 5640; fp32 2048 rows 212, 6180). The threshold and the
 // places are what the difference is: a chain of two barriers and LDS for each of three workgroups a CU. Short calls are latency: 1 x 160000
 // with 20 places 13 us (two launches), 16 x 131072 10.2, 77 x 32003 9.0, 1 x 4000 5.2.
 #include <hip/hip_runtime.h>
@@ -182,13 +182,10 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
     const float M = max_over(64, set);
     const float least = d.top ? threshold(set, M, d.top) : 0.f;
 
-    // exp(z) = exp2(l k + c) with c = -M k: c's rounding is a factor of all terms, taken out of the sums afterwards. slope
-    // is summed in units of the exponent.
-    // Where M k is no finite number all others are too far below M to count (their distance is at least 2^-24 of M), or
-    // there are none.
-    const bool finite = fabsf(M * d.by) < INFINITY;
-    const float k = finite ? d.by : 0.f, c = finite ? -M * k : -1e30f, off = finite ? fmaf(-M, k, -c) : 0.f;
-    const auto exponent = [&](float l) { return fmaxf(fmaf(l, k, c), -1e30f); };   // -1e30: masked, and exp2 of it is 0
+    // exp(z) = exp2((l - M) by): the distance from the largest logit is taken first, one rounding of it, so that a term's error
+    // goes by |z| and not by M. (l by - M by in one instruction less has M by's rounding in every term: for M by of 1e3 1e-4 of it.)
+    // slope is summed in logits.
+    const auto distance = [&](float l) { return fmaxf(l - M, -1e30f); };   // -1e30: masked (and NaN), exp2 of it is 0
     float rest = 0.f, slope = 0.f, count = 0.f;
 #pragma unroll
     for (int g = 0; g < V; ++g) {
@@ -197,7 +194,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
             const f8_t l = fresh<TYPE>(raw[g]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float x = exponent(l[j]), e = __builtin_amdgcn_exp2f(x);
+                const float x = distance(l[j]), e = __builtin_amdgcn_exp2f(x * d.by);
                 if (l[j] == M) count += 1.f;
                 else rest += e, slope = fmaf(x, e, slope);
             }
@@ -206,7 +203,7 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
             const f8_t l = fresh<TYPE>(raw[g]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float x = exponent(l[j]), e = __builtin_amdgcn_exp2f(x);
+                const float x = distance(l[j]), e = __builtin_amdgcn_exp2f(x * d.by);
                 rest += e, slope = fmaf(x, e, slope);
             }
             asm volatile("; another group" : "+v"(rest), "+v"(slope));
@@ -234,8 +231,6 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
     if (ONE || tid < WAVES) {
         const int w = lane & (WAVES - 1);
         s.count = sum_over(WAVES, sums[w][2]), s.rest = sum_over(WAVES, sums[w][0]), s.slope = sum_over(WAVES, sums[w][1]);
-        const float right = __builtin_amdgcn_exp2f(-off);
-        s.rest *= right, s.slope *= right / d.by;
     }
     Row r;
     uint64_t* out = nullptr;

@@ -436,7 +436,7 @@ int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d);
  * all fp32 but the ids. Masked logits (-inf, NaN) have probability 0 and log p -inf; they are among the top only where the
  * row has fewer others, by lower token. Several logits of +inf share the probability. A row of masked logits only: -inf,
  * entropy 0. logits in GFR_BF16, GFR_F16 or GFR_F32, rows of any stride and element-aligned address; sums in fp32, log p
- * within a few units of 32 bits also where it is near 0. A row's results depend on no other row; its last bits may on the
+ * within a few units of 32 bits wherever the logits lie, also where it is near 0. A row's results depend on no other row; its last bits may on the
  * number of rows, which the order of its sums follows (the tokens' order does not). tokens or top may be 0; top <= 32 and
  * vocab, vocab <= 2^21, temperature 1e-6 .. 1e6, at least one row.
  * workspace: gfr_logprobs_workspace(rows, vocab, top) bytes of device memory (0 for vocab <= 32768; NULL then), 8-byte
