@@ -113,9 +113,10 @@ __device__ __forceinline__ float threshold(float set, float most, int top) {
 // A row's results from its sums: the entropy, the tokens' log probabilities (thread `from` of `threads` on), a place's.
 struct Row {
     float most, log_sum;
+    // (halves: the difference of two finite logits may pass the range where its quotient does not)
     __device__ __forceinline__ float log_p(const LogprobsJob& d, float l) const {
         if (!(l > -INFINITY)) return -INFINITY;
-        return (l == most ? 0.f : (l - most) / d.temperature) - log_sum;
+        return (l == most ? 0.f : 2.f * ((0.5f * l - 0.5f * most) / d.temperature)) - log_sum;
     }
     __device__ __forceinline__ void tokens(const LogprobsJob& d, int row, int from, int threads) const {
         for (int i = from; i < d.tokens; i += threads) {

@@ -124,3 +124,21 @@ def test_finite_far_values(gfr, temperature, dtype):
         l = torch.stack(lines).cuda()
         t = torch.tensor([[0, vocab // 3, vocab // 4, vocab - 1]]).repeat(len(lines), 1).cuda()
         check(gfr, l, t, 5, temperature, f"vocab {vocab}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("temperature", [1.5, 4.0, 1e6])
+def test_differences_beyond_32_bits(gfr, temperature, dtype):
+    """Logits whose difference passes the range of 32 bits and whose difference over the temperature does not: no infinity."""
+    dt = TYPES[dtype]
+    big = torch.finfo(dt).max
+    for vocab in (40, 5000, 70000):
+        l = torch.zeros((3, vocab), dtype=dt)
+        l[0, 3], l[0, 5] = big, -big
+        l[1] = -big
+        l[1, 3] = 0.75 * big
+        l[2, 3], l[2, 4], l[2, 5] = big, -0.7 * big, -torch.inf
+        t = torch.tensor([[3, 4, 5, 0]]).repeat(3, 1).cuda()
+        check(gfr, l.cuda(), t, 5, temperature, f"vocab {vocab}")
+        if temperature > 2:
+            assert torch.isfinite(gfr.token_logprobs(l.cuda(), t, temperature=temperature).logprobs[:2]).all()
