@@ -2,8 +2,10 @@
 //   g, u   = the halves of gu[e] x[r];  a = act(min(g, limit)) * clamp(u, -limit, limit)
 //   out[r] = residual[r] + sum over s of weights[r][s] * down[e] a       (slots in order; picks outside [0, experts): none)
 // x, gu and down in bf16 or fp16; sums, activations and weights in fp32, one rounding at the end. Between the two products
-// the activations are held as the sum of two 16-bit values, 16 bits of them or more, which costs the matrix core a second
-// pass over the same weights in registers.
+// the activations are held as two 16-bit values, which costs the matrix core a second pass over the same weights in
+// registers: as h + l in bf16, 16 bits of them; as 2 h + l / 1024 in fp16, 22 bits or 2^-35 where that is more, up to twice its
+// range. (2 h leaves 2^-11 of an activation or 2^-24, so that l is in range, and most of what is below fp16's least values is in
+// it; with h + l that was lost, 2^-25, which left 12 bits of 1e-4.) The two parts' sums meet once a chunk.
 //
 // Bound: HBM, the weights of the experts that are picked, read once. A workgroup takes one expert's share of the columns and
 // all the rows that picked it, in passes of up to 16 RB, so that an expert's weights are read once however many rows pick it
@@ -27,6 +29,12 @@ namespace gfr {
 namespace {
 
 constexpr int PASS = 64;                                             // a pass's members at most
+
+// What an activation's two parts are in units of.
+template <int TYPE>
+constexpr float HIGH = TYPE == TYPE_BF16 ? 1.f : 2.f;
+template <int TYPE>
+constexpr float LOW = TYPE == TYPE_BF16 ? 1.f : 1.f / 1024;
 
 // The members of an expert: the pairs (by number) whose pick it is, in order; first and their count over all, and those from
 // number `from` on, up to `room` of them, in LDS. Called by the whole workgroup (waves of it, at most 16).
@@ -227,11 +235,9 @@ __device__ __forceinline__ void up_pass(const Experts16Job& d, const Weights<TYP
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float x = col + e < d.inter ? v[e] : 0.f;           // (columns up to a multiple of 64 are read)
-            hi[e] = f_to_16(x, TYPE);
-            // (up to twice fp16's range the second value holds what is above the first's)
-            if (TYPE == TYPE_F16 && fabsf(x) > 65504.f && fabsf(x) <= 131008.f) hi[e] = x > 0.f ? 0x7bff : 0xfbff;
-            const float h = TYPE == TYPE_BF16 ? bf16_to_f(hi[e]) : f16_to_f(hi[e]);
-            lo[e] = fabsf(h) < INFINITY ? f_to_16(x - h, TYPE) : 0;
+            hi[e] = f_to_16(x / HIGH<TYPE>, TYPE);
+            const float h = HIGH<TYPE> * (TYPE == TYPE_BF16 ? bf16_to_f(hi[e]) : f16_to_f(hi[e]));
+            lo[e] = fabsf(h) < INFINITY ? f_to_16((x - h) / LOW<TYPE>, TYPE) : 0;
         }
         uint16_t* to = d.acts + (int64_t)m.pair[16 * j + row] * 2 * d.inter_pad + col;
         *reinterpret_cast<uint2*>(to) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
@@ -274,10 +280,19 @@ __global__ void __launch_bounds__(64 * UP_WAVES, RB == 1 ? 4 : 2) experts16_up_k
 // (146 registers, three waves a SIMD; held to four, with registers spilled, 12 rows took 161 us and not 148)
 constexpr int DOWN_WAVES = 4, DOWN_TILES = 2, DOWN_COLS = 16 * DOWN_TILES * DOWN_WAVES;
 
-// A tile's sum over a chunk, in an order that both forms of the product share (each adds the chunks' sums in turn).
+// A tile's sum over a chunk in units of HIGH, in an order that both forms of the product share (each adds the chunks' sums in
+// turn).
 template <int TYPE>
 __device__ __forceinline__ f4_t chunk_sum(uint4 w0, uint4 w1, const uint4 (&x)[2][2]) {
-    f4_t v = mfma<TYPE>(w0, x[0][0], (f4_t){0.f, 0.f, 0.f, 0.f});
+    const f4_t none = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (LOW<TYPE> != HIGH<TYPE>) {
+        f4_t high = mfma<TYPE>(w0, x[0][0], none), low = mfma<TYPE>(w0, x[0][1], none);
+        high = mfma<TYPE>(w1, x[1][0], high), low = mfma<TYPE>(w1, x[1][1], low);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) high[j] = fmaf(low[j], LOW<TYPE> / HIGH<TYPE>, high[j]);
+        return high;
+    }
+    f4_t v = mfma<TYPE>(w0, x[0][0], none);
     v = mfma<TYPE>(w0, x[0][1], v);
     v = mfma<TYPE>(w1, x[1][0], v);
     return mfma<TYPE>(w1, x[1][1], v);
@@ -344,7 +359,7 @@ __device__ __forceinline__ void down_pass(const Experts16Job& d, const Weights<T
 #pragma unroll
         for (int i = 0; i < EB; ++i) {
             const int col = c0 + 16 * i + 4 * q;
-            if (col < d.hidden) *reinterpret_cast<f4_t*>(y + col) = acc[i][j];
+            if (col < d.hidden) *reinterpret_cast<f4_t*>(y + col) = acc[i][j] * HIGH<TYPE>;
         }
     }
 }
@@ -507,7 +522,7 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) experts16_few_kernel(Experts16
         f4_t v = {0.f, 0.f, 0.f, 0.f};
         if (there[threadIdx.x >> 2])
             for (int i = 0; i < chunks; ++i) v += parts[((threadIdx.x >> 2) * chunks + i) * 4 + (threadIdx.x & 3)];
-        sums[threadIdx.x] = v;
+        sums[threadIdx.x] = v * HIGH<TYPE>;
     }
     __syncthreads();
     if (my_row < d.rows) {

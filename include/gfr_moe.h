@@ -350,8 +350,8 @@ int gfr_dense_form(const gfr_dense* d);
  * [rows][slots] as gfr_route_gate gives them (a shared expert is the last of the stacks, its id `routed`); out and residual
  * in `type` or GFR_F32, residual may be NULL. A pick outside [0, experts) adds nothing: a row padded with -1 gets its
  * residual, or zeros. Picks of a row may repeat, each counts. Sums, activations and weights in fp32, the activations kept
- * to 16 bits or more between the products (with fp16 weights, beyond 131008 they are infinite), one rounding to out's
- * type. A row's result depends neither on the other rows nor on how many there are. The weights of the picked experts are
+ * between the products to 16 bits (bf16 weights), or to 22 bits or 2^-35, whichever is more (fp16 weights; above 131008 they
+ * may be infinite), one rounding to out's type. A row's result depends neither on the other rows nor on how many there are. The weights of the picked experts are
  * read once for 64 rows of theirs (for 16 in windows of up to 16 rows): meant for windows in which an expert has few.
  * Any size, stride and element-aligned address works, rows at 16-byte aligned addresses are the fast ones. residual may be
  * out itself (address, type and stride); an out that shares memory with an operand in any other way is refused.
