@@ -9,7 +9,10 @@
 // and drain are about 3; one of 4096 2.9, two trips to memory. Which lanes hold a row follows its width alone, so that a
 // row's results do not depend on the window: 16 lanes up to 128 columns, a wave up to 512, else a workgroup with eight columns
 // a lane (with sixteen, half the threads, 16384 x 5120 took 384 us and not 265, one row 4.4 and not 3.4: fewer rows in flight
-// for the registers), sixteen over 8192, where eight would need more than 1024 threads.
+// for the registers), sixteen over 8192, where eight would need more than 1024 threads, and 32 over 16384, whose operands but x
+// are loaded where they are used (registers hold one row). The wide forms have fewer rows under way: the norm alone of 8192 x
+// 8200 bf16 88 us, 3040 GB/s, of 8192 x 12288 104, 3870, of 4096 x 16384 65, 4100, of 4096 x 20000 121, 2710, of 4096 x 32768 175,
+// 3070; with an fp32 stream 4096 x 16384 156, 5160, 4096 x 32768 354, 4550; 16 rows of 16384 5.1, of 32768 10.7.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(L ? 256 : 1024, 8) norm_rows_kernel(NormJob d)
     }
 }
 
-// The rows of more threads than the card holds at once.
+// The rows of more threads than the card holds at once; up to what 1024 threads hold at eight columns each.
 constexpr int RESIDENT = 256 * 2048;
 bool alone(const NormJob& d) {
     return d.n <= 8192 && (int64_t)d.rows * d.n >= (int64_t)8 * RESIDENT && d.y && !d.has_post && !d.gate && !d.residual && !d.h &&
