@@ -390,9 +390,8 @@ int gfr_experts16_run(hipStream_t stream, const gfr_experts16* d);
  * is not there is 0, a weight that is not there 1, whatever the offset). h or y may be NULL, and y is exactly where pre.kind is not
  * GFR_NORM_NONE. The gate's element of row r and column c is gate[r * gate_row + c * gate_column], gate_column 0 or 1,
  * gate_row 0 or any (at least n, or 1 where gate_column is 0). Values and statistics in fp32 (pre takes h before its
- * rounding; squares of values beyond 1e19 pass its range, and those of values below 1e-19 fall under it: rows of nothing
- * larger need an eps of at least 1e-36), one rounding an output. Strides count elements; any size, stride and
- * element-aligned address works. h and y may each be x or the residual itself (address, type and stride); one that
+ * rounding; squares of values beyond 1e19 pass its range, and rows whose root mean square is below 1e-18 need an eps of at
+ * least 1e-36), one rounding an output. Strides count elements; any size, stride and element-aligned address works. h and y may each be x or the residual itself (address, type and stride); one that
  * shares memory with another operand, or with the other, in any other way is refused. A row's results do not depend on the
  * other rows, nor on how many there are. No scratch: calls may overlap on any streams. At least one row; n from 1 to 32768,
  * eps >= 0, scales finite. */
