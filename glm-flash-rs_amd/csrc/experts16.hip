@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(64 * UP_WAVES, RB == 1 ? 4 : 2) experts16_up_k
 }
 
 // ---- down ---------------------------------------------------------------------------------------------------------
-// (146 registers, three waves a SIMD; held to four, with registers spilled, 12 rows took 161 us and not 148)
+// (bounds of three waves a SIMD, 123 registers; held to four when it had 146, with registers spilled, 12 rows took 161 us and
+// not 148)
 constexpr int DOWN_WAVES = 4, DOWN_TILES = 2, DOWN_COLS = 16 * DOWN_TILES * DOWN_WAVES;
 
 // A tile's sum over a chunk in units of HIGH, in an order that both forms of the product share (each adds the chunks' sums in

@@ -12,7 +12,7 @@
 // among equal ones), and that is its place. Where more reach it than LDS has room for (rows of one value, a set far below the
 // others), the places are filled one by one.
 //
-// Bound: HBM, the logits read once; next to it VALU issue, 16 instructions a logit, half of them a chunk's fixed part (4096 rows
+// Bound: HBM, the logits read once; next to it VALU issue, 15 instructions a logit, half of them a chunk's fixed part (4096 rows
 // of 160000 bf16 with 4 places 264 us, 4960 GB/s; without places 232, 5640; fp32 2048 rows 212, 6180). The threshold and the
 // places are what the difference is: a chain of two barriers and LDS for each of three workgroups a CU. Short calls are latency: 1 x 160000
 // with 20 places 13 us (two launches), 16 x 131072 10.2, 77 x 32003 9.0, 1 x 4000 5.2.
