@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(THREADS) logprobs_chunk_kernel(LogprobsJob d) 
     const float least = d.top ? threshold(set, M, d.top) : 0.f;
 
     // exp(z) = exp2((l - M) by): the distance from the largest logit is taken first, one rounding of it, so that a term's error
-    // goes by |z| and not by M. (l by - M by in one instruction less has M by's rounding in every term: for M by of 1e3 1e-4 of it.)
-    // slope is summed in logits.
+    // goes by |z| and not by M. (A fused l by - M by, one instruction less, has the rounding of M by in every term: at M / T of
+    // 1000 up to 4e-5 of it, and beyond 1e9 no small factor.) slope is summed in logits.
     const auto distance = [&](float l) { return fmaxf(l - M, -1e30f); };   // -1e30: masked (and NaN), exp2 of it is 0
     float rest = 0.f, slope = 0.f, count = 0.f;
 #pragma unroll

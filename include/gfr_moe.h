@@ -351,10 +351,10 @@ int gfr_dense_form(const gfr_dense* d);
  * in `type` or GFR_F32, residual may be NULL. A pick outside [0, experts) adds nothing: a row padded with -1 gets its
  * residual, or zeros. Picks of a row may repeat, each counts. Sums, activations and weights in fp32, the activations kept
  * between the products to 16 bits (bf16 weights), or to 22 bits or 2^-35, whichever is more (fp16 weights; above 131008 they
- * may be infinite), one rounding to out's type. A row's result depends neither on the other rows nor on how many there are. The weights of the picked experts are
- * read once for 64 rows of theirs (for 16 in windows of up to 16 rows): meant for windows in which an expert has few. In
- * longer ones the results are as right, but the time grows with every further 64 (2048 rows of 8 in 160 experts of 4096 ->
- * 1408 6.5 ms, 512 rows 1.6).
+ * may be infinite), one rounding to out's type. A row's result depends neither on the other rows nor on how many there are.
+ * The weights of the picked experts are read once for 64 rows of theirs (for 16 in windows of up to 16 rows): meant for
+ * windows in which an expert has few. In longer ones the results are as right, but the time grows with every further 64
+ * (2048 rows of 8 in 160 experts of 4096 -> 1408 6.5 ms, 512 rows 1.6).
  * Any size, stride and element-aligned address works, rows at 16-byte aligned addresses are the fast ones. residual may be
  * out itself (address, type and stride); an out that shares memory with an operand in any other way is refused.
  * workspace: gfr_experts16_workspace(rows, slots, hidden, inter) bytes of device memory, 16-byte aligned, that are the
@@ -443,8 +443,8 @@ int gfr_block_norm_run(hipStream_t stream, const gfr_block_norm* d);
  * the order of its sums follows (the tokens' order does not). tokens or top may be 0; top <= 32 and vocab, vocab <= 2^21,
  * temperature 1e-6 .. 1e6, at least one row.
  * workspace: gfr_logprobs_workspace(rows, vocab, top) bytes of device memory (0 for vocab <= 32768; NULL then), 8-byte
- * aligned, that are the call's until its work is done: two calls that may overlap, or two captured graphs that may, take two workspaces. Outputs
- * and the workspace must not share memory with anything else. */
+ * aligned, that are the call's until its work is done: two calls that may overlap, or two captured graphs that may, take two
+ * workspaces. Outputs and the workspace must not share memory with anything else. */
 typedef struct gfr_logprobs {
     int rows, vocab, tokens, top;
     int type;
